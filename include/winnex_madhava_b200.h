@@ -331,6 +331,130 @@ mdh_status mdh_ivf_search_f32(mdh_ivf_f32* index, const float* host_queries, int
                               int32_t* out_ids, double* out_scores, mdh_stats* stats);
 mdh_status mdh_ivf_destroy_f32(mdh_ivf_f32* index);
 
+/* ---------------------------------------------------------------- operators around the search
+ * What makes the rows that an index holds and what reads the rows that a
+ * search found: layer norm, a linear layer, a cache of 8-bit rows, and
+ * attention over found rows.  No counterpart in the reference (its vectors
+ * come from elsewhere and its ids go elsewhere).
+ *
+ * Every buffer is device memory of the current device; the calls enqueue on
+ * `stream` (a cudaStream_t, NULL = the default stream) and return without
+ * waiting.  They allocate nothing: where scratch is needed the caller passes
+ * `ws` of at least the *_workspace() bytes, 16-byte aligned, and keeps it
+ * until the stream has passed the call, so a call can be captured in a CUDA
+ * graph.  Strides count elements; the last dimension is contiguous.  Sums,
+ * statistics and accumulators are 32-bit floats, and results do not depend on
+ * the order in which blocks run.  MDH_ERR_INVALID_ARG for a bad pointer,
+ * size, stride or type, MDH_ERR_UNSUPPORTED past a stated limit. */
+typedef enum { MDH_F32 = 0, MDH_BF16 = 1, MDH_F16 = 2 } mdh_dtype;
+typedef enum { MDH_ACT_NONE = 0, MDH_ACT_RELU = 1, MDH_ACT_GELU = 2, MDH_ACT_SILU = 3 } mdh_activation;
+
+/* Layer norm of rows x [rows][width]: y = (x - mean) * rstd * w + b, with
+ * mean and rstd = (var + eps)^-1/2 of each row (var: the mean of the squared
+ * deviations).  x and y have type `dtype`; w and b (NULL: 1 and 0) have type
+ * w_dtype, float32 or `dtype`.  mean / rstd ([rows] float32, NULL allowed)
+ * are kept for the backward pass.  width <= 16384. */
+mdh_status mdh_layer_norm_forward(const void* x, int64_t x_stride, int32_t dtype, const void* w, const void* b,
+                                  int32_t w_dtype, int64_t rows, int32_t width, float eps, void* y, int64_t y_stride,
+                                  float* mean, float* rstd, void* stream);
+/* Gradients of x, w and b from dy [rows][width].  dx, dw and db may be NULL
+ * (not formed); dw and db have type w_dtype.  Rows = 0 gives dw = db = 0. */
+int64_t mdh_layer_norm_backward_workspace(int64_t rows, int32_t width);
+mdh_status mdh_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int32_t dtype,
+                                   const void* w, int32_t w_dtype, const float* mean, const float* rstd, int64_t rows,
+                                   int32_t width, void* dx, int64_t dx_stride, void* dw, void* db, void* ws,
+                                   int64_t ws_bytes, void* stream);
+
+/* Linear layer: z = x w^T + bias, y = act(z) + residual, for x [rows][inner],
+ * w [outer][inner], bias [outer] (NULL: 0), residual and y [rows][outer], all
+ * of type `dtype` (bfloat16 or float16; float32 accumulators).  z_out (NULL
+ * allowed, [rows][outer] contiguous) receives z rounded to `dtype`, which the
+ * backward pass takes.  GELU is z Phi(z). */
+int64_t mdh_linear_forward_workspace(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t rows,
+                                     int32_t inner, int32_t outer);
+mdh_status mdh_linear_forward(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
+                              const void* residual, int64_t residual_stride, int32_t dtype, int32_t activation,
+                              int64_t rows, int32_t inner, int32_t outer, void* y, int64_t y_stride, void* z_out,
+                              void* ws, int64_t ws_bytes, void* stream);
+/* Gradients from dy [rows][outer]: dz = dy act'(z) rounded to `dtype` (the
+ * products' operand type), dx = dz w, dw = dz^T x, db = the column sums of dz
+ * in float32.  dx, dw and db may be NULL (not formed) and are contiguous;
+ * z may be NULL for MDH_ACT_NONE.  The residual's gradient is dy itself. */
+int64_t mdh_linear_backward_workspace(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                                      const void* w, int64_t w_stride, int32_t activation, int64_t rows, int32_t inner,
+                                      int32_t outer);
+mdh_status mdh_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w,
+                               int64_t w_stride, const void* z, int32_t dtype, int32_t activation, int64_t rows,
+                               int32_t inner, int32_t outer, void* dx, void* dw, void* db, void* ws, int64_t ws_bytes,
+                               void* stream);
+
+/* A cache of 8-bit rows in the caller's memory: codes [slots][width], one
+ * byte each, `stride` bytes from row to row.
+ *   code 0, int8: `group` (a positive multiple of 16, or 0 for the whole row)
+ *   elements share one float32 scale, scales [slots][ceil(width / group)];
+ *   an element reads back as code * scale.  Writing takes the group's
+ *   largest magnitude a: scale = a / 127, code = round(x * (127 / a)), each
+ *   rounded to float32, halves to even.  a < 2^-100 stores zeros; a group
+ *   with an infinity or NaN reads back as NaN throughout.
+ *   code 1, uint8: one affine map for the cache: code = round((x - lo) *
+ *   (1 / step)) limited to [0, 255] (NaN to 0), read back as lo + step *
+ *   code; lo, step, 1 / step and each result are rounded to float32.  These codes are a corpus of the exact u8 search: its distances
+ *   times step^2 are the distances of the rows as read back.
+ * width <= 65536, slots < 2^31. */
+typedef struct {
+    void* codes;
+    float* scales;   /* code 0 only */
+    int64_t slots;
+    int64_t stride;  /* bytes, >= width */
+    int32_t width;
+    int32_t group;
+    int32_t code;
+    double lo, step; /* code 1 only */
+} mdh_rows;
+/* Writes row i of rows [n][width] to slot ids[i].  ids: n int32 (id_bits 32)
+ * or int64 (64); an id outside [0, slots) writes nothing.  The ids of one
+ * call that are inside differ from one another. */
+mdh_status mdh_rows_write(const mdh_rows* cache, const void* ids, int32_t id_bits, const void* rows,
+                          int64_t row_stride, int32_t dtype, int64_t n, void* stream);
+/* out [n][width]: the rows of slots ids[i]; zeros where ids[i] is outside. */
+mdh_status mdh_rows_read(const mdh_rows* cache, const void* ids, int32_t id_bits, int64_t n, void* out,
+                         int64_t out_stride, int32_t dtype, void* stream);
+
+/* Attention of each query over its own list of cached rows, the lists that a
+ * search returns.  q [queries][heads][head]; ids [queries][found] int32; key
+ * and value rows hold heads / shared heads of `head` elements each, and
+ * `shared` consecutive query heads read the same one.  Score of entry j:
+ *   s = scale * q . key;  cap > 0: s = cap * tanh(s / cap);  s += bias[j]
+ * An entry is hidden where its id is outside [0, slots), where row_docs[id]
+ * differs from the query's query_docs (both or neither given), or where its
+ * bias is -infinity: its rows are not read.  out = sum_j softmax(s)_j value_j
+ * in q's type; lse (float32 [queries][heads]) = log sum_j exp(s).  A query
+ * with every entry hidden gives out = 0, lse = -infinity.  head: a multiple
+ * of 8 up to 256; key and value caches have the same slots and width (and
+ * may differ in code).  A list stride of 0 gives every query the same list. */
+typedef struct {
+    const void* q;          /* [queries][heads][head], strides below, `head` contiguous */
+    const int32_t* ids;     /* [queries][found], ids_stride */
+    const float* bias;      /* [queries][found], bias_stride; NULL: none */
+    const int32_t* query_docs; /* [queries] or NULL */
+    const int32_t* row_docs;   /* [slots] or NULL */
+    int64_t q_stride, q_head_stride, ids_stride, bias_stride;
+    int64_t queries;
+    int32_t found, heads, shared, head, dtype;
+    float scale, cap;
+} mdh_attend_args;
+int64_t mdh_attend_workspace(const mdh_attend_args* a);
+mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values, void* out, float* lse,
+                      void* ws, int64_t ws_bytes, void* stream);
+/* Gradients of q (dq, q's type, contiguous) and of bias (dbias, float32
+ * [queries][found] contiguous, summed over the heads; NULL: not formed) from
+ * dout (contiguous, q's type) and the lse of the forward call.  The caches
+ * are constants.  dbias is 0 at hidden entries. */
+int64_t mdh_attend_backward_workspace(const mdh_attend_args* a, int32_t want_dbias);
+mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values,
+                               const void* dout, const float* lse, void* dq, float* dbias, void* ws, int64_t ws_bytes,
+                               void* stream);
+
 /* Options (process-wide): force the scan path for testing and measurement.
  * path: 0 = automatic, 1 = CUDA-core scan only, 2 = tensor-core scan on
  * single SMs, 3 = tensor-core scan on SM pairs (each whenever the shape

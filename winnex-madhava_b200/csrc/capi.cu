@@ -23,6 +23,7 @@
 #include <vector>
 
 #include "internal.h"
+#include "op_common.cuh"
 
 namespace mdh {
 
@@ -1016,6 +1017,22 @@ void ensure(void** p, size_t* have, size_t need) { grow(p, have, need); }
 mdh_status run_guarded(void (*fn)(void*), void* ctx) {
     return guard([&] { fn(ctx); });
 }
+
+namespace op {
+
+int current_device() {
+    static std::atomic<uint64_t> usable{0};  // bit d: device d was checked
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= 64 || !(usable.load(std::memory_order_relaxed) >> dev & 1)) {
+        cudaGetLastError();
+        check_device_usable(e == cudaSuccess ? dev : 0);
+        if (dev >= 0 && dev < 64) usable.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    }
+    return dev;
+}
+
+}  // namespace op
 
 }  // namespace mdh
 

@@ -1,0 +1,97 @@
+// Shared by the operators around the search (layer_norm.cu, linear.cu,
+// rows.cu, attend.cu): element types, vector loads and stores, warp and block
+// sums, and the host-side checks of a call.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "internal.h"
+
+namespace mdh {
+namespace op {
+
+using bf16 = __nv_bfloat16;
+using f16 = __half;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(f16 v) { return __half2float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ f16 from_f32<f16>(float v) { return __float2half_rn(v); }
+
+template <class T, int N>
+struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Pack {
+    T v[N];
+};
+
+// N consecutive elements; N * sizeof(T) is 16 (one vector access) or N is 1.
+template <class T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+    if constexpr (sizeof(T) * N == 16) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        return *reinterpret_cast<const Pack<T, N>*>(&u);
+    } else {
+        Pack<T, N> r;
+#pragma unroll
+        for (int i = 0; i < N; i++) r.v[i] = p[i];
+        return r;
+    }
+}
+template <class T, int N>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& r) {
+    if constexpr (sizeof(T) * N == 16)
+        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
+    else {
+#pragma unroll
+        for (int i = 0; i < N; i++) p[i] = r.v[i];
+    }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// ------------------------------------------------------------ host side
+inline size_t dtype_size(int32_t t) { return t == MDH_F32 ? 4 : 2; }
+inline bool dtype_ok(int32_t t) { return t == MDH_F32 || t == MDH_BF16 || t == MDH_F16; }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Rows of `stride` elements of `size` bytes from p can be read 16 bytes at a time.
+inline bool rows_aligned(const void* p, int64_t stride, size_t size) {
+    return aligned16(p) && (stride * (int64_t)size) % 16 == 0;
+}
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The current device, checked once per device to be an sm_100 GPU.
+int current_device();
+
+// fn() under the C ABI's error convention (status code and message).
+template <class F>
+mdh_status guarded(F&& fn) {
+    return run_guarded([](void* p) { (*static_cast<F*>(p))(); }, &fn);
+}
+
+inline void check_launch() { MDH_CUDA(cudaPeekAtLastError()); }
+
+// fn with a value of the element type that `t` names.
+template <class F>
+void by_dtype(int32_t t, F&& fn) {
+    switch (t) {
+        case MDH_F32: fn(float{}); break;
+        case MDH_BF16: fn(bf16{}); break;
+        default: fn(f16{}); break;
+    }
+}
+
+}  // namespace op
+}  // namespace mdh

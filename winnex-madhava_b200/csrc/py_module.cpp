@@ -871,4 +871,81 @@ PYBIND11_MODULE(_winnex_madhava, m) {
     m.def("set_verify", [](int n) { check(mdh_set_verify(n)); }, py::arg("max_queries"),
           "Re-check up to max_queries queries of every search with an exact unpruned scan; misplaced rows are "
           "counted in bound_violations (0 = off).");
+    // Operators around the search: device addresses and sizes as integers
+    // (winnex_madhava/memory.py holds the tensors and checks their shapes).
+    py::class_<mdh_rows>(m, "_Rows")
+        .def(py::init([](uintptr_t codes, uintptr_t scales, int64_t slots, int64_t stride, int32_t width, int32_t group,
+                         int32_t code, double lo, double step) {
+            return mdh_rows{(void*)codes, (float*)scales, slots, stride, width, group, code, lo, step};
+        }));
+    m.def("_layer_norm_forward",
+          [](uintptr_t x, int64_t xs, int32_t dtype, uintptr_t w, uintptr_t b, int32_t w_dtype, int64_t rows,
+             int32_t width, float eps, uintptr_t y, int64_t ys, uintptr_t mean, uintptr_t rstd, uintptr_t stream) {
+              check(mdh_layer_norm_forward((void*)x, xs, dtype, (void*)w, (void*)b, w_dtype, rows, width, eps, (void*)y,
+                                           ys, (float*)mean, (float*)rstd, (void*)stream));
+          });
+    m.def("_layer_norm_backward_workspace", &mdh_layer_norm_backward_workspace);
+    m.def("_layer_norm_backward",
+          [](uintptr_t dy, int64_t dys, uintptr_t x, int64_t xs, int32_t dtype, uintptr_t w, int32_t w_dtype,
+             uintptr_t mean, uintptr_t rstd, int64_t rows, int32_t width, uintptr_t dx, int64_t dxs, uintptr_t dw,
+             uintptr_t db, uintptr_t ws, int64_t ws_bytes, uintptr_t stream) {
+              check(mdh_layer_norm_backward((void*)dy, dys, (void*)x, xs, dtype, (void*)w, w_dtype, (float*)mean,
+                                            (float*)rstd, rows, width, (void*)dx, dxs, (void*)dw, (void*)db, (void*)ws,
+                                            ws_bytes, (void*)stream));
+          });
+    m.def("_linear_forward_workspace",
+          [](uintptr_t x, int64_t xs, uintptr_t w, int64_t wst, int64_t rows, int32_t inner, int32_t outer) {
+              return mdh_linear_forward_workspace((void*)x, xs, (void*)w, wst, rows, inner, outer);
+          });
+    m.def("_linear_forward",
+          [](uintptr_t x, int64_t xs, uintptr_t w, int64_t wst, uintptr_t bias, uintptr_t res, int64_t rs,
+             int32_t dtype, int32_t act, int64_t rows, int32_t inner, int32_t outer, uintptr_t y, int64_t ys,
+             uintptr_t z, uintptr_t ws, int64_t ws_bytes, uintptr_t stream) {
+              check(mdh_linear_forward((void*)x, xs, (void*)w, wst, (void*)bias, (void*)res, rs, dtype, act, rows,
+                                       inner, outer, (void*)y, ys, (void*)z, (void*)ws, ws_bytes, (void*)stream));
+          });
+    m.def("_linear_backward_workspace",
+          [](uintptr_t dy, int64_t dys, uintptr_t x, int64_t xs, uintptr_t w, int64_t wst, int32_t act, int64_t rows,
+             int32_t inner, int32_t outer) {
+              return mdh_linear_backward_workspace((void*)dy, dys, (void*)x, xs, (void*)w, wst, act, rows, inner, outer);
+          });
+    m.def("_linear_backward",
+          [](uintptr_t dy, int64_t dys, uintptr_t x, int64_t xs, uintptr_t w, int64_t wst, uintptr_t z, int32_t dtype,
+             int32_t act, int64_t rows, int32_t inner, int32_t outer, uintptr_t dx, uintptr_t dw, uintptr_t db,
+             uintptr_t ws, int64_t ws_bytes, uintptr_t stream) {
+              check(mdh_linear_backward((void*)dy, dys, (void*)x, xs, (void*)w, wst, (void*)z, dtype, act, rows, inner,
+                                        outer, (void*)dx, (void*)dw, (void*)db, (void*)ws, ws_bytes, (void*)stream));
+          });
+    m.def("_rows_write", [](const mdh_rows& c, uintptr_t ids, int32_t bits, uintptr_t rows, int64_t stride,
+                            int32_t dtype, int64_t n, uintptr_t stream) {
+        check(mdh_rows_write(&c, (void*)ids, bits, (void*)rows, stride, dtype, n, (void*)stream));
+    });
+    m.def("_rows_read", [](const mdh_rows& c, uintptr_t ids, int32_t bits, int64_t n, uintptr_t out, int64_t stride,
+                           int32_t dtype, uintptr_t stream) {
+        check(mdh_rows_read(&c, (void*)ids, bits, n, (void*)out, stride, dtype, (void*)stream));
+    });
+    py::class_<mdh_attend_args>(m, "_AttendArgs")
+        .def(py::init([](uintptr_t q, uintptr_t ids, uintptr_t bias, uintptr_t query_docs, uintptr_t row_docs,
+                         int64_t q_stride, int64_t q_head_stride, int64_t ids_stride, int64_t bias_stride,
+                         int64_t queries, int32_t found, int32_t heads, int32_t shared, int32_t head, int32_t dtype,
+                         float scale, float cap) {
+            return mdh_attend_args{(void*)q,      (int32_t*)ids,  (float*)bias, (int32_t*)query_docs,
+                                   (int32_t*)row_docs, q_stride,  q_head_stride, ids_stride,
+                                   bias_stride,   queries,        found,        heads,
+                                   shared,        head,           dtype,        scale,
+                                   cap};
+        }));
+    m.def("_attend_workspace", [](const mdh_attend_args& a) { return mdh_attend_workspace(&a); });
+    m.def("_attend", [](const mdh_attend_args& a, const mdh_rows& keys, const mdh_rows& values, uintptr_t out,
+                        uintptr_t lse, uintptr_t ws, int64_t ws_bytes, uintptr_t stream) {
+        check(mdh_attend(&a, &keys, &values, (void*)out, (float*)lse, (void*)ws, ws_bytes, (void*)stream));
+    });
+    m.def("_attend_backward_workspace",
+          [](const mdh_attend_args& a, bool want) { return mdh_attend_backward_workspace(&a, want ? 1 : 0); });
+    m.def("_attend_backward",
+          [](const mdh_attend_args& a, const mdh_rows& keys, const mdh_rows& values, uintptr_t dout, uintptr_t lse,
+             uintptr_t dq, uintptr_t dbias, uintptr_t ws, int64_t ws_bytes, uintptr_t stream) {
+              check(mdh_attend_backward(&a, &keys, &values, (void*)dout, (float*)lse, (void*)dq, (float*)dbias,
+                                        (void*)ws, ws_bytes, (void*)stream));
+          });
 }
