@@ -3,21 +3,15 @@
 //
 //   z = x w^T + b,  y = act(z) + residual
 //   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  db = sum_rows dz
-#include "op_common.cuh"
+#include <algorithm>
+
+#include "product.h"
 
 namespace mdh {
 namespace {
 
 using namespace op;
 
-__device__ __forceinline__ float activate(float z, int act) {
-    switch (act) {
-        case MDH_ACT_RELU: return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-        case MDH_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case MDH_ACT_SILU: return z / (1.0f + expf(-z));
-        default: return z;
-    }
-}
 __device__ __forceinline__ float activation_slope(float z, int act) {
     switch (act) {
         case MDH_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
@@ -31,68 +25,13 @@ __device__ __forceinline__ float activation_slope(float z, int act) {
     }
 }
 
-// An operand of a product: element (row, k) at p[row * row_stride + k * k_stride].
-template <class T>
-struct Operand {
-    const T* p;
-    int64_t row_stride, k_stride;
-    __device__ __forceinline__ float at(int64_t row, int64_t k) const { return to_f32(p[row * row_stride + k * k_stride]); }
-};
-
-template <class T>
-struct Epilogue {
-    const T* bias;
-    const T* residual;
-    int64_t residual_stride;
-    int act;
-    T* y;
-    int64_t y_stride;
-    T* z;
-};
-
-constexpr int kTile = 64, kDepth = 16;
-
-// C[m][n] = sum_k a(m, k) b(n, k): a 64 x 64 tile of a block, 4 x 4 outputs of a thread.
-template <class T>
-__global__ void __launch_bounds__(256) k_product(Operand<T> a, Operand<T> b, int64_t m, int64_t n, int64_t k,
-                                                 Epilogue<T> ep) {
-    __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
-    const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
-    const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < k; k0 += kDepth) {
-        for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-            const int r = i / kDepth, c = i % kDepth;
-            sa[c][r] = m0 + r < m && k0 + c < k ? a.at(m0 + r, k0 + c) : 0.0f;
-            sb[c][r] = n0 + r < n && k0 + c < k ? b.at(n0 + r, k0 + c) : 0.0f;
-        }
-        __syncthreads();
-        for (int c = 0; c < kDepth; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] += sa[c][tm + 16 * i] * sb[c][tn + 16 * j];
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            const int64_t r = m0 + tm + 16 * i, c = n0 + tn + 16 * j;
-            if (r >= m || c >= n) continue;
-            float z = acc[i][j] + (ep.bias ? to_f32(ep.bias[c]) : 0.0f);
-            if (ep.z) ep.z[r * n + c] = from_f32<T>(z);
-            z = activate(z, ep.act);
-            if (ep.residual) z += to_f32(ep.residual[r * ep.residual_stride + c]);
-            ep.y[r * ep.y_stride + c] = from_f32<T>(z);
-        }
-}
-
 // dz [rows][n] = dy act'(z) (dz null: not stored), and part[block][n] = the
 // column sums of a block's rows.
 constexpr int kSlopeRows = 64;
 template <class T>
 __global__ void __launch_bounds__(256)
     k_slope(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z, int act, int64_t rows, int64_t n,
-            T* __restrict__ dz, float* __restrict__ part) {
+            T* __restrict__ dz, int64_t dz_stride, float* __restrict__ part) {
     const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= n) return;
     const int64_t r0 = (int64_t)blockIdx.y * kSlopeRows, r1 = min(r0 + kSlopeRows, rows);
@@ -101,7 +40,7 @@ __global__ void __launch_bounds__(256)
         float v = to_f32(dy[r * dy_stride + c]);
         if (act != MDH_ACT_NONE) v *= activation_slope(to_f32(z[r * n + c]), act);
         sum += v;
-        if (dz) dz[r * n + c] = from_f32<T>(v);
+        if (dz) dz[r * dz_stride + c] = from_f32<T>(v);
     }
     if (part) part[blockIdx.y * n + c] = sum;
 }
@@ -114,13 +53,6 @@ __global__ void __launch_bounds__(256) k_join(const float* __restrict__ part, in
     float v = 0.0f;
     for (int64_t i = 0; i < blocks; i++) v += part[i * n + c];
     out[c] = from_f32<T>(v);
-}
-
-template <class T>
-void product(Operand<T> a, Operand<T> b, int64_t m, int64_t n, int64_t k, const Epilogue<T>& ep, cudaStream_t st) {
-    const dim3 grid((unsigned)ceil_div(m, kTile), (unsigned)ceil_div(n, kTile));
-    k_product<T><<<grid, 256, 0, st>>>(a, b, m, n, k, ep);
-    check_launch();
 }
 
 void check_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int32_t dtype, int32_t act,
@@ -136,6 +68,30 @@ void check_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stri
                 "linear: row stride below the inner size");
 }
 
+bool enough(const void* ws, int64_t have, int64_t need) { return need == 0 || (ws && aligned16(ws) && have >= need); }
+
+// The backward pass's scratch: dz (rows of a 16-byte stride) where there is
+// an activation, the partial column sums, and the products' own scratch,
+// which the second product takes over from the first.
+struct BackwardLayout {
+    int64_t dz_stride, part, product, bytes;
+};
+BackwardLayout backward_layout(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w,
+                               int64_t w_stride, int32_t activation, int64_t rows, int32_t inner, int32_t outer) {
+    BackwardLayout l;
+    l.dz_stride = round_up(outer, 8);
+    const bool has_dz = activation != MDH_ACT_NONE;
+    l.part = has_dz ? round_up(rows * l.dz_stride * 2, 128) : 0;
+    l.product = l.part + round_up(ceil_div(rows, kSlopeRows) * outer * 4, 128);
+    // Any 16-byte aligned address stands for dz: only its alignment is looked at.
+    const void* g = has_dz ? nullptr : dy;
+    const int64_t gs = has_dz ? l.dz_stride : dy_stride;
+    const int64_t a = product_workspace({g, gs, true}, {w, w_stride, false}, rows, inner, outer);
+    const int64_t b = product_workspace({g, gs, false}, {x, x_stride, false}, outer, inner, rows);
+    l.bytes = l.product + std::max(a, b);
+    return l;
+}
+
 template <class F>
 void by_half(int32_t t, F&& fn) {
     if (t == MDH_BF16) fn(bf16{});
@@ -149,14 +105,15 @@ using namespace mdh;
 
 extern "C" {
 
-int64_t mdh_linear_forward_workspace(const void*, int64_t, const void*, int64_t, int64_t, int32_t, int32_t) { return 0; }
+int64_t mdh_linear_forward_workspace(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t rows,
+                                     int32_t inner, int32_t outer) {
+    return product_workspace({x, x_stride, true}, {w, w_stride, true}, rows, outer, inner);
+}
 
 mdh_status mdh_linear_forward(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
                               const void* residual, int64_t residual_stride, int32_t dtype, int32_t activation,
                               int64_t rows, int32_t inner, int32_t outer, void* y, int64_t y_stride, void* z_out,
                               void* ws, int64_t ws_bytes, void* stream) {
-    (void)ws;
-    (void)ws_bytes;
     return guarded([&] {
         check_linear(x, x_stride, w, w_stride, dtype, activation, rows, inner, outer);
         MDH_REQUIRE(rows <= 1 || (y_stride >= outer && (!residual || residual_stride >= outer)), MDH_ERR_INVALID_ARG,
@@ -164,20 +121,26 @@ mdh_status mdh_linear_forward(const void* x, int64_t x_stride, const void* w, in
         current_device();
         if (rows == 0) return;
         MDH_REQUIRE(y, MDH_ERR_INVALID_ARG, "linear: null output");
-        by_half(dtype, [&](auto zero) {
-            using T = decltype(zero);
-            const Epilogue<T> ep{(const T*)bias, (const T*)residual, residual_stride, activation, (T*)y, y_stride,
-                                 (T*)z_out};
-            product<T>({(const T*)x, x_stride, 1}, {(const T*)w, w_stride, 1}, rows, outer, inner, ep,
-                       (cudaStream_t)stream);
-        });
+        check_product_status();
+        MDH_REQUIRE(enough(ws, ws_bytes, mdh_linear_forward_workspace(x, x_stride, w, w_stride, rows, inner, outer)),
+                    MDH_ERR_INVALID_ARG, "linear: workspace too small or not 16-byte aligned");
+        ProductEpilogue ep;
+        ep.bias = bias;
+        ep.residual = residual;
+        ep.residual_stride = residual_stride;
+        ep.act = activation;
+        ep.y = y;
+        ep.y_stride = y_stride;
+        ep.z = z_out;
+        product({x, x_stride, true}, {w, w_stride, true}, rows, outer, inner, dtype, ep, ws, (cudaStream_t)stream);
     });
 }
 
-int64_t mdh_linear_backward_workspace(const void*, int64_t, const void*, int64_t, const void*, int64_t,
-                                      int32_t activation, int64_t rows, int32_t, int32_t outer) {
-    if (rows <= 0 || outer <= 0) return 0;
-    return round_up(activation == MDH_ACT_NONE ? 0 : rows * outer * 2, 16) + ceil_div(rows, kSlopeRows) * outer * 4;
+int64_t mdh_linear_backward_workspace(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                                      const void* w, int64_t w_stride, int32_t activation, int64_t rows, int32_t inner,
+                                      int32_t outer) {
+    if (rows <= 0 || outer <= 0 || inner <= 0) return 0;
+    return backward_layout(dy, dy_stride, x, x_stride, w, w_stride, activation, rows, inner, outer).bytes;
 }
 
 mdh_status mdh_linear_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w,
@@ -196,33 +159,38 @@ mdh_status mdh_linear_backward(const void* dy, int64_t dy_stride, const void* x,
             if (db) MDH_CUDA(cudaMemsetAsync(db, 0, (size_t)outer * 2, st));
             return;
         }
-        const int64_t need = mdh_linear_backward_workspace(dy, dy_stride, x, x_stride, w, w_stride, activation, rows,
-                                                           inner, outer);
-        MDH_REQUIRE(ws && aligned16(ws) && ws_bytes >= need, MDH_ERR_INVALID_ARG,
+        check_product_status();
+        const BackwardLayout lay = backward_layout(dy, dy_stride, x, x_stride, w, w_stride, activation, rows, inner, outer);
+        MDH_REQUIRE(enough(ws, ws_bytes, lay.bytes), MDH_ERR_INVALID_ARG,
                     "linear: workspace too small or not 16-byte aligned");
+        char* base = static_cast<char*>(ws);
         by_half(dtype, [&](auto zero) {
             using T = decltype(zero);
-            T* dz = activation == MDH_ACT_NONE ? nullptr : (T*)ws;
-            float* part = (float*)((char*)ws + round_up(dz ? rows * outer * 2 : 0, 16));
+            T* dz = activation == MDH_ACT_NONE ? nullptr : reinterpret_cast<T*>(base);
+            float* part = reinterpret_cast<float*>(base + lay.part);
             const int64_t blocks = ceil_div(rows, kSlopeRows);
             if (dz || db) {
                 const dim3 grid((unsigned)ceil_div(outer, 256), (unsigned)blocks);
                 k_slope<T><<<grid, 256, 0, st>>>((const T*)dy, dy_stride, (const T*)z, activation, rows, outer, dz,
-                                                 db ? part : nullptr);
+                                                 lay.dz_stride, db ? part : nullptr);
                 check_launch();
             }
             if (db) {
                 k_join<T><<<(unsigned)ceil_div(outer, 256), 256, 0, st>>>(part, blocks, outer, (T*)db);
                 check_launch();
             }
-            const T* g = dz ? dz : (const T*)dy;
-            const int64_t gs = dz ? outer : dy_stride;
-            if (dx)
-                product<T>({g, gs, 1}, {(const T*)w, 1, w_stride}, rows, inner, outer,
-                           {nullptr, nullptr, 0, MDH_ACT_NONE, (T*)dx, inner, nullptr}, st);
-            if (dw)
-                product<T>({g, 1, gs}, {(const T*)x, 1, x_stride}, outer, inner, rows,
-                           {nullptr, nullptr, 0, MDH_ACT_NONE, (T*)dw, inner, nullptr}, st);
+            const void* g = dz ? dz : dy;
+            const int64_t gs = dz ? lay.dz_stride : dy_stride;
+            ProductEpilogue ep;
+            ep.y_stride = inner;
+            if (dx) {
+                ep.y = dx;
+                product({g, gs, true}, {w, w_stride, false}, rows, inner, outer, dtype, ep, base + lay.product, st);
+            }
+            if (dw) {
+                ep.y = dw;
+                product({g, gs, false}, {x, x_stride, false}, outer, inner, rows, dtype, ep, base + lay.product, st);
+            }
         });
     });
 }
