@@ -532,3 +532,23 @@ def test_refusals():
     refused(lambda: memory.attend(q, ids[:, None], cache, cache, cap=-1.0), "cap")
     refused(lambda: memory.attend(q, ids[:, None], cache, cache, row_docs=ids), "go together")
     refused(lambda: memory.attend(q, ids[:, None], cache, cache, bias=q[:, 0, :1].double()), "bias must be")
+
+
+def test_attend_lowest_value_everywhere_weighs_alike():
+    """A list whose every bias is the type's lowest value is not empty: its entries weigh alike."""
+    head, slots, found = 64, 40, 12
+    keys, values = filled(slots, head, 0, "int8", 1), filled(slots, head, 0, "int8", 2)
+    q, dout = rand(3, 2, 3, head), rand(4, 2, 3, head)
+    ids = lists(11, 2, found, slots).clamp(min=0)
+    bias = torch.full((2, found), torch.finfo(F32).min, device="cuda")
+    out, lse = memory.attend(q, ids, keys, values, bias=bias)
+    dq, dbias = memory.attend_backward(dout, q, ids, keys, values, lse, bias=bias)
+    k, v = held(keys, head)[:, 0][ids.cpu().long()], held(values, head)[:, 0][ids.cpu().long()]
+    mean = v.mean(1)[:, None].expand(2, 3, head)
+    assert_close(out, mean, 64 * plain.U32 * v.abs().mean(1)[:, None].expand(2, 3, head), "out")
+    dp = torch.einsum("qhd,qkd->qhk", d64(dout), v)
+    ds = (dp - dp.mean(2, keepdim=True)) / found
+    room = 256 * plain.U32 * torch.einsum("qhd,qkd->qhk", d64(dout).abs(), v.abs()).amax(2, keepdim=True)
+    want = head ** -0.5 * torch.einsum("qhk,qkd->qhd", ds, k)
+    assert_close(dq, want, room * head ** -0.5 * k.abs().mean(1)[:, None], "dq")
+    assert_close(dbias, ds.sum(1), (room / found).sum(1).expand(2, found), "dbias")
