@@ -10,14 +10,17 @@
 //   A = sum_j p_j dP_j (1 - t_j^2) k_j,  B = sum_j p_j (1 - t_j^2) k_j:
 // one pass over the rows as well, since p_j follows from lse.
 //
-// Bound by memory: a key and a value code are read once and meet one multiply
-// each for every head that shares them.  A warp takes one (query, group of
-// heads that share a row's head, slice of the list).  LANES lanes hold one
-// entry, 8 elements each (an 8-byte load of codes); 32 / LANES entries go side
-// by side and STEPS of them are loaded before the first is used.  Each lane
-// group keeps its own maximum, sum and vector, joined at the end: first
-// inside the warp, then over the block's slices in shared memory, then over
-// blocks by a second kernel where a list is cut across blocks.
+// A block takes one query, some of its units (a unit: a head of the rows and
+// up to kMaxShared query heads that share it) and a range of its list.  It
+// first lists the range's visible entries in shared memory (ids, documents and
+// biases are read once for all units), then its warps share units and slices
+// of that list.  In a warp LANES lanes hold one entry, 8 elements each (an
+// 8-byte load of codes), 32 / LANES entries go side by side and STEPS of them
+// are loaded at a time.  The STEPS x heads partial products of a lane are
+// summed by halving: each step sends half of the values to the partner lane,
+// so a lane ends with one finished score and the softmax arithmetic is done
+// once per score.  The maximum runs over the whole warp.  Slices are joined in
+// shared memory, ranges of other blocks by a second kernel, in a fixed order.
 //
 // Codes become floats without a conversion instruction: the byte c + 128 in
 // the mantissa of 2^23 is the float 8388736 + c, and one subtraction (two
@@ -33,9 +36,10 @@ namespace {
 
 using namespace op;
 
-constexpr int kWarps = 8;             // of a block
+constexpr int kMaxWarps = 12;         // of a block
+constexpr int kRound = 128;           // entries of the list that a warp looks at at a time
 constexpr int kMaxHead = 256;
-constexpr int kMaxShared = 4;         // query heads a warp takes at a time
+constexpr int kMaxShared = 4;         // query heads of a unit
 constexpr int kMinSlice = 16;         // entries below which a list is not cut further
 
 struct CodeView {
@@ -58,14 +62,16 @@ struct AttendParams {
     int64_t queries;
     int found, heads, shared, head, dtype;
     float scale, cap, inv_cap;
-    int r_blocks;          // blocks of kMaxShared heads of a group
-    int units;             // (group, block of heads) pairs of a query
-    int slices;            // of a list, over the warps of a block
-    int splits;            // of a list, over blocks
-    int slice_len;         // entries of a slice
+    int r_blocks, rb;      // units of a row's head, query heads of each (the last may have fewer)
+    int units;             // of a query
+    int block_units;       // of a block
+    int unit_blocks;       // blocks that share a query's units
+    int slices;            // warps of a block that share a unit
+    int splits, split_len; // ranges of a list over blocks, entries of each
     void* out;
     float* lse;
-    float* part;           // splits > 1
+    float* part;           // splits > 1: vectors [splits][queries][heads][head] (backward: two of them), then float2
+                           // [splits][queries][heads] (m, l) or (D, P)
     // backward
     const void* dout;
     const float* lse_in;
@@ -166,51 +172,169 @@ __device__ __forceinline__ void store_elements(void* p, int64_t i, int dtype, co
 // What a warp works on.
 struct Work {
     int64_t i;       // query
-    int h0, nr;      // first head, heads
+    int h0, nr;      // first head, heads (0: an idle warp)
     int e0;          // this lane's first element of a row
     int d0;          // ... of a head
     bool live;       // the lane holds elements (a head may end inside the lane group)
-    int j0, j1;      // entries
-    int slice;       // within the block
+    int slice;
 };
-template <int LANES, int RB>
-__device__ __forceinline__ bool work_of(const AttendParams& a, Work& w) {
+template <int LANES>
+__device__ __forceinline__ Work work_of(const AttendParams& a) {
+    Work w;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t at = (int64_t)blockIdx.x * (kWarps / a.slices) + warp / a.slices;
-    w.i = at / a.units;
+    w.i = blockIdx.x / a.unit_blocks;
+    const int unit = (int)(blockIdx.x - w.i * a.unit_blocks) * a.block_units + warp / a.slices;
     w.slice = warp % a.slices;
-    if (w.i >= a.queries) return false;
-    const int unit = (int)(at - w.i * a.units);
-    const int g = unit / a.r_blocks, rb = unit - g * a.r_blocks;
-    w.h0 = g * a.shared + rb * RB;
-    w.nr = min(RB, a.shared - rb * RB);
+    const int g = min(unit, a.units - 1) / a.r_blocks, r0 = (unit - g * a.r_blocks) * a.rb;
+    w.h0 = g * a.shared + r0;
+    w.nr = unit < a.units ? max(0, min(a.rb, a.shared - r0)) : 0;
     w.d0 = (lane % LANES) * 8;
     w.live = w.d0 < a.head;
     w.e0 = g * a.head + (w.live ? w.d0 : 0);
-    const int64_t s = (int64_t)(blockIdx.y * a.slices + w.slice) * a.slice_len;
-    w.j0 = (int)min(s, (int64_t)a.found);
-    w.j1 = (int)min(s + a.slice_len, (int64_t)a.found);
-    return true;
+    return w;
 }
 
 // Entry j of the list: its slot, or -1 when it is hidden; its bias.
 __device__ __forceinline__ int entry_slot(const AttendParams& a, int64_t i, int j, int32_t doc, float& bias) {
     const int id = __ldg(a.ids + i * a.ids_stride + j);
-    bias = 0.0f;
-    if (id < 0 || id >= a.slots) return -1;
-    if (a.bias) {
-        bias = __ldg(a.bias + i * a.bias_stride + j);
-        if (bias == -INFINITY) return -1;
-    }
+    bias = a.bias ? __ldg(a.bias + i * a.bias_stride + j) : 0.0f;
+    if (id < 0 || id >= a.slots || bias == -INFINITY) return -1;
     if (a.row_docs && __ldg(a.row_docs + id) != doc) return -1;
     return id;
 }
 
-template <int LANES>
-__device__ __forceinline__ float group_sum(float v) {
+// The visible entries of a range, in order.
+struct Entries {
+    int slot[kMaxWarps * kRound];
+    float bias[kMaxWarps * kRound];
+    int place[kMaxWarps * kRound];  // in the query's list
+    int count[kMaxWarps];
+};
+// Lists the visible entries of [j0, j1), at most kRound a warp.
+__device__ __forceinline__ int list_entries(const AttendParams& a, Entries& e, int64_t i, int32_t doc, int j0, int j1) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    int slot[kRound / 32], n = 0;
+    float bias[kRound / 32];
+    uint32_t seen[kRound / 32];
 #pragma unroll
-    for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    for (int c = 0; c < kRound / 32; c++) {
+        const int j = j0 + warp * kRound + c * 32 + lane;
+        slot[c] = -1;
+        if (j < j1) slot[c] = entry_slot(a, i, j, doc, bias[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < kRound / 32; c++) {
+        seen[c] = __ballot_sync(0xffffffffu, slot[c] >= 0);
+        n += __popc(seen[c]);
+    }
+    __syncthreads();  // the previous list has been read
+    if (lane == 0) e.count[warp] = n;
+    __syncthreads();
+    int before = 0, total = 0;
+    for (int k = 0; k < warps; k++) {
+        const int x = e.count[k];
+        if (k < warp) before += x;
+        total += x;
+    }
+#pragma unroll
+    for (int c = 0; c < kRound / 32; c++) {
+        if (slot[c] >= 0) {
+            const int at = before + __popc(seen[c] & ((1u << lane) - 1u));
+            e.slot[at] = slot[c];
+            e.bias[at] = bias[c];
+            e.place[at] = j0 + warp * kRound + c * 32 + lane;
+        }
+        before += __popc(seen[c]);
+    }
+    __syncthreads();
+    return total;
+}
+// Entries [lo, hi) of n that a slice takes: multiples of `step` but for the end.
+__device__ __forceinline__ void slice_of(int n, int slice, int slices, int step, int& lo, int& hi) {
+    const int per = ((n + slices - 1) / slices + step - 1) / step * step;
+    lo = min(slice * per, n);
+    hi = min(lo + per, n);
+}
+
+// Sums over LANES lanes by halving.  In: N values a lane (N a power of two).
+// Out: KEEP = max(1, N / LANES) finished values a lane, v[x] the sum of the
+// values number value_of(lane, x) over the lane group.
+template <int LANES, int N>
+struct Halving {
+    static constexpr int KEEP = N > LANES ? N / LANES : 1;
+    static constexpr int BITS = N > LANES ? LANES : N;  // lanes that hold different values
+    static constexpr int DUP = LANES / BITS;            // lanes that hold the same
+    static __device__ __forceinline__ void sum(float (&v)[N]) {
+        const int lane = threadIdx.x & 31;
+        int n = N;
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) {
+            if (n > KEEP) {
+                n >>= 1;
+                const bool up = lane & o;
+#pragma unroll
+                for (int x = 0; x < N / 2; x++) {
+                    if (x >= n) break;
+                    const float keep = up ? v[n + x] : v[x], send = up ? v[x] : v[n + x];
+                    v[x] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < KEEP; x++) v[x] += __shfl_xor_sync(0xffffffffu, v[x], o);
+            }
+        }
+    }
+    // Number of the lane's value x.
+    static __device__ __forceinline__ int value_of(int x) { return (threadIdx.x & 31) % LANES / DUP * KEEP + x; }
+    // The lane of this lane's group that holds value number v (in its place v % KEEP).
+    static __device__ __forceinline__ int lane_of(int v) { return (threadIdx.x & 31) / LANES * LANES + v / KEEP * DUP; }
+    template <class T>
+    static __device__ __forceinline__ T get(const T (&v)[KEEP], int number) {
+        return __shfl_sync(0xffffffffu, v[number % KEEP], lane_of(number));
+    }
+};
+
+template <int LANES, int RB>
+struct Steps {
+    static constexpr int RP = RB == 3 ? 4 : RB;                    // heads, as a power of two
+    static constexpr int WANT = RB > 2 ? 2 : 4;
+    static constexpr int N = WANT > LANES ? LANES : WANT;          // steps loaded at a time
+    static constexpr int ENTRIES = 32 / LANES;                     // side by side
+    using Sums = Halving<LANES, N * RP>;                           // value number step * RP + head
+    // Over the lanes that hold the same head: the bits of the step and of the side-by-side entry.
+    template <class F>
+    static __device__ __forceinline__ void over_entries(F&& f) {
+#pragma unroll
+        for (int o = 16; o >= LANES; o >>= 1) f(o);
+#pragma unroll
+        for (int o = LANES / 2; o >= LANES / N && o > 0; o >>= 1) f(o);
+    }
+};
+
+// q (times the scale) or dout of a unit's heads as float pairs; sums of each.
+template <int RB>
+__device__ __forceinline__ void load_heads(const void* p, int64_t at, int64_t stride, int dtype, const Work& w,
+                                           float scale, u64 (&v)[RB][4], float (&sum)[RB]) {
+#pragma unroll
+    for (int r = 0; r < RB; r++) {
+        float x[8] = {};
+        if (w.live && r < w.nr) load_elements(p, at + (w.h0 + r) * stride + w.d0, dtype, x);
+        sum[r] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) sum[r] += x[j] *= scale;
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[r][j] = pair(x[2 * j], x[2 * j + 1]);
+    }
+}
+
+// The scaled, capped and biased score of a finished sum; t = tanh of the capped one.
+__device__ __forceinline__ float score_of(const AttendParams& a, float x, float bias, float& t) {
+    t = 0.0f;
+    if (a.cap > 0.0f) {
+        t = tanh_fast(x * a.inv_cap);
+        x = a.cap * t;
+    }
+    return x + bias;
 }
 
 // Joins two running softmaxes (m, l, vector scaled alike): the factors for
@@ -222,188 +346,14 @@ __device__ __forceinline__ float join(float m, float mo, float& mine, float& oth
     return top;
 }
 
-template <int LANES, int RB>
-__global__ void __launch_bounds__(32 * kWarps) k_attend(const __grid_constant__ AttendParams a) {
-    constexpr int ENTRIES = 32 / LANES;               // side by side
-    constexpr int STEPS = RB == 4 ? 2 : 4;            // loaded at a time
-    constexpr int ROW = LANES * 8 + 2;                // vector, m, l
-    __shared__ float joined[kWarps][ROW];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES;
-    Work w;
-    const bool some = work_of<LANES, RB>(a, w);
-    if (!some) w.nr = 0;
-    u64 q[RB][4], acc[RB][4];
-    float m[RB], l[RB], kb[RB];
-    if (some) {
-#pragma unroll
-        for (int r = 0; r < RB; r++) {
-            float v[8] = {};
-            if (w.live && r < w.nr) load_elements(a.q, w.i * a.q_stride + (w.h0 + r) * a.q_head_stride + w.d0, a.dtype, v);
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) sum += v[j] *= a.scale;
-#pragma unroll
-            for (int j = 0; j < 4; j++) q[r][j] = pair(v[2 * j], v[2 * j + 1]), acc[r][j] = 0;
-            kb[r] = a.k.base * sum;
-            m[r] = -INFINITY;
-            l[r] = 0.0f;
-        }
-        const int kg = w.e0 / a.k.group, vg = w.e0 / a.v.group;
-        const int32_t doc = a.query_docs ? a.query_docs[w.i] : 0;
-        for (int j0 = w.j0; j0 < w.j1; j0 += 32) {
-            float my_bias = 0.0f;
-            const int my_slot = j0 + lane < w.j1 ? entry_slot(a, w.i, j0 + lane, doc, my_bias) : -1;
-            const int n = min(32, w.j1 - j0);
-            for (int t = 0; t < n; t += STEPS * ENTRIES) {
-                uint2 kraw[STEPS], vraw[STEPS];
-                float ks[STEPS], vs[STEPS], bias[STEPS];
-                bool seen[STEPS];
-#pragma unroll
-                for (int u = 0; u < STEPS; u++) {
-                    const int e = t + u * ENTRIES + sub;  // past the list: lane e & 31 holds -1 or e wraps
-                    const int slot = __shfl_sync(0xffffffffu, my_slot, e & 31);
-                    bias[u] = __shfl_sync(0xffffffffu, my_bias, e & 31);
-                    seen[u] = e < n && slot >= 0;
-                    kraw[u] = vraw[u] = make_uint2(0, 0);
-                    ks[u] = vs[u] = 0.0f;
-                    if (seen[u] && w.live) {
-                        kraw[u] = load_codes(a.k, slot, w.e0);
-                        vraw[u] = load_codes(a.v, slot, w.e0);
-                        ks[u] = load_scale(a.k, slot, kg);
-                        vs[u] = load_scale(a.v, slot, vg);
-                    }
-                }
-                float s[STEPS][RB];
-#pragma unroll
-                for (int u = 0; u < STEPS; u++) {
-                    u64 c[4];
-                    code_pairs(kraw[u], a.k.flip, c);
-#pragma unroll
-                    for (int r = 0; r < RB; r++) {
-                        if (r >= w.nr) continue;
-                        float x = group_sum<LANES>(fmaf(ks[u], dot_pairs(q[r], c), kb[r]));
-                        if (a.cap > 0.0f) x = a.cap * tanh_fast(x * a.inv_cap);
-                        s[u][r] = seen[u] ? x + bias[u] : -INFINITY;
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < RB; r++) {
-                    if (r >= w.nr) continue;
-                    float top = m[r];
-#pragma unroll
-                    for (int u = 0; u < STEPS; u++) top = fmaxf(top, s[u][r]);
-                    const float ref = top == -INFINITY ? 0.0f : top, keep = exp_fast(m[r] - ref);
-                    m[r] = top;
-                    l[r] *= keep;
-                    const u64 kk = pair(keep, keep);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[r][j] = mul2(acc[r][j], kk);
-#pragma unroll
-                    for (int u = 0; u < STEPS; u++) {
-                        s[u][r] = exp_fast(s[u][r] - ref);  // now the weight
-                        l[r] += s[u][r];
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < STEPS; u++) {
-                    u64 c[4];
-                    code_pairs(vraw[u], a.v.flip, c);
-#pragma unroll
-                    for (int r = 0; r < RB; r++) {
-                        if (r >= w.nr) continue;
-                        const float p = s[u][r] * vs[u];
-                        const u64 pp = pair(p, p);
-#pragma unroll
-                        for (int j = 0; j < 4; j++) acc[r][j] = fma2(pp, c[j], acc[r][j]);
-                    }
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < RB; r++) {
-        // The lane groups of the warp, then the block's slices.
-        if (r < w.nr) {
-#pragma unroll
-            for (int o = LANES; o < 32; o <<= 1) {
-                const float mo = __shfl_xor_sync(0xffffffffu, m[r], o), lo = __shfl_xor_sync(0xffffffffu, l[r], o);
-                float mine, other;
-                m[r] = join(m[r], mo, mine, other);
-                l[r] = l[r] * mine + lo * other;
-                const u64 mm = pair(mine, mine), oo = pair(other, other);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const u64 x = __shfl_xor_sync(0xffffffffu, acc[r][j], o);
-                    acc[r][j] = fma2(acc[r][j], mm, mul2(x, oo));
-                }
-            }
-            if (a.slices > 1 && lane < LANES) {
-                float* dst = joined[warp];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float2 f = unpair(acc[r][j]);
-                    dst[w.d0 + 2 * j] = f.x;
-                    dst[w.d0 + 2 * j + 1] = f.y;
-                }
-                if (lane == 0) dst[LANES * 8] = m[r], dst[LANES * 8 + 1] = l[r];
-            }
-        }
-        if (a.slices > 1) __syncthreads();
-        if (r < w.nr && w.slice == 0 && lane < LANES && w.live) {
-            float v[8], mm = m[r], ll = l[r];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float2 f = unpair(acc[r][j]);
-                v[2 * j] = f.x, v[2 * j + 1] = f.y;
-            }
-            for (int k = 1; k < a.slices; k++) {
-                const float* src = joined[warp + k];
-                float mine, other;
-                mm = join(mm, src[LANES * 8], mine, other);
-                ll = ll * mine + src[LANES * 8 + 1] * other;
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = v[j] * mine + src[w.d0 + j] * other;
-            }
-            const int64_t at = w.i * a.heads + w.h0 + r;
-            if (a.part) {
-                float* dst = a.part + ((int64_t)blockIdx.y * a.queries * a.heads + at) * (a.head + 2);
-#pragma unroll
-                for (int j = 0; j < 8; j++) dst[w.d0 + j] = v[j];
-                if (lane == 0) dst[a.head] = mm, dst[a.head + 1] = ll;
-            } else {
-                const float inv = ll != 0.0f ? 1.0f / ll : 0.0f, base = ll != 0.0f ? a.v.base : 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = fmaf(v[j], inv, base);
-                store_elements(a.out, at * a.head + w.d0, a.dtype, v);
-                if (lane == 0) a.lse[at] = ll != 0.0f ? mm + logf(ll) : -INFINITY;
-            }
-        }
-        if (a.slices > 1) __syncthreads();  // `joined` has been read
-    }
-}
-
-// Joins the blocks' parts of a list in order: a warp for each (query, head).
-__global__ void __launch_bounds__(128) k_attend_join(const __grid_constant__ AttendParams a) {
-    const int64_t n = a.queries * a.heads, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, d0 = lane * 8;
-    if (at >= n) return;
-    float v[8] = {}, m = -INFINITY, l = 0.0f;
-    for (int s = 0; s < a.splits; s++) {
-        const float* src = a.part + (s * n + at) * (a.head + 2);
-        float mine, other;
-        m = join(m, src[a.head], mine, other);
-        l = l * mine + src[a.head + 1] * other;
-        if (d0 < a.head)
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = v[j] * mine + src[d0 + j] * other;
-    }
+__device__ __forceinline__ void finish_forward(const AttendParams& a, int64_t at, int d0, bool first, float (&v)[8],
+                                               float m, float l) {
     const float inv = l != 0.0f ? 1.0f / l : 0.0f, base = l != 0.0f ? a.v.base : 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = fmaf(v[j], inv, base);
-    if (d0 < a.head) store_elements(a.out, at * a.head + d0, a.dtype, v);
-    if (lane == 0) a.lse[at] = l != 0.0f ? m + logf(l) : -INFINITY;
+    store_elements(a.out, at * a.head + d0, a.dtype, v);
+    if (first) a.lse[at] = l != 0.0f ? m + logf(l) : -INFINITY;
 }
-
 __device__ __forceinline__ void finish_backward(const AttendParams& a, int64_t at, int d0, bool first, float (&x)[8],
                                                 const float (&y)[8], float d, float p) {
     const float inv = p != 0.0f ? 1.0f / p : 0.0f;
@@ -414,192 +364,398 @@ __device__ __forceinline__ void finish_backward(const AttendParams& a, int64_t a
     if (a.sum_d && first) a.sum_d[at] = make_float2(d, inv);
 }
 
+template <int LANES, int RB>
+__global__ void __launch_bounds__(32 * kMaxWarps) k_attend(const __grid_constant__ AttendParams a) {
+    using St = Steps<LANES, RB>;
+    using Sums = typename St::Sums;
+    constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP, ENTRIES = St::ENTRIES;
+    __shared__ union {
+        Entries e;
+        float joined[kMaxWarps][LANES * 8 + 2];  // vector, m, l
+    } sm;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES;
+    const Work w = work_of<LANES>(a);
+    u64 q[RB][4], acc[RB][4];
+    float kb[RB];
+    load_heads<RB>(a.q, w.i * a.q_stride, a.q_head_stride, a.dtype, w, a.scale, q, kb);
+#pragma unroll
+    for (int r = 0; r < RB; r++) {
+        kb[r] *= a.k.base;
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[r][j] = 0;
+    }
+    float m[KEEP], l[KEEP];  // of the lane's own values' heads
+#pragma unroll
+    for (int x = 0; x < KEEP; x++) m[x] = -INFINITY, l[x] = 0.0f;
+    const int kg = w.e0 / a.k.group, vg = w.e0 / a.v.group;
+    const int32_t doc = a.query_docs ? a.query_docs[w.i] : 0;
+    const int j0 = (int)min((int64_t)blockIdx.y * a.split_len, (int64_t)a.found);
+    const int j1 = (int)min((int64_t)j0 + a.split_len, (int64_t)a.found);
+    for (int from = j0; from < j1; from += (blockDim.x >> 5) * kRound) {
+        int lo, hi;
+        slice_of(list_entries(a, sm.e, w.i, doc, from, j1), w.slice, a.slices, STEPS * ENTRIES, lo, hi);
+        if (w.nr == 0) hi = lo;
+        for (int t = lo; t < hi; t += STEPS * ENTRIES) {
+            uint2 kraw[STEPS], vraw[STEPS];
+            float ks[STEPS], vs[STEPS];
+#pragma unroll
+            for (int u = 0; u < STEPS; u++) {
+                const int e = t + u * ENTRIES + sub;
+                kraw[u] = vraw[u] = make_uint2(0, 0);
+                ks[u] = vs[u] = 0.0f;
+                if (e < hi && w.live) {
+                    const int slot = sm.e.slot[e];
+                    kraw[u] = load_codes(a.k, slot, w.e0);
+                    vraw[u] = load_codes(a.v, slot, w.e0);
+                    ks[u] = load_scale(a.k, slot, kg);
+                    vs[u] = load_scale(a.v, slot, vg);
+                }
+            }
+            float s[STEPS * RP];
+#pragma unroll
+            for (int u = 0; u < STEPS; u++) {
+                u64 c[4];
+                code_pairs(kraw[u], a.k.flip, c);
+#pragma unroll
+                for (int r = 0; r < RP; r++) s[u * RP + r] = r < RB ? fmaf(ks[u], dot_pairs(q[r < RB ? r : 0], c), kb[r < RB ? r : 0]) : 0.0f;
+            }
+            Sums::sum(s);
+            float p[KEEP], keep[KEEP];
+            bool grown = false;
+#pragma unroll
+            for (int x = 0; x < KEEP; x++) {
+                const int e = t + Sums::value_of(x) / RP * ENTRIES + sub;
+                float th;
+                p[x] = e < hi ? score_of(a, s[x], sm.e.bias[e], th) : -INFINITY;
+                float top = p[x];
+                St::over_entries([&](int o) { top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o)); });
+                top = fmaxf(top, m[x]);
+                grown |= top > m[x];
+                const float ref = top == -INFINITY ? 0.0f : top;
+                keep[x] = exp_fast(m[x] - ref);
+                m[x] = top;
+                p[x] = exp_fast(p[x] - ref);
+                l[x] = l[x] * keep[x] + p[x];
+            }
+            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                for (int r = 0; r < RB; r++) {
+                    const float k = Sums::get(keep, r);  // every step's lanes hold the same
+                    const u64 kk = pair(k, k);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[r][j] = mul2(acc[r][j], kk);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < STEPS; u++) {
+                u64 c[4];
+                code_pairs(vraw[u], a.v.flip, c);
+#pragma unroll
+                for (int r = 0; r < RB; r++) {
+                    const float pv = Sums::get(p, u * RP + r) * vs[u];
+                    const u64 pp = pair(pv, pv);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[r][j] = fma2(pp, c[j], acc[r][j]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < KEEP; x++)
+        St::over_entries([&](int o) { l[x] += __shfl_xor_sync(0xffffffffu, l[x], o); });
+#pragma unroll
+    for (int r = 0; r < RB; r++) {
+        float v[8], mm = Sums::get(m, r), ll = Sums::get(l, r);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            u64 x = acc[r][j];
+#pragma unroll
+            for (int o = LANES; o < 32; o <<= 1) x = add2(x, __shfl_xor_sync(0xffffffffu, x, o));
+            const float2 f = unpair(x);
+            v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        }
+        const bool write = r < w.nr && w.slice == 0 && lane < LANES && w.live;
+        if (a.slices > 1) {
+            __syncthreads();  // the list, or the previous head's vectors, have been read
+            if (lane < LANES) {
+                float* dst = sm.joined[warp];
+#pragma unroll
+                for (int j = 0; j < 8; j++) dst[w.d0 + j] = v[j];
+                if (lane == 0) dst[LANES * 8] = mm, dst[LANES * 8 + 1] = ll;
+            }
+            __syncthreads();
+            if (write) {
+                for (int k = 1; k < a.slices; k++) {
+                    const float* src = sm.joined[warp + k];
+                    float mine, other;
+                    mm = join(mm, src[LANES * 8], mine, other);
+                    ll = ll * mine + src[LANES * 8 + 1] * other;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] = v[j] * mine + src[w.d0 + j] * other;
+                }
+            }
+        }
+        if (!write) continue;
+        const int64_t at = w.i * a.heads + w.h0 + r;
+        if (a.part) {
+            const int64_t n = a.queries * a.heads, row = (int64_t)blockIdx.y * n + at;
+            float4* dst = reinterpret_cast<float4*>(a.part + row * a.head + w.d0);
+            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+            if (lane == 0) reinterpret_cast<float2*>(a.part + a.splits * n * a.head)[row] = make_float2(mm, ll);
+        } else {
+            finish_forward(a, at, w.d0, lane == 0, v, mm, ll);
+        }
+    }
+}
+
+// Joins the ranges of a list: a block for each (query, head), 8 elements a
+// lane group of 4 warps, each every fourth range; the warps' sums in order.
+__global__ void __launch_bounds__(128) k_attend_join(const __grid_constant__ AttendParams a) {
+    __shared__ float joined[4][kMaxHead + 1];
+    const int64_t n = a.queries * a.heads, at = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d0 = lane * 8;
+    const float2* ml = reinterpret_cast<const float2*>(a.part + a.splits * n * a.head);
+    float m = -INFINITY;
+    for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, ml[s * n + at].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float v[8] = {}, l = 0.0f;
+#pragma unroll 4
+    for (int s = warp; s < a.splits; s += 4) {
+        const float2 x = ml[s * n + at];
+        const float f = exp_fast(x.x - ref);
+        l += x.y * f;
+        if (d0 < a.head) {
+            const float4* src = reinterpret_cast<const float4*>(a.part + (s * n + at) * a.head + d0);
+            const float4 y = src[0], z = src[1];
+            v[0] += y.x * f, v[1] += y.y * f, v[2] += y.z * f, v[3] += y.w * f;
+            v[4] += z.x * f, v[5] += z.y * f, v[6] += z.z * f, v[7] += z.w * f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) joined[warp][d0 + j] = v[j];
+    if (lane == 0) joined[warp][kMaxHead] = l;
+    __syncthreads();
+    if (warp != 0) return;
+    for (int k = 1; k < 4; k++) {
+        l += joined[k][kMaxHead];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] += joined[k][d0 + j];
+    }
+    if (d0 < a.head) finish_forward(a, at, d0, lane == 0, v, m, l);
+}
+
 // A, B, D and the weights' own sum P of the lists' slices; dq = scale (A - (D / P) B) / P.
 // P is 1 up to rounding, except where lse cannot hold its own digits beside
 // scores of 1e9 and more (a mask of the type's lowest value throughout).
 template <int LANES, int RB>
-__global__ void __launch_bounds__(32 * kWarps) k_attend_backward(const __grid_constant__ AttendParams a) {
-    constexpr int ENTRIES = 32 / LANES;
-    constexpr int STEPS = 2;
-    constexpr int ROW = LANES * 16 + 2;               // A, B, D, P
-    __shared__ float joined[kWarps][ROW];
+__global__ void __launch_bounds__(32 * kMaxWarps) k_attend_backward(const __grid_constant__ AttendParams a) {
+    using St = Steps<LANES, RB>;
+    using Sums = typename St::Sums;
+    constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP, ENTRIES = St::ENTRIES;
+    __shared__ union {
+        Entries e;
+        float joined[kMaxWarps][LANES * 16 + 2];  // A, B, D, P
+    } sm;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES;
-    Work w;
-    const bool some = work_of<LANES, RB>(a, w);
-    if (!some) w.nr = 0;
+    const Work w = work_of<LANES>(a);
     u64 q[RB][4], g[RB][4], va[RB][4], vb[RB][4];
-    float kb[RB], gb[RB], z[RB], dsum[RB], psum[RB];
-    if (some) {
+    float kb[RB], gb[RB];
+    load_heads<RB>(a.q, w.i * a.q_stride, a.q_head_stride, a.dtype, w, a.scale, q, kb);
+    load_heads<RB>(a.dout, w.i * a.heads * a.head, a.head, a.dtype, w, 1.0f, g, gb);
 #pragma unroll
-        for (int r = 0; r < RB; r++) {
-            float v[8] = {}, d[8] = {};
-            const int64_t at = w.i * a.heads + w.h0 + r;
-            z[r] = 0.0f;
-            if (r < w.nr) {
-                z[r] = a.lse_in[at];
-                if (w.live) {
-                    load_elements(a.q, w.i * a.q_stride + (w.h0 + r) * a.q_head_stride + w.d0, a.dtype, v);
-                    load_elements(a.dout, at * a.head + w.d0, a.dtype, d);
+    for (int r = 0; r < RB; r++) {
+        kb[r] *= a.k.base;
+        gb[r] *= a.v.base;
+#pragma unroll
+        for (int j = 0; j < 4; j++) va[r][j] = vb[r][j] = 0;
+    }
+    float z[KEEP], dsum[KEEP], psum[KEEP];  // of the lane's own values' heads
+#pragma unroll
+    for (int x = 0; x < KEEP; x++) {
+        const int r = Sums::value_of(x) % RP;
+        z[x] = r < w.nr ? a.lse_in[w.i * a.heads + w.h0 + r] : 0.0f;
+        dsum[x] = psum[x] = 0.0f;
+    }
+    const int kg = w.e0 / a.k.group, vg = w.e0 / a.v.group;
+    const int32_t doc = a.query_docs ? a.query_docs[w.i] : 0;
+    const u64 kbase = pair(a.k.base, a.k.base);
+    const int j0 = (int)min((int64_t)blockIdx.y * a.split_len, (int64_t)a.found);
+    const int j1 = (int)min((int64_t)j0 + a.split_len, (int64_t)a.found);
+    for (int from = j0; from < j1; from += (blockDim.x >> 5) * kRound) {
+        int lo, hi;
+        slice_of(list_entries(a, sm.e, w.i, doc, from, j1), w.slice, a.slices, STEPS * ENTRIES, lo, hi);
+        if (w.nr == 0) hi = lo;
+        for (int t = lo; t < hi; t += STEPS * ENTRIES) {
+            uint2 kraw[STEPS], vraw[STEPS];
+            float ks[STEPS], vs[STEPS];
+#pragma unroll
+            for (int u = 0; u < STEPS; u++) {
+                const int e = t + u * ENTRIES + sub;
+                kraw[u] = vraw[u] = make_uint2(0, 0);
+                ks[u] = vs[u] = 0.0f;
+                if (e < hi && w.live) {
+                    const int slot = sm.e.slot[e];
+                    kraw[u] = load_codes(a.k, slot, w.e0);
+                    vraw[u] = load_codes(a.v, slot, w.e0);
+                    ks[u] = load_scale(a.k, slot, kg);
+                    vs[u] = load_scale(a.v, slot, vg);
                 }
             }
-            float sq = 0.0f, sg = 0.0f;
+            float s[STEPS * RP], dp[STEPS * RP];
 #pragma unroll
-            for (int j = 0; j < 8; j++) sq += v[j] *= a.scale, sg += d[j];
+            for (int u = 0; u < STEPS; u++) {
+                u64 c[4];
+                code_pairs(kraw[u], a.k.flip, c);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                q[r][j] = pair(v[2 * j], v[2 * j + 1]);
-                g[r][j] = pair(d[2 * j], d[2 * j + 1]);
-                va[r][j] = vb[r][j] = 0;
+                for (int r = 0; r < RP; r++) s[u * RP + r] = r < RB ? fmaf(ks[u], dot_pairs(q[r < RB ? r : 0], c), kb[r < RB ? r : 0]) : 0.0f;
+                code_pairs(vraw[u], a.v.flip, c);
+#pragma unroll
+                for (int r = 0; r < RP; r++) dp[u * RP + r] = r < RB ? fmaf(vs[u], dot_pairs(g[r < RB ? r : 0], c), gb[r < RB ? r : 0]) : 0.0f;
             }
-            kb[r] = a.k.base * sq;
-            gb[r] = a.v.base * sg;
-            dsum[r] = psum[r] = 0.0f;
-        }
-        const int kg = w.e0 / a.k.group, vg = w.e0 / a.v.group;
-        const int32_t doc = a.query_docs ? a.query_docs[w.i] : 0;
-        const u64 kbase = pair(a.k.base, a.k.base);
-        for (int j0 = w.j0; j0 < w.j1; j0 += 32) {
-            float my_bias = 0.0f;
-            const int my_slot = j0 + lane < w.j1 ? entry_slot(a, w.i, j0 + lane, doc, my_bias) : -1;
-            const int n = min(32, w.j1 - j0);
-            for (int t = 0; t < n; t += STEPS * ENTRIES) {
-                uint2 kraw[STEPS], vraw[STEPS];
-                float ks[STEPS], vs[STEPS], bias[STEPS];
-                bool seen[STEPS];
+            Sums::sum(s);
+            Sums::sum(dp);
+            float fa[KEEP], fb[KEEP];
 #pragma unroll
-                for (int u = 0; u < STEPS; u++) {
-                    const int e = t + u * ENTRIES + sub;
-                    const int slot = __shfl_sync(0xffffffffu, my_slot, e & 31);
-                    bias[u] = __shfl_sync(0xffffffffu, my_bias, e & 31);
-                    seen[u] = e < n && slot >= 0;
-                    kraw[u] = vraw[u] = make_uint2(0, 0);
-                    ks[u] = vs[u] = 0.0f;
-                    if (seen[u] && w.live) {
-                        kraw[u] = load_codes(a.k, slot, w.e0);
-                        vraw[u] = load_codes(a.v, slot, w.e0);
-                        ks[u] = load_scale(a.k, slot, kg);
-                        vs[u] = load_scale(a.v, slot, vg);
-                    }
+            for (int x = 0; x < KEEP; x++) {
+                const int v = Sums::value_of(x), r = v % RP, e = t + v / RP * ENTRIES + sub;
+                fa[x] = fb[x] = 0.0f;
+                if (e < hi && r < w.nr) {
+                    float th;
+                    const float sc = score_of(a, s[x], sm.e.bias[e], th);
+                    const float p = exp_fast(sc - z[x]), pdp = p * dp[x], slope = 1.0f - th * th;
+                    dsum[x] += pdp;
+                    psum[x] += p;
+                    fa[x] = pdp * slope;
+                    fb[x] = p * slope;
+                    if (a.pd && lane % Sums::DUP == 0)
+                        a.pd[(w.i * a.heads + w.h0 + r) * a.found + sm.e.place[e]] = make_float2(pdp, p);
                 }
+            }
 #pragma unroll
-                for (int u = 0; u < STEPS; u++) {
-                    const int e = t + u * ENTRIES + sub;
-                    u64 kc[4], vc[4];
-                    code_pairs(kraw[u], a.k.flip, kc);
-                    code_pairs(vraw[u], a.v.flip, vc);
-                    const u64 kss = pair(ks[u], ks[u]);
+            for (int u = 0; u < STEPS; u++) {
+                u64 c[4];
+                code_pairs(kraw[u], a.k.flip, c);
+                const u64 kss = pair(ks[u], ks[u]);
 #pragma unroll
-                    for (int r = 0; r < RB; r++) {
-                        if (r >= w.nr) continue;
-                        float x = group_sum<LANES>(fmaf(ks[u], dot_pairs(q[r], kc), kb[r]));
-                        const float dp = group_sum<LANES>(fmaf(vs[u], dot_pairs(g[r], vc), gb[r]));
-                        float slope = 1.0f;
-                        if (a.cap > 0.0f) {
-                            const float th = tanh_fast(x * a.inv_cap);
-                            x = a.cap * th;
-                            slope = 1.0f - th * th;
-                        }
-                        const float p = seen[u] ? exp_fast(x + bias[u] - z[r]) : 0.0f;
-                        const float pdp = seen[u] ? p * dp : 0.0f;
-                        dsum[r] += pdp;
-                        psum[r] += p;
-                        if (a.pd && lane % LANES == 0 && e < n)
-                            a.pd[(w.i * a.heads + w.h0 + r) * a.found + j0 + e] = make_float2(pdp, p);
-                        const float fa = pdp * slope, fb = p * slope;
-                        const u64 pa = pair(fa, fa), pb = pair(fb, fb);
+                for (int j = 0; j < 4; j++) c[j] = fma2(kss, c[j], kbase);  // the key's values
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const u64 kv = fma2(kss, kc[j], kbase);  // the key's values (an unseen entry: pa = pb = 0)
-                            va[r][j] = fma2(pa, kv, va[r][j]);
-                            vb[r][j] = fma2(pb, kv, vb[r][j]);
-                        }
+                for (int r = 0; r < RB; r++) {
+                    const float xa = Sums::get(fa, u * RP + r), xb = Sums::get(fb, u * RP + r);
+                    const u64 pa = pair(xa, xa), pb = pair(xb, xb);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        va[r][j] = fma2(pa, c[j], va[r][j]);
+                        vb[r][j] = fma2(pb, c[j], vb[r][j]);
                     }
                 }
             }
         }
     }
 #pragma unroll
+    for (int x = 0; x < KEEP; x++)
+        St::over_entries([&](int o) {
+            dsum[x] += __shfl_xor_sync(0xffffffffu, dsum[x], o);
+            psum[x] += __shfl_xor_sync(0xffffffffu, psum[x], o);
+        });
+#pragma unroll
     for (int r = 0; r < RB; r++) {
-        if (r < w.nr) {
+        float x[8], y[8], d = Sums::get(dsum, r), p = Sums::get(psum, r);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            u64 xa = va[r][j], xb = vb[r][j];
 #pragma unroll
             for (int o = LANES; o < 32; o <<= 1) {
-                dsum[r] += __shfl_xor_sync(0xffffffffu, dsum[r], o);
-                psum[r] += __shfl_xor_sync(0xffffffffu, psum[r], o);
+                xa = add2(xa, __shfl_xor_sync(0xffffffffu, xa, o));
+                xb = add2(xb, __shfl_xor_sync(0xffffffffu, xb, o));
+            }
+            const float2 f = unpair(xa), h = unpair(xb);
+            x[2 * j] = f.x, x[2 * j + 1] = f.y, y[2 * j] = h.x, y[2 * j + 1] = h.y;
+        }
+        const bool write = r < w.nr && w.slice == 0 && lane < LANES && w.live;
+        if (a.slices > 1) {
+            __syncthreads();  // the list, or the previous head's vectors, have been read
+            if (lane < LANES) {
+                float* dst = sm.joined[warp];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    va[r][j] = add2(va[r][j], __shfl_xor_sync(0xffffffffu, va[r][j], o));
-                    vb[r][j] = add2(vb[r][j], __shfl_xor_sync(0xffffffffu, vb[r][j], o));
+                for (int j = 0; j < 8; j++) dst[w.d0 + j] = x[j], dst[LANES * 8 + w.d0 + j] = y[j];
+                if (lane == 0) dst[LANES * 16] = d, dst[LANES * 16 + 1] = p;
+            }
+            __syncthreads();
+            if (write) {
+                for (int k = 1; k < a.slices; k++) {
+                    const float* src = sm.joined[warp + k];
+                    d += src[LANES * 16];
+                    p += src[LANES * 16 + 1];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] += src[w.d0 + j], y[j] += src[LANES * 8 + w.d0 + j];
                 }
             }
-            if (a.slices > 1 && lane < LANES) {
-                float* dst = joined[warp];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float2 x = unpair(va[r][j]), y = unpair(vb[r][j]);
-                    dst[w.d0 + 2 * j] = x.x, dst[w.d0 + 2 * j + 1] = x.y;
-                    dst[LANES * 8 + w.d0 + 2 * j] = y.x, dst[LANES * 8 + w.d0 + 2 * j + 1] = y.y;
-                }
-                if (lane == 0) dst[LANES * 16] = dsum[r], dst[LANES * 16 + 1] = psum[r];
-            }
         }
-        if (a.slices > 1) __syncthreads();
-        if (r < w.nr && w.slice == 0 && lane < LANES && w.live) {
-            float x[8], y[8], d = dsum[r], p = psum[r];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float2 fa = unpair(va[r][j]), fb = unpair(vb[r][j]);
-                x[2 * j] = fa.x, x[2 * j + 1] = fa.y, y[2 * j] = fb.x, y[2 * j + 1] = fb.y;
-            }
-            for (int k = 1; k < a.slices; k++) {
-                const float* src = joined[warp + k];
-                d += src[LANES * 16];
-                p += src[LANES * 16 + 1];
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[j] += src[w.d0 + j], y[j] += src[LANES * 8 + w.d0 + j];
-            }
-            const int64_t at = w.i * a.heads + w.h0 + r;
-            if (a.part) {
-                float* dst = a.part + ((int64_t)blockIdx.y * a.queries * a.heads + at) * (2 * a.head + 2);
-#pragma unroll
-                for (int j = 0; j < 8; j++) dst[w.d0 + j] = x[j], dst[a.head + w.d0 + j] = y[j];
-                if (lane == 0) dst[2 * a.head] = d, dst[2 * a.head + 1] = p;
-            } else {
-                finish_backward(a, at, w.d0, lane == 0, x, y, d, p);
-            }
+        if (!write) continue;
+        const int64_t at = w.i * a.heads + w.h0 + r;
+        if (a.part) {
+            const int64_t n = a.queries * a.heads, row = (int64_t)blockIdx.y * n + at;
+            float4* dst = reinterpret_cast<float4*>(a.part + row * 2 * a.head + w.d0);
+            float4* dsb = reinterpret_cast<float4*>(a.part + (row * 2 + 1) * a.head + w.d0);
+            dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+            dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+            dsb[0] = make_float4(y[0], y[1], y[2], y[3]);
+            dsb[1] = make_float4(y[4], y[5], y[6], y[7]);
+            if (lane == 0) reinterpret_cast<float2*>(a.part + a.splits * n * 2 * a.head)[row] = make_float2(d, p);
+        } else {
+            finish_backward(a, at, w.d0, lane == 0, x, y, d, p);
         }
-        if (a.slices > 1) __syncthreads();  // `joined` has been read
     }
 }
 
+// Joins the ranges of a list, as k_attend_join: plain sums.
 __global__ void __launch_bounds__(128) k_attend_backward_join(const __grid_constant__ AttendParams a) {
-    const int64_t n = a.queries * a.heads, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, d0 = lane * 8;
-    if (at >= n) return;
+    __shared__ float joined[4][2 * kMaxHead + 2];
+    const int64_t n = a.queries * a.heads, at = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d0 = lane * 8;
+    const float2* dp = reinterpret_cast<const float2*>(a.part + a.splits * n * 2 * a.head);
     float x[8] = {}, y[8] = {}, d = 0.0f, p = 0.0f;
-    for (int s = 0; s < a.splits; s++) {
-        const float* src = a.part + (s * n + at) * (2 * a.head + 2);
-        d += src[2 * a.head];
-        p += src[2 * a.head + 1];
-        if (d0 < a.head)
+#pragma unroll 4
+    for (int s = warp; s < a.splits; s += 4) {
+        const float2 f = dp[s * n + at];
+        d += f.x;
+        p += f.y;
+        if (d0 < a.head) {
+            const float* src = a.part + (s * n + at) * 2 * a.head + d0;
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] += src[d0 + j], y[j] += src[a.head + d0 + j];
+            for (int j = 0; j < 8; j++) x[j] += src[j], y[j] += src[a.head + j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) joined[warp][d0 + j] = x[j], joined[warp][kMaxHead + d0 + j] = y[j];
+    if (lane == 0) joined[warp][2 * kMaxHead] = d, joined[warp][2 * kMaxHead + 1] = p;
+    __syncthreads();
+    if (warp != 0) return;
+    for (int k = 1; k < 4; k++) {
+        d += joined[k][2 * kMaxHead];
+        p += joined[k][2 * kMaxHead + 1];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] += joined[k][d0 + j], y[j] += joined[k][kMaxHead + d0 + j];
     }
     if (d0 < a.head) finish_backward(a, at, d0, lane == 0, x, y, d, p);
 }
 
-// dbias[i][j] = sum over heads of (p dP - p D / P) / P, in head order.
-__global__ void __launch_bounds__(256) k_attend_dbias(const float2* __restrict__ pd, const float2* __restrict__ sum_d,
-                                                      int64_t queries, int heads, int found,
-                                                      float* __restrict__ dbias) {
+// dbias[i][j] = sum over heads of (p dP - p D / P) / P, in head order; 0 at hidden entries.
+__global__ void __launch_bounds__(256) k_attend_dbias(const __grid_constant__ AttendParams a, float* __restrict__ dbias) {
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= queries * found) return;
-    const int64_t i = at / found;
-    const int j = (int)(at - i * found);
-    float v = 0.0f;
-    for (int h = 0; h < heads; h++) {
-        const float2 x = pd[(i * heads + h) * found + j];
-        const float2 d = __ldg(sum_d + i * heads + h);
-        v += (x.x - x.y * d.x) * d.y;
+    if (at >= a.queries * a.found) return;
+    const int64_t i = at / a.found;
+    const int j = (int)(at - i * a.found);
+    float v = 0.0f, bias;
+    if (entry_slot(a, i, j, a.query_docs ? a.query_docs[i] : 0, bias) >= 0) {
+#pragma unroll 4
+        for (int h = 0; h < a.heads; h++) {
+            const float2 x = __ldg(a.pd + (i * a.heads + h) * a.found + j), d = __ldg(a.sum_d + i * a.heads + h);
+            v += (x.x - x.y * d.x) * d.y;
+        }
     }
     dbias[at] = v;
 }
@@ -618,19 +774,22 @@ CodeView code_view(const RowsView& r) {
     return c;
 }
 
-// How a call's lists are cut: enough warps to fill the GPU, no slice below
-// kMinSlice entries; over a block's warps first (joined in shared memory),
-// then over blocks.
-void cut_lists(AttendParams& p) {
+// How a call is laid out over blocks.  A block takes up to kMaxWarps units of
+// a query; where they are few, several warps share a unit's list, up to 8
+// warps a block and no slice below kMinSlice entries; where the blocks do not
+// fill the GPU, a list is cut into ranges for several blocks.
+void lay_out(AttendParams& p) {
     p.r_blocks = (int)ceil_div(p.shared, kMaxShared);
+    p.rb = (int)ceil_div(p.shared, p.r_blocks);
     p.units = p.heads / p.shared * p.r_blocks;
-    const int64_t want = 148 * 24;
-    const int64_t most = std::max<int64_t>(1, ceil_div(p.found, kMinSlice));
-    const int64_t cuts = std::max<int64_t>(1, std::min(most, want / std::max<int64_t>(1, p.queries * p.units)));
-    p.slices = 1;
-    while (p.slices * 2 <= std::min<int64_t>(cuts, kWarps)) p.slices *= 2;
-    p.splits = (int)std::min<int64_t>(ceil_div(cuts, p.slices), 65535);
-    p.slice_len = (int)std::max<int64_t>(1, ceil_div(p.found, (int64_t)p.slices * p.splits));
+    p.unit_blocks = (int)ceil_div(p.units, kMaxWarps);
+    p.block_units = (int)ceil_div(p.units, p.unit_blocks);
+    const int64_t slices = std::min<int64_t>(8 / std::min(8, p.block_units), ceil_div(p.found, kMinSlice));
+    p.slices = (int)std::max<int64_t>(1, slices);
+    const int64_t warps = std::max<int64_t>(1, p.queries * p.unit_blocks * p.block_units * p.slices);
+    const int64_t splits = std::min(ceil_div(p.found, p.slices * kMinSlice), 148 * 16 / warps);
+    p.split_len = (int)std::max<int64_t>(1, ceil_div(p.found, std::max<int64_t>(1, splits)));
+    p.splits = (int)std::max<int64_t>(1, ceil_div(p.found, p.split_len));
 }
 
 AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values) {
@@ -677,20 +836,20 @@ AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const 
     p.scale = a->scale;
     p.cap = a->cap;
     p.inv_cap = a->cap > 0.0f ? 1.0f / a->cap : 0.0f;
-    cut_lists(p);
-    MDH_REQUIRE(p.queries * p.units <= INT32_MAX, MDH_ERR_UNSUPPORTED, "attend: too many queries");
+    lay_out(p);
+    MDH_REQUIRE(p.queries * p.unit_blocks <= INT32_MAX && p.queries * p.heads <= INT32_MAX, MDH_ERR_UNSUPPORTED, "attend: too many queries");
     return p;
 }
 
-// The cut of a call from its sizes alone, for the workspace.
-AttendParams cut_of(const mdh_attend_args* a) {
+// The layout of a call from its sizes alone, for the workspace.
+AttendParams layout_of(const mdh_attend_args* a) {
     AttendParams p{};
     p.queries = a->queries;
     p.found = a->found;
     p.heads = a->heads;
     p.shared = a->shared;
     p.head = a->head;
-    cut_lists(p);
+    lay_out(p);
     return p;
 }
 bool has_sizes(const mdh_attend_args* a) {
@@ -703,11 +862,12 @@ int64_t backward_part(const AttendParams& p) {
 
 // fn(LANES, RB): lanes that hold a head, and heads of a warp.
 template <class F>
-void by_shape(int head, int shared, F&& fn) {
+void by_shape(int head, int rb, F&& fn) {
     auto heads = [&](auto lanes) {
-        if (shared == 1) fn(lanes, std::integral_constant<int, 1>{});
-        else if (shared == 2) fn(lanes, std::integral_constant<int, 2>{});
-        else fn(lanes, std::integral_constant<int, kMaxShared>{});
+        if (rb == 1) fn(lanes, std::integral_constant<int, 1>{});
+        else if (rb == 2) fn(lanes, std::integral_constant<int, 2>{});
+        else if (rb == 3) fn(lanes, std::integral_constant<int, 3>{});
+        else fn(lanes, std::integral_constant<int, 4>{});
     };
     if (head <= 8) heads(std::integral_constant<int, 1>{});
     else if (head <= 16) heads(std::integral_constant<int, 2>{});
@@ -717,8 +877,9 @@ void by_shape(int head, int shared, F&& fn) {
     else heads(std::integral_constant<int, 32>{});
 }
 dim3 attend_grid(const AttendParams& p) {
-    return dim3((unsigned)ceil_div(p.queries * p.units, kWarps / p.slices), (unsigned)p.splits);
+    return dim3((unsigned)(p.queries * p.unit_blocks), (unsigned)p.splits);
 }
+int attend_threads(const AttendParams& p) { return 32 * p.block_units * p.slices; }
 
 }  // namespace
 }  // namespace mdh
@@ -729,7 +890,7 @@ extern "C" {
 
 int64_t mdh_attend_workspace(const mdh_attend_args* a) {
     if (!has_sizes(a)) return 0;
-    const AttendParams p = cut_of(a);
+    const AttendParams p = layout_of(a);
     return p.splits > 1 ? p.splits * p.queries * p.heads * ((int64_t)p.head + 2) * 4 : 0;
 }
 
@@ -747,10 +908,11 @@ mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_
         p.out = out;
         p.lse = lse;
         p.part = need ? (float*)ws : nullptr;
-        by_shape(p.head, p.shared, [&](auto lanes, auto rb) { k_attend<lanes, rb><<<attend_grid(p), 32 * kWarps, 0, st>>>(p); });
+        by_shape(p.head, p.rb,
+                 [&](auto lanes, auto rb) { k_attend<lanes, rb><<<attend_grid(p), attend_threads(p), 0, st>>>(p); });
         check_launch();
         if (p.splits > 1) {
-            k_attend_join<<<(unsigned)ceil_div(p.queries * p.heads, 4), 128, 0, st>>>(p);
+            k_attend_join<<<(unsigned)(p.queries * p.heads), 128, 0, st>>>(p);
             check_launch();
         }
     });
@@ -758,7 +920,7 @@ mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_
 
 int64_t mdh_attend_backward_workspace(const mdh_attend_args* a, int32_t want_dbias) {
     if (!has_sizes(a)) return 0;
-    int64_t need = backward_part(cut_of(a));
+    int64_t need = backward_part(layout_of(a));
     if (want_dbias) need += a->queries * a->heads * 8 + a->queries * a->heads * (int64_t)a->found * 8;
     return need;
 }
@@ -787,15 +949,16 @@ mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, c
         p.out = dq;
         p.dout = dout;
         p.lse_in = lse;
-        by_shape(p.head, p.shared,
-                 [&](auto lanes, auto rb) { k_attend_backward<lanes, rb><<<attend_grid(p), 32 * kWarps, 0, st>>>(p); });
+        by_shape(p.head, p.rb, [&](auto lanes, auto rb) {
+            k_attend_backward<lanes, rb><<<attend_grid(p), attend_threads(p), 0, st>>>(p);
+        });
         check_launch();
         if (p.splits > 1) {
-            k_attend_backward_join<<<(unsigned)ceil_div(p.queries * p.heads, 4), 128, 0, st>>>(p);
+            k_attend_backward_join<<<(unsigned)(p.queries * p.heads), 128, 0, st>>>(p);
             check_launch();
         }
         if (dbias && p.found) {
-            k_attend_dbias<<<(unsigned)bias_blocks, 256, 0, st>>>(p.pd, p.sum_d, p.queries, p.heads, p.found, dbias);
+            k_attend_dbias<<<(unsigned)bias_blocks, 256, 0, st>>>(p, dbias);
             check_launch();
         }
     });
