@@ -36,7 +36,7 @@ namespace {
 
 using namespace op;
 
-constexpr int kMaxWarps = 12;         // of a block
+constexpr int kMaxWarps = 8;          // of a block
 constexpr int kRound = 128;           // entries of the list that a warp looks at at a time
 constexpr int kMaxHead = 256;
 constexpr int kMaxShared = 4;         // query heads of a unit
@@ -49,7 +49,6 @@ struct CodeView {
     int group, n_groups;
     uint32_t flip;        // 0x80808080 for int8: the stored byte becomes c + 128
     float scale, base;    // affine: value = base + scale c
-    bool vec;             // 8-byte loads of codes are aligned
 };
 
 struct AttendParams {
@@ -61,6 +60,7 @@ struct AttendParams {
     int64_t q_stride, q_head_stride, ids_stride, bias_stride, slots;
     int64_t queries;
     int found, heads, shared, head, dtype;
+    bool q_vec, dout_vec;  // heads start on 16 bytes
     float scale, cap, inv_cap;
     int r_blocks, rb;      // units of a row's head, query heads of each (the last may have fewer)
     int units;             // of a query
@@ -68,6 +68,7 @@ struct AttendParams {
     int unit_blocks;       // blocks that share a query's units
     int slices;            // warps of a block that share a unit
     int splits, split_len; // ranges of a list over blocks, entries of each
+    bool aligned;          // rows of both caches start and step on 8 bytes
     void* out;
     float* lse;
     float* part;           // splits > 1: vectors [splits][queries][heads][head] (backward: two of them), then float2
@@ -118,10 +119,10 @@ __device__ __forceinline__ float tanh_fast(float x) {
     return 1.0f - __fdividef(2.0f, exp2_fast(fminf(x * (2.0f * kLog2e), 126.0f)) + 1.0f);
 }
 
-// 8 codes of a row.
-__device__ __forceinline__ uint2 load_codes(const CodeView& c, int64_t slot, int e) {
-    const uint8_t* p = c.codes + slot * c.stride + e;
-    if (c.vec) return __ldg(reinterpret_cast<const uint2*>(p));
+// 8 codes of a row; ALIGNED: rows start and step on 8 bytes.
+template <bool ALIGNED>
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p) {
+    if (ALIGNED) return __ldg(reinterpret_cast<const uint2*>(p));
     uint2 r = make_uint2(0, 0);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -129,9 +130,6 @@ __device__ __forceinline__ uint2 load_codes(const CodeView& c, int64_t slot, int
         r.y |= (uint32_t)p[4 + j] << (8 * j);
     }
     return r;
-}
-__device__ __forceinline__ float load_scale(const CodeView& c, int64_t slot, int group) {
-    return c.scales ? __ldg(c.scales + slot * c.n_groups + group) : c.scale;
 }
 // The codes c as four pairs of floats.
 __device__ __forceinline__ void code_pairs(uint2 raw, uint32_t flip, u64 (&c)[4]) {
@@ -152,21 +150,45 @@ __device__ __forceinline__ float dot_pairs(const u64 (&a)[4], const u64 (&b)[4])
     return f.x + f.y;
 }
 
-// 8 elements of q's type at p + i.
-__device__ __forceinline__ void load_elements(const void* p, int64_t i, int dtype, float (&v)[8]) {
+// 8 elements of q's type at p + i; vec: on a 16-byte boundary.
+__device__ __forceinline__ void load_elements(const void* p, int64_t i, int dtype, bool vec, float (&v)[8]) {
+    if (dtype == MDH_F32) {
+        const float* f = static_cast<const float*>(p) + i;
+        if (vec) {
+            const float4 x = __ldg(reinterpret_cast<const float4*>(f)), y = __ldg(reinterpret_cast<const float4*>(f) + 1);
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+        } else {
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-        v[j] = dtype == MDH_F32    ? static_cast<const float*>(p)[i + j]
-               : dtype == MDH_BF16 ? to_f32(static_cast<const bf16*>(p)[i + j])
-                                   : to_f32(static_cast<const f16*>(p)[i + j]);
-}
-__device__ __forceinline__ void store_elements(void* p, int64_t i, int dtype, const float (&v)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        if (dtype == MDH_F32) static_cast<float*>(p)[i + j] = v[j];
-        else if (dtype == MDH_BF16) static_cast<bf16*>(p)[i + j] = from_f32<bf16>(v[j]);
-        else static_cast<f16*>(p)[i + j] = from_f32<f16>(v[j]);
+            for (int j = 0; j < 8; j++) v[j] = f[j];
+        }
+        return;
     }
+    const uint16_t* h = static_cast<const uint16_t*>(p) + i;
+    uint32_t w[4];
+    if (vec) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(h));
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (dtype == MDH_BF16) {
+            v[2 * j] = __uint_as_float(w[j] << 16);
+            v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        }
+    }
+}
+// Two elements at the even place i of an aligned output.
+__device__ __forceinline__ void store_pair(void* p, int64_t i, int dtype, float x, float y) {
+    if (dtype == MDH_F32) *reinterpret_cast<float2*>(static_cast<float*>(p) + i) = make_float2(x, y);
+    else if (dtype == MDH_BF16)
+        *reinterpret_cast<__nv_bfloat162*>(static_cast<bf16*>(p) + i) = __floats2bfloat162_rn(x, y);
+    else *reinterpret_cast<__half2*>(static_cast<f16*>(p) + i) = __floats2half2_rn(x, y);
 }
 
 // What a warp works on.
@@ -212,23 +234,26 @@ struct Entries {
 };
 // Lists the visible entries of [j0, j1), at most kRound a warp.
 __device__ __forceinline__ int list_entries(const AttendParams& a, Entries& e, int64_t i, int32_t doc, int j0, int j1) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warps = min((int)blockDim.x >> 5, (j1 - j0 + kRound - 1) / kRound);  // that look at entries
     int slot[kRound / 32], n = 0;
     float bias[kRound / 32];
     uint32_t seen[kRound / 32];
+    if (warp < warps) {
 #pragma unroll
-    for (int c = 0; c < kRound / 32; c++) {
-        const int j = j0 + warp * kRound + c * 32 + lane;
-        slot[c] = -1;
-        if (j < j1) slot[c] = entry_slot(a, i, j, doc, bias[c]);
-    }
+        for (int c = 0; c < kRound / 32; c++) {
+            const int j = j0 + warp * kRound + c * 32 + lane;
+            slot[c] = -1;
+            if (j < j1) slot[c] = entry_slot(a, i, j, doc, bias[c]);
+        }
 #pragma unroll
-    for (int c = 0; c < kRound / 32; c++) {
-        seen[c] = __ballot_sync(0xffffffffu, slot[c] >= 0);
-        n += __popc(seen[c]);
+        for (int c = 0; c < kRound / 32; c++) {
+            seen[c] = __ballot_sync(0xffffffffu, slot[c] >= 0);
+            n += __popc(seen[c]);
+        }
     }
     __syncthreads();  // the previous list has been read
-    if (lane == 0) e.count[warp] = n;
+    if (lane == 0 && warp < warps) e.count[warp] = n;
     __syncthreads();
     int before = 0, total = 0;
     for (int k = 0; k < warps; k++) {
@@ -236,6 +261,7 @@ __device__ __forceinline__ int list_entries(const AttendParams& a, Entries& e, i
         if (k < warp) before += x;
         total += x;
     }
+    if (warp < warps) {
 #pragma unroll
     for (int c = 0; c < kRound / 32; c++) {
         if (slot[c] >= 0) {
@@ -245,6 +271,7 @@ __device__ __forceinline__ int list_entries(const AttendParams& a, Entries& e, i
             e.place[at] = j0 + warp * kRound + c * 32 + lane;
         }
         before += __popc(seen[c]);
+    }
     }
     __syncthreads();
     return total;
@@ -314,11 +341,11 @@ struct Steps {
 // q (times the scale) or dout of a unit's heads as float pairs; sums of each.
 template <int RB>
 __device__ __forceinline__ void load_heads(const void* p, int64_t at, int64_t stride, int dtype, const Work& w,
-                                           float scale, u64 (&v)[RB][4], float (&sum)[RB]) {
+                                           bool vec, float scale, u64 (&v)[RB][4], float (&sum)[RB]) {
 #pragma unroll
     for (int r = 0; r < RB; r++) {
         float x[8] = {};
-        if (w.live && r < w.nr) load_elements(p, at + (w.h0 + r) * stride + w.d0, dtype, x);
+        if (w.live && r < w.nr) load_elements(p, at + (w.h0 + r) * stride + w.d0, dtype, vec, x);
         sum[r] = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; j++) sum[r] += x[j] *= scale;
@@ -326,6 +353,35 @@ __device__ __forceinline__ void load_heads(const void* p, int64_t at, int64_t st
         for (int j = 0; j < 4; j++) v[r][j] = pair(x[2 * j], x[2 * j + 1]);
     }
 }
+
+// Four pairs of elements a lane, summed over the warp's side-by-side entries
+// by halving: PAIRS finished pairs a lane, elements w.d0 + 2 first_pair() + 0
+// .. 2 PAIRS - 1.
+template <int LANES>
+struct Vector {
+    static constexpr int PAIRS = LANES == 32 ? 4 : LANES == 16 ? 2 : 1;
+    static __device__ __forceinline__ void sum(u64 (&v)[4]) {
+        const int lane = threadIdx.x & 31;
+        if (LANES <= 16) {
+            const bool up = lane & 16;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                v[j] = add2(up ? v[2 + j] : v[j], __shfl_xor_sync(0xffffffffu, up ? v[j] : v[2 + j], 16));
+        }
+        if (LANES <= 8) {
+            const bool up = lane & 8;
+            v[0] = add2(up ? v[1] : v[0], __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 8));
+        }
+#pragma unroll
+        for (int o = 4; o >= LANES; o >>= 1) v[0] = add2(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+    }
+    static __device__ __forceinline__ int first_pair() {
+        const int lane = threadIdx.x & 31;
+        return LANES == 32 ? 0 : LANES == 16 ? lane >> 4 << 1 : lane >> 4 << 1 | (lane >> 3 & 1);
+    }
+    // One lane for each of the elements (lanes between LANES and 8 repeat others).
+    static __device__ __forceinline__ bool writer() { return LANES >= 8 || (threadIdx.x & 7) < LANES; }
+};
 
 // The scaled, capped and biased score of a finished sum; t = tanh of the capped one.
 __device__ __forceinline__ float score_of(const AttendParams& a, float x, float bias, float& t) {
@@ -346,30 +402,62 @@ __device__ __forceinline__ float join(float m, float mo, float& mine, float& oth
     return top;
 }
 
-__device__ __forceinline__ void finish_forward(const AttendParams& a, int64_t at, int d0, bool first, float (&v)[8],
-                                               float m, float l) {
+// The finished pair of elements d, d + 1 of (query, head) `at`.
+__device__ __forceinline__ void finish_forward(const AttendParams& a, int64_t at, int d, float2 v, float m, float l) {
     const float inv = l != 0.0f ? 1.0f / l : 0.0f, base = l != 0.0f ? a.v.base : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = fmaf(v[j], inv, base);
-    store_elements(a.out, at * a.head + d0, a.dtype, v);
-    if (first) a.lse[at] = l != 0.0f ? m + logf(l) : -INFINITY;
+    store_pair(a.out, at * a.head + d, a.dtype, fmaf(v.x, inv, base), fmaf(v.y, inv, base));
+    if (d == 0) a.lse[at] = l != 0.0f ? m + logf(l) : -INFINITY;
 }
-__device__ __forceinline__ void finish_backward(const AttendParams& a, int64_t at, int d0, bool first, float (&x)[8],
-                                                const float (&y)[8], float d, float p) {
-    const float inv = p != 0.0f ? 1.0f / p : 0.0f;
-    d *= inv;
-#pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = a.scale * inv * (x[j] - d * y[j]);
-    store_elements(a.out, at * a.head + d0, a.dtype, x);
-    if (a.sum_d && first) a.sum_d[at] = make_float2(d, inv);
+__device__ __forceinline__ void finish_backward(const AttendParams& a, int64_t at, int d, float2 x, float2 y, float sum_d,
+                                                float sum_p) {
+    const float inv = sum_p != 0.0f ? 1.0f / sum_p : 0.0f, f = a.scale * inv;
+    sum_d *= inv;
+    store_pair(a.out, at * a.head + d, a.dtype, f * (x.x - sum_d * y.x), f * (x.y - sum_d * y.y));
+    if (a.sum_d && d == 0) a.sum_d[at] = make_float2(sum_d, inv);
 }
 
-template <int LANES, int RB>
-__global__ void __launch_bounds__(32 * kMaxWarps) k_attend(const __grid_constant__ AttendParams a) {
+// The codes and scales of STEPS entries side by side, in flight.
+template <int STEPS>
+struct Rows {
+    uint2 k[STEPS], v[STEPS];
+    float ks[STEPS], vs[STEPS];
+};
+// Where a lane reads rows.
+struct Places {
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    int64_t k_stride, v_stride;
+    int kn, vn;
+    float k_scale, v_scale;
+};
+__device__ __forceinline__ Places places_of(const AttendParams& a, const Work& w) {
+    return {a.k.codes + w.e0, a.v.codes + w.e0, a.k.scales ? a.k.scales + w.e0 / a.k.group : nullptr,
+            a.v.scales ? a.v.scales + w.e0 / a.v.group : nullptr, a.k.stride, a.v.stride, a.k.n_groups, a.v.n_groups,
+            a.k.scale, a.v.scale};
+}
+template <bool ALIGNED, int STEPS, int ENTRIES>
+__device__ __forceinline__ void load_rows(Rows<STEPS>& r, const Places& p, const int* slots, int first, int hi, bool live) {
+#pragma unroll
+    for (int u = 0; u < STEPS; u++) {
+        const int e = first + u * ENTRIES;
+        r.k[u] = r.v[u] = make_uint2(0, 0);
+        r.ks[u] = r.vs[u] = 0.0f;
+        if (e < hi && live) {
+            const int64_t slot = slots[e];
+            r.k[u] = load_codes<ALIGNED>(p.k + slot * p.k_stride);
+            r.v[u] = load_codes<ALIGNED>(p.v + slot * p.v_stride);
+            r.ks[u] = p.ks ? __ldg(p.ks + slot * p.kn) : p.k_scale;
+            r.vs[u] = p.vs ? __ldg(p.vs + slot * p.vn) : p.v_scale;
+        }
+    }
+}
+
+template <int LANES, int RB, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(const __grid_constant__ AttendParams a) {
     using St = Steps<LANES, RB>;
     using Sums = typename St::Sums;
     constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP, ENTRIES = St::ENTRIES;
-    __shared__ union {
+    __shared__ union alignas(16) {
         Entries e;
         float joined[kMaxWarps][LANES * 8 + 2];  // vector, m, l
     } sm;
@@ -377,7 +465,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps) k_attend(const __grid_constant
     const Work w = work_of<LANES>(a);
     u64 q[RB][4], acc[RB][4];
     float kb[RB];
-    load_heads<RB>(a.q, w.i * a.q_stride, a.q_head_stride, a.dtype, w, a.scale, q, kb);
+    load_heads<RB>(a.q, w.i * a.q_stride, a.q_head_stride, a.dtype, w, a.q_vec, a.scale, q, kb);
 #pragma unroll
     for (int r = 0; r < RB; r++) {
         kb[r] *= a.k.base;
@@ -387,7 +475,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps) k_attend(const __grid_constant
     float m[KEEP], l[KEEP];  // of the lane's own values' heads
 #pragma unroll
     for (int x = 0; x < KEEP; x++) m[x] = -INFINITY, l[x] = 0.0f;
-    const int kg = w.e0 / a.k.group, vg = w.e0 / a.v.group;
+    const Places places = places_of(a, w);
     const int32_t doc = a.query_docs ? a.query_docs[w.i] : 0;
     const int j0 = (int)min((int64_t)blockIdx.y * a.split_len, (int64_t)a.found);
     const int j1 = (int)min((int64_t)j0 + a.split_len, (int64_t)a.found);
@@ -395,29 +483,18 @@ __global__ void __launch_bounds__(32 * kMaxWarps) k_attend(const __grid_constant
         int lo, hi;
         slice_of(list_entries(a, sm.e, w.i, doc, from, j1), w.slice, a.slices, STEPS * ENTRIES, lo, hi);
         if (w.nr == 0) hi = lo;
+        Rows<STEPS> next;
+        load_rows<ALIGNED, STEPS, ENTRIES>(next, places, sm.e.slot, lo + sub, hi, w.live);
         for (int t = lo; t < hi; t += STEPS * ENTRIES) {
-            uint2 kraw[STEPS], vraw[STEPS];
-            float ks[STEPS], vs[STEPS];
-#pragma unroll
-            for (int u = 0; u < STEPS; u++) {
-                const int e = t + u * ENTRIES + sub;
-                kraw[u] = vraw[u] = make_uint2(0, 0);
-                ks[u] = vs[u] = 0.0f;
-                if (e < hi && w.live) {
-                    const int slot = sm.e.slot[e];
-                    kraw[u] = load_codes(a.k, slot, w.e0);
-                    vraw[u] = load_codes(a.v, slot, w.e0);
-                    ks[u] = load_scale(a.k, slot, kg);
-                    vs[u] = load_scale(a.v, slot, vg);
-                }
-            }
+            const Rows<STEPS> now = next;  // the next entries are loaded while these are used
+            load_rows<ALIGNED, STEPS, ENTRIES>(next, places, sm.e.slot, t + STEPS * ENTRIES + sub, hi, w.live);
             float s[STEPS * RP];
 #pragma unroll
             for (int u = 0; u < STEPS; u++) {
                 u64 c[4];
-                code_pairs(kraw[u], a.k.flip, c);
+                code_pairs(now.k[u], a.k.flip, c);
 #pragma unroll
-                for (int r = 0; r < RP; r++) s[u * RP + r] = r < RB ? fmaf(ks[u], dot_pairs(q[r < RB ? r : 0], c), kb[r < RB ? r : 0]) : 0.0f;
+                for (int r = 0; r < RP; r++) s[u * RP + r] = r < RB ? fmaf(now.ks[u], dot_pairs(q[r < RB ? r : 0], c), kb[r < RB ? r : 0]) : 0.0f;
             }
             Sums::sum(s);
             float p[KEEP], keep[KEEP];
@@ -449,10 +526,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps) k_attend(const __grid_constant
 #pragma unroll
             for (int u = 0; u < STEPS; u++) {
                 u64 c[4];
-                code_pairs(vraw[u], a.v.flip, c);
+                code_pairs(now.v[u], a.v.flip, c);
 #pragma unroll
                 for (int r = 0; r < RB; r++) {
-                    const float pv = Sums::get(p, u * RP + r) * vs[u];
+                    const float pv = Sums::get(p, u * RP + r) * now.vs[u];
                     const u64 pp = pair(pv, pv);
 #pragma unroll
                     for (int j = 0; j < 4; j++) acc[r][j] = fma2(pp, c[j], acc[r][j]);
@@ -463,49 +540,48 @@ __global__ void __launch_bounds__(32 * kMaxWarps) k_attend(const __grid_constant
 #pragma unroll
     for (int x = 0; x < KEEP; x++)
         St::over_entries([&](int o) { l[x] += __shfl_xor_sync(0xffffffffu, l[x], o); });
+    using Vec = Vector<LANES>;
+    const int d0 = w.d0 + 2 * Vec::first_pair();
 #pragma unroll
     for (int r = 0; r < RB; r++) {
-        float v[8], mm = Sums::get(m, r), ll = Sums::get(l, r);
+        float2 v[Vec::PAIRS];
+        float mm = Sums::get(m, r), ll = Sums::get(l, r);
+        Vec::sum(acc[r]);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            u64 x = acc[r][j];
-#pragma unroll
-            for (int o = LANES; o < 32; o <<= 1) x = add2(x, __shfl_xor_sync(0xffffffffu, x, o));
-            const float2 f = unpair(x);
-            v[2 * j] = f.x, v[2 * j + 1] = f.y;
-        }
-        const bool write = r < w.nr && w.slice == 0 && lane < LANES && w.live;
+        for (int j = 0; j < Vec::PAIRS; j++) v[j] = unpair(acc[r][j]);
         if (a.slices > 1) {
             __syncthreads();  // the list, or the previous head's vectors, have been read
-            if (lane < LANES) {
-                float* dst = sm.joined[warp];
+            float* mine = sm.joined[warp];
+            if (Vec::writer()) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) dst[w.d0 + j] = v[j];
-                if (lane == 0) dst[LANES * 8] = mm, dst[LANES * 8 + 1] = ll;
+                for (int j = 0; j < Vec::PAIRS; j++) *reinterpret_cast<float2*>(mine + d0 + 2 * j) = v[j];
             }
+            if (lane == 0) mine[LANES * 8] = mm, mine[LANES * 8 + 1] = ll;
             __syncthreads();
-            if (write) {
+            if (w.slice == 0) {
                 for (int k = 1; k < a.slices; k++) {
                     const float* src = sm.joined[warp + k];
-                    float mine, other;
-                    mm = join(mm, src[LANES * 8], mine, other);
-                    ll = ll * mine + src[LANES * 8 + 1] * other;
+                    float f, g;
+                    mm = join(mm, src[LANES * 8], f, g);
+                    ll = ll * f + src[LANES * 8 + 1] * g;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = v[j] * mine + src[w.d0 + j] * other;
+                    for (int j = 0; j < Vec::PAIRS; j++) {
+                        const float2 o = *reinterpret_cast<const float2*>(src + d0 + 2 * j);
+                        v[j].x = v[j].x * f + o.x * g;
+                        v[j].y = v[j].y * f + o.y * g;
+                    }
                 }
             }
         }
-        if (!write) continue;
-        const int64_t at = w.i * a.heads + w.h0 + r;
-        if (a.part) {
-            const int64_t n = a.queries * a.heads, row = (int64_t)blockIdx.y * n + at;
-            float4* dst = reinterpret_cast<float4*>(a.part + row * a.head + w.d0);
-            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-            if (lane == 0) reinterpret_cast<float2*>(a.part + a.splits * n * a.head)[row] = make_float2(mm, ll);
-        } else {
-            finish_forward(a, at, w.d0, lane == 0, v, mm, ll);
+        if (r >= w.nr || w.slice != 0 || !w.live || !Vec::writer()) continue;
+        const int64_t at = w.i * a.heads + w.h0 + r, n = a.queries * a.heads, row = (int64_t)blockIdx.y * n + at;
+#pragma unroll
+        for (int j = 0; j < Vec::PAIRS; j++) {
+            const int d = d0 + 2 * j;
+            if (a.part) *reinterpret_cast<float2*>(a.part + row * a.head + d) = v[j];
+            else finish_forward(a, at, d, v[j], mm, ll);
         }
+        if (a.part && lane == 0) reinterpret_cast<float2*>(a.part + a.splits * n * a.head)[row] = make_float2(mm, ll);
     }
 }
 
@@ -544,18 +620,20 @@ __global__ void __launch_bounds__(128) k_attend_join(const __grid_constant__ Att
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] += joined[k][d0 + j];
     }
-    if (d0 < a.head) finish_forward(a, at, d0, lane == 0, v, m, l);
+    if (d0 < a.head)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) finish_forward(a, at, d0 + j, make_float2(v[j], v[j + 1]), m, l);
 }
 
 // A, B, D and the weights' own sum P of the lists' slices; dq = scale (A - (D / P) B) / P.
 // P is 1 up to rounding, except where lse cannot hold its own digits beside
 // scores of 1e9 and more (a mask of the type's lowest value throughout).
-template <int LANES, int RB>
-__global__ void __launch_bounds__(32 * kMaxWarps) k_attend_backward(const __grid_constant__ AttendParams a) {
+template <int LANES, int RB, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_backward(const __grid_constant__ AttendParams a) {
     using St = Steps<LANES, RB>;
     using Sums = typename St::Sums;
     constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP, ENTRIES = St::ENTRIES;
-    __shared__ union {
+    __shared__ union alignas(16) {
         Entries e;
         float joined[kMaxWarps][LANES * 16 + 2];  // A, B, D, P
     } sm;
@@ -563,8 +641,8 @@ __global__ void __launch_bounds__(32 * kMaxWarps) k_attend_backward(const __grid
     const Work w = work_of<LANES>(a);
     u64 q[RB][4], g[RB][4], va[RB][4], vb[RB][4];
     float kb[RB], gb[RB];
-    load_heads<RB>(a.q, w.i * a.q_stride, a.q_head_stride, a.dtype, w, a.scale, q, kb);
-    load_heads<RB>(a.dout, w.i * a.heads * a.head, a.head, a.dtype, w, 1.0f, g, gb);
+    load_heads<RB>(a.q, w.i * a.q_stride, a.q_head_stride, a.dtype, w, a.q_vec, a.scale, q, kb);
+    load_heads<RB>(a.dout, w.i * a.heads * a.head, a.head, a.dtype, w, a.dout_vec, 1.0f, g, gb);
 #pragma unroll
     for (int r = 0; r < RB; r++) {
         kb[r] *= a.k.base;
@@ -579,7 +657,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps) k_attend_backward(const __grid
         z[x] = r < w.nr ? a.lse_in[w.i * a.heads + w.h0 + r] : 0.0f;
         dsum[x] = psum[x] = 0.0f;
     }
-    const int kg = w.e0 / a.k.group, vg = w.e0 / a.v.group;
+    const Places places = places_of(a, w);
     const int32_t doc = a.query_docs ? a.query_docs[w.i] : 0;
     const u64 kbase = pair(a.k.base, a.k.base);
     const int j0 = (int)min((int64_t)blockIdx.y * a.split_len, (int64_t)a.found);
@@ -588,32 +666,21 @@ __global__ void __launch_bounds__(32 * kMaxWarps) k_attend_backward(const __grid
         int lo, hi;
         slice_of(list_entries(a, sm.e, w.i, doc, from, j1), w.slice, a.slices, STEPS * ENTRIES, lo, hi);
         if (w.nr == 0) hi = lo;
+        Rows<STEPS> next;
+        load_rows<ALIGNED, STEPS, ENTRIES>(next, places, sm.e.slot, lo + sub, hi, w.live);
         for (int t = lo; t < hi; t += STEPS * ENTRIES) {
-            uint2 kraw[STEPS], vraw[STEPS];
-            float ks[STEPS], vs[STEPS];
-#pragma unroll
-            for (int u = 0; u < STEPS; u++) {
-                const int e = t + u * ENTRIES + sub;
-                kraw[u] = vraw[u] = make_uint2(0, 0);
-                ks[u] = vs[u] = 0.0f;
-                if (e < hi && w.live) {
-                    const int slot = sm.e.slot[e];
-                    kraw[u] = load_codes(a.k, slot, w.e0);
-                    vraw[u] = load_codes(a.v, slot, w.e0);
-                    ks[u] = load_scale(a.k, slot, kg);
-                    vs[u] = load_scale(a.v, slot, vg);
-                }
-            }
+            const Rows<STEPS> now = next;  // the next entries are loaded while these are used
+            load_rows<ALIGNED, STEPS, ENTRIES>(next, places, sm.e.slot, t + STEPS * ENTRIES + sub, hi, w.live);
             float s[STEPS * RP], dp[STEPS * RP];
 #pragma unroll
             for (int u = 0; u < STEPS; u++) {
                 u64 c[4];
-                code_pairs(kraw[u], a.k.flip, c);
+                code_pairs(now.k[u], a.k.flip, c);
 #pragma unroll
-                for (int r = 0; r < RP; r++) s[u * RP + r] = r < RB ? fmaf(ks[u], dot_pairs(q[r < RB ? r : 0], c), kb[r < RB ? r : 0]) : 0.0f;
-                code_pairs(vraw[u], a.v.flip, c);
+                for (int r = 0; r < RP; r++) s[u * RP + r] = r < RB ? fmaf(now.ks[u], dot_pairs(q[r < RB ? r : 0], c), kb[r < RB ? r : 0]) : 0.0f;
+                code_pairs(now.v[u], a.v.flip, c);
 #pragma unroll
-                for (int r = 0; r < RP; r++) dp[u * RP + r] = r < RB ? fmaf(vs[u], dot_pairs(g[r < RB ? r : 0], c), gb[r < RB ? r : 0]) : 0.0f;
+                for (int r = 0; r < RP; r++) dp[u * RP + r] = r < RB ? fmaf(now.vs[u], dot_pairs(g[r < RB ? r : 0], c), gb[r < RB ? r : 0]) : 0.0f;
             }
             Sums::sum(s);
             Sums::sum(dp);
@@ -637,8 +704,8 @@ __global__ void __launch_bounds__(32 * kMaxWarps) k_attend_backward(const __grid
 #pragma unroll
             for (int u = 0; u < STEPS; u++) {
                 u64 c[4];
-                code_pairs(kraw[u], a.k.flip, c);
-                const u64 kss = pair(ks[u], ks[u]);
+                code_pairs(now.k[u], a.k.flip, c);
+                const u64 kss = pair(now.ks[u], now.ks[u]);
 #pragma unroll
                 for (int j = 0; j < 4; j++) c[j] = fma2(kss, c[j], kbase);  // the key's values
 #pragma unroll
@@ -660,54 +727,56 @@ __global__ void __launch_bounds__(32 * kMaxWarps) k_attend_backward(const __grid
             dsum[x] += __shfl_xor_sync(0xffffffffu, dsum[x], o);
             psum[x] += __shfl_xor_sync(0xffffffffu, psum[x], o);
         });
+    using Vec = Vector<LANES>;
+    const int d0 = w.d0 + 2 * Vec::first_pair();
 #pragma unroll
     for (int r = 0; r < RB; r++) {
-        float x[8], y[8], d = Sums::get(dsum, r), p = Sums::get(psum, r);
+        float2 x[Vec::PAIRS], y[Vec::PAIRS];
+        float sd = Sums::get(dsum, r), sp = Sums::get(psum, r);
+        Vec::sum(va[r]);
+        Vec::sum(vb[r]);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            u64 xa = va[r][j], xb = vb[r][j];
-#pragma unroll
-            for (int o = LANES; o < 32; o <<= 1) {
-                xa = add2(xa, __shfl_xor_sync(0xffffffffu, xa, o));
-                xb = add2(xb, __shfl_xor_sync(0xffffffffu, xb, o));
-            }
-            const float2 f = unpair(xa), h = unpair(xb);
-            x[2 * j] = f.x, x[2 * j + 1] = f.y, y[2 * j] = h.x, y[2 * j + 1] = h.y;
-        }
-        const bool write = r < w.nr && w.slice == 0 && lane < LANES && w.live;
+        for (int j = 0; j < Vec::PAIRS; j++) x[j] = unpair(va[r][j]), y[j] = unpair(vb[r][j]);
         if (a.slices > 1) {
             __syncthreads();  // the list, or the previous head's vectors, have been read
-            if (lane < LANES) {
-                float* dst = sm.joined[warp];
+            float* mine = sm.joined[warp];
+            if (Vec::writer()) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) dst[w.d0 + j] = x[j], dst[LANES * 8 + w.d0 + j] = y[j];
-                if (lane == 0) dst[LANES * 16] = d, dst[LANES * 16 + 1] = p;
+                for (int j = 0; j < Vec::PAIRS; j++) {
+                    *reinterpret_cast<float2*>(mine + d0 + 2 * j) = x[j];
+                    *reinterpret_cast<float2*>(mine + LANES * 8 + d0 + 2 * j) = y[j];
+                }
             }
+            if (lane == 0) mine[LANES * 16] = sd, mine[LANES * 16 + 1] = sp;
             __syncthreads();
-            if (write) {
+            if (w.slice == 0) {
                 for (int k = 1; k < a.slices; k++) {
                     const float* src = sm.joined[warp + k];
-                    d += src[LANES * 16];
-                    p += src[LANES * 16 + 1];
+                    sd += src[LANES * 16];
+                    sp += src[LANES * 16 + 1];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] += src[w.d0 + j], y[j] += src[LANES * 8 + w.d0 + j];
+                    for (int j = 0; j < Vec::PAIRS; j++) {
+                        const float2 o = *reinterpret_cast<const float2*>(src + d0 + 2 * j);
+                        const float2 h = *reinterpret_cast<const float2*>(src + LANES * 8 + d0 + 2 * j);
+                        x[j].x += o.x, x[j].y += o.y, y[j].x += h.x, y[j].y += h.y;
+                    }
                 }
             }
         }
-        if (!write) continue;
-        const int64_t at = w.i * a.heads + w.h0 + r;
-        if (a.part) {
-            const int64_t n = a.queries * a.heads, row = (int64_t)blockIdx.y * n + at;
-            float4* dst = reinterpret_cast<float4*>(a.part + row * 2 * a.head + w.d0);
-            float4* dsb = reinterpret_cast<float4*>(a.part + (row * 2 + 1) * a.head + w.d0);
-            dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-            dst[1] = make_float4(x[4], x[5], x[6], x[7]);
-            dsb[0] = make_float4(y[0], y[1], y[2], y[3]);
-            dsb[1] = make_float4(y[4], y[5], y[6], y[7]);
-            if (lane == 0) reinterpret_cast<float2*>(a.part + a.splits * n * 2 * a.head)[row] = make_float2(d, p);
-        } else {
-            finish_backward(a, at, w.d0, lane == 0, x, y, d, p);
+        if (r >= w.nr || w.slice != 0 || !w.live || !Vec::writer()) continue;
+        const int64_t at = w.i * a.heads + w.h0 + r, n = a.queries * a.heads, row = (int64_t)blockIdx.y * n + at;
+#pragma unroll
+        for (int j = 0; j < Vec::PAIRS; j++) {
+            const int d = d0 + 2 * j;
+            if (a.part) {
+                *reinterpret_cast<float2*>(a.part + row * 2 * a.head + d) = x[j];
+                *reinterpret_cast<float2*>(a.part + (row * 2 + 1) * a.head + d) = y[j];
+            } else {
+                finish_backward(a, at, d, x[j], y[j], sd, sp);
+            }
         }
+        if (a.part && lane == 0)
+            reinterpret_cast<float2*>(a.part + a.splits * n * 2 * a.head)[row] = make_float2(sd, sp);
     }
 }
 
@@ -740,7 +809,10 @@ __global__ void __launch_bounds__(128) k_attend_backward_join(const __grid_const
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] += joined[k][d0 + j], y[j] += joined[k][kMaxHead + d0 + j];
     }
-    if (d0 < a.head) finish_backward(a, at, d0, lane == 0, x, y, d, p);
+    if (d0 < a.head)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+            finish_backward(a, at, d0 + j, make_float2(x[j], x[j + 1]), make_float2(y[j], y[j + 1]), d, p);
 }
 
 // dbias[i][j] = sum over heads of (p dP - p D / P) / P, in head order; 0 at hidden entries.
@@ -760,6 +832,7 @@ __global__ void __launch_bounds__(256) k_attend_dbias(const __grid_constant__ At
     dbias[at] = v;
 }
 
+bool rows_on_8(const RowsView& r) { return reinterpret_cast<uintptr_t>(r.codes) % 8 == 0 && r.stride % 8 == 0; }
 CodeView code_view(const RowsView& r) {
     CodeView c{};
     c.codes = r.codes;
@@ -770,24 +843,24 @@ CodeView code_view(const RowsView& r) {
     c.flip = r.affine ? 0u : 0x80808080u;
     c.scale = r.step;
     c.base = r.affine ? r.lo + 128.0f * r.step : 0.0f;
-    c.vec = reinterpret_cast<uintptr_t>(r.codes) % 8 == 0 && r.stride % 8 == 0;
     return c;
 }
 
 // How a call is laid out over blocks.  A block takes up to kMaxWarps units of
-// a query; where they are few, several warps share a unit's list, up to 8
-// warps a block and no slice below kMinSlice entries; where the blocks do not
-// fill the GPU, a list is cut into ranges for several blocks.
+// a query; where the calls' units do not fill the GPU, several warps of a
+// block share a unit's list, and then blocks take ranges of it; no slice is
+// below kMinSlice entries.
 void lay_out(AttendParams& p) {
+    constexpr int64_t kFill = 148 * 16;  // warps
     p.r_blocks = (int)ceil_div(p.shared, kMaxShared);
     p.rb = (int)ceil_div(p.shared, p.r_blocks);
     p.units = p.heads / p.shared * p.r_blocks;
     p.unit_blocks = (int)ceil_div(p.units, kMaxWarps);
     p.block_units = (int)ceil_div(p.units, p.unit_blocks);
-    const int64_t slices = std::min<int64_t>(8 / std::min(8, p.block_units), ceil_div(p.found, kMinSlice));
-    p.slices = (int)std::max<int64_t>(1, slices);
-    const int64_t warps = std::max<int64_t>(1, p.queries * p.unit_blocks * p.block_units * p.slices);
-    const int64_t splits = std::min(ceil_div(p.found, p.slices * kMinSlice), 148 * 16 / warps);
+    const int64_t units = std::max<int64_t>(1, p.queries * p.unit_blocks * p.block_units);
+    p.slices = (int)std::max<int64_t>(
+        1, std::min({(int64_t)kMaxWarps / p.block_units, ceil_div(p.found, kMinSlice), ceil_div(kFill, units)}));
+    const int64_t splits = std::min(ceil_div(p.found, p.slices * kMinSlice), kFill / (units * p.slices));
     p.split_len = (int)std::max<int64_t>(1, ceil_div(p.found, std::max<int64_t>(1, splits)));
     p.splits = (int)std::max<int64_t>(1, ceil_div(p.found, p.split_len));
 }
@@ -817,6 +890,10 @@ AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const 
                 "attend: list stride below its length (0: one list for every query)");
     p.k = code_view(k);
     p.v = code_view(v);
+    p.aligned = rows_on_8(k) && rows_on_8(v);
+    const size_t size = dtype_size(a->dtype);
+    p.q_vec = rows_aligned(a->q, a->q_stride, size) && rows_aligned(a->q, a->q_head_stride, size) &&
+              a->head * size % 16 == 0;
     p.q = a->q;
     p.ids = a->ids;
     p.bias = a->bias;
@@ -860,21 +937,24 @@ int64_t backward_part(const AttendParams& p) {
     return p.splits > 1 ? round_up(p.splits * p.queries * p.heads * (2 * (int64_t)p.head + 2) * 4, 16) : 0;
 }
 
-// fn(LANES, RB): lanes that hold a head, and heads of a warp.
+// fn(LANES, RB, ALIGNED): lanes that hold a head, query heads of a unit.  Rows
+// off 8 bytes are read byte by byte, by the widest form alone.
 template <class F>
-void by_shape(int head, int rb, F&& fn) {
+void by_shape(const AttendParams& p, F&& fn) {
+    using std::integral_constant;
+    if (!p.aligned) return fn(integral_constant<int, 32>{}, integral_constant<int, 4>{}, std::false_type{});
     auto heads = [&](auto lanes) {
-        if (rb == 1) fn(lanes, std::integral_constant<int, 1>{});
-        else if (rb == 2) fn(lanes, std::integral_constant<int, 2>{});
-        else if (rb == 3) fn(lanes, std::integral_constant<int, 3>{});
-        else fn(lanes, std::integral_constant<int, 4>{});
+        if (p.rb == 1) fn(lanes, integral_constant<int, 1>{}, std::true_type{});
+        else if (p.rb == 2) fn(lanes, integral_constant<int, 2>{}, std::true_type{});
+        else if (p.rb == 3) fn(lanes, integral_constant<int, 3>{}, std::true_type{});
+        else fn(lanes, integral_constant<int, 4>{}, std::true_type{});
     };
-    if (head <= 8) heads(std::integral_constant<int, 1>{});
-    else if (head <= 16) heads(std::integral_constant<int, 2>{});
-    else if (head <= 32) heads(std::integral_constant<int, 4>{});
-    else if (head <= 64) heads(std::integral_constant<int, 8>{});
-    else if (head <= 128) heads(std::integral_constant<int, 16>{});
-    else heads(std::integral_constant<int, 32>{});
+    if (p.head <= 8) heads(integral_constant<int, 1>{});
+    else if (p.head <= 16) heads(integral_constant<int, 2>{});
+    else if (p.head <= 32) heads(integral_constant<int, 4>{});
+    else if (p.head <= 64) heads(integral_constant<int, 8>{});
+    else if (p.head <= 128) heads(integral_constant<int, 16>{});
+    else heads(integral_constant<int, 32>{});
 }
 dim3 attend_grid(const AttendParams& p) {
     return dim3((unsigned)(p.queries * p.unit_blocks), (unsigned)p.splits);
@@ -900,7 +980,7 @@ mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_
         AttendParams p = check_attend(a, keys, values);
         current_device();
         if (p.queries == 0) return;
-        MDH_REQUIRE(out && lse, MDH_ERR_INVALID_ARG, "attend: null output");
+        MDH_REQUIRE(out && lse && aligned16(out), MDH_ERR_INVALID_ARG, "attend: output null or not 16-byte aligned");
         const int64_t need = mdh_attend_workspace(a);
         MDH_REQUIRE(need == 0 || (ws && aligned16(ws) && ws_bytes >= need), MDH_ERR_INVALID_ARG,
                     "attend: workspace too small or not 16-byte aligned");
@@ -908,8 +988,9 @@ mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_
         p.out = out;
         p.lse = lse;
         p.part = need ? (float*)ws : nullptr;
-        by_shape(p.head, p.rb,
-                 [&](auto lanes, auto rb) { k_attend<lanes, rb><<<attend_grid(p), attend_threads(p), 0, st>>>(p); });
+        by_shape(p, [&](auto lanes, auto rb, auto aligned) {
+            k_attend<lanes, rb, aligned><<<attend_grid(p), attend_threads(p), 0, st>>>(p);
+        });
         check_launch();
         if (p.splits > 1) {
             k_attend_join<<<(unsigned)(p.queries * p.heads), 128, 0, st>>>(p);
@@ -932,7 +1013,8 @@ mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, c
         AttendParams p = check_attend(a, keys, values);
         current_device();
         if (p.queries == 0) return;
-        MDH_REQUIRE(dout && lse && dq, MDH_ERR_INVALID_ARG, "attend: null dout, lse or dq");
+        MDH_REQUIRE(dout && lse && dq && aligned16(dq), MDH_ERR_INVALID_ARG,
+                    "attend: null dout, lse or dq, or dq not 16-byte aligned");
         const int64_t need = mdh_attend_backward_workspace(a, dbias != nullptr);
         MDH_REQUIRE(need == 0 || (ws && aligned16(ws) && ws_bytes >= need), MDH_ERR_INVALID_ARG,
                     "attend: workspace too small or not 16-byte aligned");
@@ -948,9 +1030,10 @@ mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, c
         }
         p.out = dq;
         p.dout = dout;
+        p.dout_vec = aligned16(dout) && a->head * dtype_size(a->dtype) % 16 == 0;
         p.lse_in = lse;
-        by_shape(p.head, p.rb, [&](auto lanes, auto rb) {
-            k_attend_backward<lanes, rb><<<attend_grid(p), attend_threads(p), 0, st>>>(p);
+        by_shape(p, [&](auto lanes, auto rb, auto aligned) {
+            k_attend_backward<lanes, rb, aligned><<<attend_grid(p), attend_threads(p), 0, st>>>(p);
         });
         check_launch();
         if (p.splits > 1) {
