@@ -10,17 +10,20 @@
 //   A = sum_j p_j dP_j (1 - t_j^2) k_j,  B = sum_j p_j (1 - t_j^2) k_j:
 // one pass over the rows as well, since p_j follows from lse.
 //
-// A block takes one query, some of its units (a unit: a head of the rows and
-// up to kMaxShared query heads that share it) and a range of its list.  It
+// A unit is a head of the rows and up to kMaxShared query heads that share it.
+// LANES lanes hold a row's head, 8 elements each (an 8-byte load of codes); the
+// 32 / LANES lane groups of a warp take units side by side (a row's
+// neighbouring heads: nothing to join) and, where a call has too few units,
+// entries side by side.  A block takes one query and a range of its list: it
 // first lists the range's visible entries in shared memory (ids, documents and
-// biases are read once for all units), then its warps share units and slices
-// of that list.  In a warp LANES lanes hold one entry, 8 elements each (an
-// 8-byte load of codes), 32 / LANES entries go side by side and STEPS of them
-// are loaded at a time.  The STEPS x heads partial products of a lane are
-// summed by halving: each step sends half of the values to the partner lane,
-// so a lane ends with one finished score and the softmax arithmetic is done
-// once per score.  The maximum runs over the whole warp.  Slices are joined in
-// shared memory, ranges of other blocks by a second kernel, in a fixed order.
+// biases are read once for all units); then its warps share the units and, if
+// there are more warps, slices of that list.  STEPS entries of a lane group
+// are loaded while the previous ones are used.  The STEPS x heads partial
+// products of a lane are summed by halving: each step sends half of the values
+// to the partner lane, so a lane ends with one finished score and the softmax
+// arithmetic is done once per score.  Entries side by side and slices are
+// joined in the block, ranges of other blocks by a second kernel, in a fixed
+// order.
 //
 // Codes become floats without a conversion instruction: the byte c + 128 in
 // the mantissa of 2^23 is the float 8388736 + c, and one subtraction (two
@@ -64,9 +67,10 @@ struct AttendParams {
     float scale, cap, inv_cap;
     int r_blocks, rb;      // units of a row's head, query heads of each (the last may have fewer)
     int units;             // of a query
-    int block_units;       // of a block
+    int entries_log;       // log2 of the entries side by side in a warp
+    int block_warps;       // warps of a block that take different units
     int unit_blocks;       // blocks that share a query's units
-    int slices;            // warps of a block that share a unit
+    int slices;            // warps of a block that share their units
     int splits, split_len; // ranges of a list over blocks, entries of each
     bool aligned;          // rows of both caches start and step on 8 bytes
     void* out;
@@ -183,35 +187,56 @@ __device__ __forceinline__ void load_elements(const void* p, int64_t i, int dtyp
         }
     }
 }
-// Two elements at the even place i of an aligned output.
-__device__ __forceinline__ void store_pair(void* p, int64_t i, int dtype, float x, float y) {
-    if (dtype == MDH_F32) *reinterpret_cast<float2*>(static_cast<float*>(p) + i) = make_float2(x, y);
-    else if (dtype == MDH_BF16)
-        *reinterpret_cast<__nv_bfloat162*>(static_cast<bf16*>(p) + i) = __floats2bfloat162_rn(x, y);
-    else *reinterpret_cast<__half2*>(static_cast<f16*>(p) + i) = __floats2half2_rn(x, y);
+// 8 elements at place i (a multiple of 8) of an aligned output.
+__device__ __forceinline__ void store_elements(void* p, int64_t i, int dtype, const float (&v)[8]) {
+    if (dtype == MDH_F32) {
+        float4* f = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+        f[0] = make_float4(v[0], v[1], v[2], v[3]);
+        f[1] = make_float4(v[4], v[5], v[6], v[7]);
+        return;
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (dtype == MDH_BF16) {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&x);
+        } else {
+            const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// What a warp works on.
+// What a lane works on.
 struct Work {
     int64_t i;       // query
-    int h0, nr;      // first head, heads (0: an idle warp)
+    int h0, nr;      // first head, heads (0: an idle lane group)
     int e0;          // this lane's first element of a row
     int d0;          // ... of a head
     bool live;       // the lane holds elements (a head may end inside the lane group)
+    int entry;       // of the entries side by side
     int slice;
+    bool idle;       // the whole warp has no unit
 };
 template <int LANES>
 __device__ __forceinline__ Work work_of(const AttendParams& a) {
     Work w;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    w.i = blockIdx.x / a.unit_blocks;
-    const int unit = (int)(blockIdx.x - w.i * a.unit_blocks) * a.block_units + warp / a.slices;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES;
+    const int side_log = (LANES == 1 ? 5 : LANES == 2 ? 4 : LANES == 4 ? 3 : LANES == 8 ? 2 : LANES == 16 ? 1 : 0) -
+                         a.entries_log;  // units side by side
+    w.i = blockIdx.x / (unsigned)a.unit_blocks;
+    const int wu = (int)(blockIdx.x - w.i * a.unit_blocks) * a.block_warps + warp / a.slices;
+    const int unit = (wu << side_log) + (sub >> a.entries_log);
     w.slice = warp % a.slices;
-    const int g = min(unit, a.units - 1) / a.r_blocks, r0 = (unit - g * a.r_blocks) * a.rb;
+    w.entry = sub & ((1 << a.entries_log) - 1);
+    w.idle = wu << side_log >= a.units;
+    const int u = min(unit, a.units - 1), g = u / a.r_blocks, r0 = (u - g * a.r_blocks) * a.rb;
     w.h0 = g * a.shared + r0;
-    w.nr = unit < a.units ? max(0, min(a.rb, a.shared - r0)) : 0;
+    w.nr = unit < a.units ? min(a.rb, a.shared - r0) : 0;
     w.d0 = (lane % LANES) * 8;
-    w.live = w.d0 < a.head;
+    w.live = w.d0 < a.head && w.nr > 0;
     w.e0 = g * a.head + (w.live ? w.d0 : 0);
     return w;
 }
@@ -326,13 +351,11 @@ struct Steps {
     static constexpr int RP = RB == 3 ? 4 : RB;                    // heads, as a power of two
     static constexpr int WANT = RB > 2 ? 2 : 4;
     static constexpr int N = WANT > LANES ? LANES : WANT;          // steps loaded at a time
-    static constexpr int ENTRIES = 32 / LANES;                     // side by side
     using Sums = Halving<LANES, N * RP>;                           // value number step * RP + head
-    // Over the lanes that hold the same head: the bits of the step and of the side-by-side entry.
+    // Over the lanes that hold the same head: the bits of the step and of the entry side by side.
     template <class F>
-    static __device__ __forceinline__ void over_entries(F&& f) {
-#pragma unroll
-        for (int o = 16; o >= LANES; o >>= 1) f(o);
+    static __device__ __forceinline__ void over_entries(int entries_log, F&& f) {
+        for (int k = 0; k < entries_log; k++) f(LANES << k);
 #pragma unroll
         for (int o = LANES / 2; o >= LANES / N && o > 0; o >>= 1) f(o);
     }
@@ -354,34 +377,26 @@ __device__ __forceinline__ void load_heads(const void* p, int64_t at, int64_t st
     }
 }
 
-// Four pairs of elements a lane, summed over the warp's side-by-side entries
-// by halving: PAIRS finished pairs a lane, elements w.d0 + 2 first_pair() + 0
-// .. 2 PAIRS - 1.
+// Sums over the entries side by side.
 template <int LANES>
-struct Vector {
-    static constexpr int PAIRS = LANES == 32 ? 4 : LANES == 16 ? 2 : 1;
-    static __device__ __forceinline__ void sum(u64 (&v)[4]) {
-        const int lane = threadIdx.x & 31;
-        if (LANES <= 16) {
-            const bool up = lane & 16;
+__device__ __forceinline__ void join_vectors(u64 (&v)[4], int entries_log, float (&out)[8]) {
+    for (int k = 0; k < entries_log; k++)
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                v[j] = add2(up ? v[2 + j] : v[j], __shfl_xor_sync(0xffffffffu, up ? v[j] : v[2 + j], 16));
-        }
-        if (LANES <= 8) {
-            const bool up = lane & 8;
-            v[0] = add2(up ? v[1] : v[0], __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 8));
-        }
+        for (int j = 0; j < 4; j++) v[j] = add2(v[j], __shfl_xor_sync(0xffffffffu, v[j], LANES << k));
 #pragma unroll
-        for (int o = 4; o >= LANES; o >>= 1) v[0] = add2(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+    for (int j = 0; j < 4; j++) {
+        const float2 f = unpair(v[j]);
+        out[2 * j] = f.x, out[2 * j + 1] = f.y;
     }
-    static __device__ __forceinline__ int first_pair() {
-        const int lane = threadIdx.x & 31;
-        return LANES == 32 ? 0 : LANES == 16 ? lane >> 4 << 1 : lane >> 4 << 1 | (lane >> 3 & 1);
-    }
-    // One lane for each of the elements (lanes between LANES and 8 repeat others).
-    static __device__ __forceinline__ bool writer() { return LANES >= 8 || (threadIdx.x & 7) < LANES; }
-};
+}
+__device__ __forceinline__ void put8(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void get8(const float* p, float (&v)[8]) {
+    const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+}
 
 // The scaled, capped and biased score of a finished sum; t = tanh of the capped one.
 __device__ __forceinline__ float score_of(const AttendParams& a, float x, float bias, float& t) {
@@ -402,17 +417,21 @@ __device__ __forceinline__ float join(float m, float mo, float& mine, float& oth
     return top;
 }
 
-// The finished pair of elements d, d + 1 of (query, head) `at`.
-__device__ __forceinline__ void finish_forward(const AttendParams& a, int64_t at, int d, float2 v, float m, float l) {
+// The 8 elements from d of (query, head) `at`.
+__device__ __forceinline__ void finish_forward(const AttendParams& a, int64_t at, int d, float (&v)[8], float m, float l) {
     const float inv = l != 0.0f ? 1.0f / l : 0.0f, base = l != 0.0f ? a.v.base : 0.0f;
-    store_pair(a.out, at * a.head + d, a.dtype, fmaf(v.x, inv, base), fmaf(v.y, inv, base));
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = fmaf(v[j], inv, base);
+    store_elements(a.out, at * a.head + d, a.dtype, v);
     if (d == 0) a.lse[at] = l != 0.0f ? m + logf(l) : -INFINITY;
 }
-__device__ __forceinline__ void finish_backward(const AttendParams& a, int64_t at, int d, float2 x, float2 y, float sum_d,
-                                                float sum_p) {
+__device__ __forceinline__ void finish_backward(const AttendParams& a, int64_t at, int d, float (&x)[8],
+                                                const float (&y)[8], float sum_d, float sum_p) {
     const float inv = sum_p != 0.0f ? 1.0f / sum_p : 0.0f, f = a.scale * inv;
     sum_d *= inv;
-    store_pair(a.out, at * a.head + d, a.dtype, f * (x.x - sum_d * y.x), f * (x.y - sum_d * y.y));
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = f * (x[j] - sum_d * y[j]);
+    store_elements(a.out, at * a.head + d, a.dtype, x);
     if (a.sum_d && d == 0) a.sum_d[at] = make_float2(sum_d, inv);
 }
 
@@ -435,11 +454,12 @@ __device__ __forceinline__ Places places_of(const AttendParams& a, const Work& w
             a.v.scales ? a.v.scales + w.e0 / a.v.group : nullptr, a.k.stride, a.v.stride, a.k.n_groups, a.v.n_groups,
             a.k.scale, a.v.scale};
 }
-template <bool ALIGNED, int STEPS, int ENTRIES>
-__device__ __forceinline__ void load_rows(Rows<STEPS>& r, const Places& p, const int* slots, int first, int hi, bool live) {
+template <bool ALIGNED, int STEPS>
+__device__ __forceinline__ void load_rows(Rows<STEPS>& r, const Places& p, const int* slots, int first, int entries_log, int hi,
+                                          bool live) {
 #pragma unroll
     for (int u = 0; u < STEPS; u++) {
-        const int e = first + u * ENTRIES;
+        const int e = first + (u << entries_log);
         r.k[u] = r.v[u] = make_uint2(0, 0);
         r.ks[u] = r.vs[u] = 0.0f;
         if (e < hi && live) {
@@ -456,12 +476,12 @@ template <int LANES, int RB, bool ALIGNED>
 __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(const __grid_constant__ AttendParams a) {
     using St = Steps<LANES, RB>;
     using Sums = typename St::Sums;
-    constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP, ENTRIES = St::ENTRIES;
+    constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP;
     __shared__ union alignas(16) {
         Entries e;
-        float joined[kMaxWarps][LANES * 8 + 2];  // vector, m, l
+        float joined[kMaxWarps][32 * 8 + 64];    // of each lane: vector; m, l
     } sm;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = STEPS << a.entries_log;
     const Work w = work_of<LANES>(a);
     u64 q[RB][4], acc[RB][4];
     float kb[RB];
@@ -481,13 +501,13 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(cons
     const int j1 = (int)min((int64_t)j0 + a.split_len, (int64_t)a.found);
     for (int from = j0; from < j1; from += (blockDim.x >> 5) * kRound) {
         int lo, hi;
-        slice_of(list_entries(a, sm.e, w.i, doc, from, j1), w.slice, a.slices, STEPS * ENTRIES, lo, hi);
-        if (w.nr == 0) hi = lo;
+        slice_of(list_entries(a, sm.e, w.i, doc, from, j1), w.slice, a.slices, step, lo, hi);
+        if (w.idle) hi = lo;
         Rows<STEPS> next;
-        load_rows<ALIGNED, STEPS, ENTRIES>(next, places, sm.e.slot, lo + sub, hi, w.live);
-        for (int t = lo; t < hi; t += STEPS * ENTRIES) {
+        load_rows<ALIGNED, STEPS>(next, places, sm.e.slot, lo + w.entry, a.entries_log, hi, w.live);
+        for (int t = lo; t < hi; t += step) {
             const Rows<STEPS> now = next;  // the next entries are loaded while these are used
-            load_rows<ALIGNED, STEPS, ENTRIES>(next, places, sm.e.slot, t + STEPS * ENTRIES + sub, hi, w.live);
+            load_rows<ALIGNED, STEPS>(next, places, sm.e.slot, t + step + w.entry, a.entries_log, hi, w.live);
             float s[STEPS * RP];
 #pragma unroll
             for (int u = 0; u < STEPS; u++) {
@@ -501,11 +521,11 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(cons
             bool grown = false;
 #pragma unroll
             for (int x = 0; x < KEEP; x++) {
-                const int e = t + Sums::value_of(x) / RP * ENTRIES + sub;
+                const int e = t + (Sums::value_of(x) / RP << a.entries_log) + w.entry;
                 float th;
                 p[x] = e < hi ? score_of(a, s[x], sm.e.bias[e], th) : -INFINITY;
                 float top = p[x];
-                St::over_entries([&](int o) { top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o)); });
+                St::over_entries(a.entries_log, [&](int o) { top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o)); });
                 top = fmaxf(top, m[x]);
                 grown |= top > m[x];
                 const float ref = top == -INFINITY ? 0.0f : top;
@@ -539,49 +559,37 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(cons
     }
 #pragma unroll
     for (int x = 0; x < KEEP; x++)
-        St::over_entries([&](int o) { l[x] += __shfl_xor_sync(0xffffffffu, l[x], o); });
-    using Vec = Vector<LANES>;
-    const int d0 = w.d0 + 2 * Vec::first_pair();
+        St::over_entries(a.entries_log, [&](int o) { l[x] += __shfl_xor_sync(0xffffffffu, l[x], o); });
 #pragma unroll
     for (int r = 0; r < RB; r++) {
-        float2 v[Vec::PAIRS];
-        float mm = Sums::get(m, r), ll = Sums::get(l, r);
-        Vec::sum(acc[r]);
-#pragma unroll
-        for (int j = 0; j < Vec::PAIRS; j++) v[j] = unpair(acc[r][j]);
+        float v[8], mm = Sums::get(m, r), ll = Sums::get(l, r);
+        join_vectors<LANES>(acc[r], a.entries_log, v);
         if (a.slices > 1) {
             __syncthreads();  // the list, or the previous head's vectors, have been read
-            float* mine = sm.joined[warp];
-            if (Vec::writer()) {
-#pragma unroll
-                for (int j = 0; j < Vec::PAIRS; j++) *reinterpret_cast<float2*>(mine + d0 + 2 * j) = v[j];
-            }
-            if (lane == 0) mine[LANES * 8] = mm, mine[LANES * 8 + 1] = ll;
+            put8(sm.joined[warp] + lane * 8, v);
+            reinterpret_cast<float2*>(sm.joined[warp] + 256)[lane] = make_float2(mm, ll);
             __syncthreads();
             if (w.slice == 0) {
                 for (int k = 1; k < a.slices; k++) {
                     const float* src = sm.joined[warp + k];
-                    float f, g;
-                    mm = join(mm, src[LANES * 8], f, g);
-                    ll = ll * f + src[LANES * 8 + 1] * g;
+                    const float2 ml = reinterpret_cast<const float2*>(src + 256)[lane];
+                    float o[8], f, g;
+                    get8(src + lane * 8, o);
+                    mm = join(mm, ml.x, f, g);
+                    ll = ll * f + ml.y * g;
 #pragma unroll
-                    for (int j = 0; j < Vec::PAIRS; j++) {
-                        const float2 o = *reinterpret_cast<const float2*>(src + d0 + 2 * j);
-                        v[j].x = v[j].x * f + o.x * g;
-                        v[j].y = v[j].y * f + o.y * g;
-                    }
+                    for (int j = 0; j < 8; j++) v[j] = v[j] * f + o[j] * g;
                 }
             }
         }
-        if (r >= w.nr || w.slice != 0 || !w.live || !Vec::writer()) continue;
+        if (r >= w.nr || w.slice != 0 || !w.live || w.entry != 0) continue;
         const int64_t at = w.i * a.heads + w.h0 + r, n = a.queries * a.heads, row = (int64_t)blockIdx.y * n + at;
-#pragma unroll
-        for (int j = 0; j < Vec::PAIRS; j++) {
-            const int d = d0 + 2 * j;
-            if (a.part) *reinterpret_cast<float2*>(a.part + row * a.head + d) = v[j];
-            else finish_forward(a, at, d, v[j], mm, ll);
+        if (a.part) {
+            put8(a.part + row * a.head + w.d0, v);
+            if (w.d0 == 0) reinterpret_cast<float2*>(a.part + a.splits * n * a.head)[row] = make_float2(mm, ll);
+        } else {
+            finish_forward(a, at, w.d0, v, mm, ll);
         }
-        if (a.part && lane == 0) reinterpret_cast<float2*>(a.part + a.splits * n * a.head)[row] = make_float2(mm, ll);
     }
 }
 
@@ -620,9 +628,7 @@ __global__ void __launch_bounds__(128) k_attend_join(const __grid_constant__ Att
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] += joined[k][d0 + j];
     }
-    if (d0 < a.head)
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) finish_forward(a, at, d0 + j, make_float2(v[j], v[j + 1]), m, l);
+    if (d0 < a.head) finish_forward(a, at, d0, v, m, l);
 }
 
 // A, B, D and the weights' own sum P of the lists' slices; dq = scale (A - (D / P) B) / P.
@@ -632,12 +638,12 @@ template <int LANES, int RB, bool ALIGNED>
 __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_backward(const __grid_constant__ AttendParams a) {
     using St = Steps<LANES, RB>;
     using Sums = typename St::Sums;
-    constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP, ENTRIES = St::ENTRIES;
+    constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP;
     __shared__ union alignas(16) {
         Entries e;
-        float joined[kMaxWarps][LANES * 16 + 2];  // A, B, D, P
+        float joined[kMaxWarps][32 * 16 + 64];   // of each lane: A, B; D, P
     } sm;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = STEPS << a.entries_log;
     const Work w = work_of<LANES>(a);
     u64 q[RB][4], g[RB][4], va[RB][4], vb[RB][4];
     float kb[RB], gb[RB];
@@ -664,13 +670,13 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_back
     const int j1 = (int)min((int64_t)j0 + a.split_len, (int64_t)a.found);
     for (int from = j0; from < j1; from += (blockDim.x >> 5) * kRound) {
         int lo, hi;
-        slice_of(list_entries(a, sm.e, w.i, doc, from, j1), w.slice, a.slices, STEPS * ENTRIES, lo, hi);
-        if (w.nr == 0) hi = lo;
+        slice_of(list_entries(a, sm.e, w.i, doc, from, j1), w.slice, a.slices, step, lo, hi);
+        if (w.idle) hi = lo;
         Rows<STEPS> next;
-        load_rows<ALIGNED, STEPS, ENTRIES>(next, places, sm.e.slot, lo + sub, hi, w.live);
-        for (int t = lo; t < hi; t += STEPS * ENTRIES) {
+        load_rows<ALIGNED, STEPS>(next, places, sm.e.slot, lo + w.entry, a.entries_log, hi, w.live);
+        for (int t = lo; t < hi; t += step) {
             const Rows<STEPS> now = next;  // the next entries are loaded while these are used
-            load_rows<ALIGNED, STEPS, ENTRIES>(next, places, sm.e.slot, t + STEPS * ENTRIES + sub, hi, w.live);
+            load_rows<ALIGNED, STEPS>(next, places, sm.e.slot, t + step + w.entry, a.entries_log, hi, w.live);
             float s[STEPS * RP], dp[STEPS * RP];
 #pragma unroll
             for (int u = 0; u < STEPS; u++) {
@@ -687,7 +693,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_back
             float fa[KEEP], fb[KEEP];
 #pragma unroll
             for (int x = 0; x < KEEP; x++) {
-                const int v = Sums::value_of(x), r = v % RP, e = t + v / RP * ENTRIES + sub;
+                const int v = Sums::value_of(x), r = v % RP, e = t + (v / RP << a.entries_log) + w.entry;
                 fa[x] = fb[x] = 0.0f;
                 if (e < hi && r < w.nr) {
                     float th;
@@ -723,60 +729,44 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_back
     }
 #pragma unroll
     for (int x = 0; x < KEEP; x++)
-        St::over_entries([&](int o) {
+        St::over_entries(a.entries_log, [&](int o) {
             dsum[x] += __shfl_xor_sync(0xffffffffu, dsum[x], o);
             psum[x] += __shfl_xor_sync(0xffffffffu, psum[x], o);
         });
-    using Vec = Vector<LANES>;
-    const int d0 = w.d0 + 2 * Vec::first_pair();
 #pragma unroll
     for (int r = 0; r < RB; r++) {
-        float2 x[Vec::PAIRS], y[Vec::PAIRS];
-        float sd = Sums::get(dsum, r), sp = Sums::get(psum, r);
-        Vec::sum(va[r]);
-        Vec::sum(vb[r]);
-#pragma unroll
-        for (int j = 0; j < Vec::PAIRS; j++) x[j] = unpair(va[r][j]), y[j] = unpair(vb[r][j]);
+        float x[8], y[8], sd = Sums::get(dsum, r), sp = Sums::get(psum, r);
+        join_vectors<LANES>(va[r], a.entries_log, x);
+        join_vectors<LANES>(vb[r], a.entries_log, y);
         if (a.slices > 1) {
             __syncthreads();  // the list, or the previous head's vectors, have been read
-            float* mine = sm.joined[warp];
-            if (Vec::writer()) {
-#pragma unroll
-                for (int j = 0; j < Vec::PAIRS; j++) {
-                    *reinterpret_cast<float2*>(mine + d0 + 2 * j) = x[j];
-                    *reinterpret_cast<float2*>(mine + LANES * 8 + d0 + 2 * j) = y[j];
-                }
-            }
-            if (lane == 0) mine[LANES * 16] = sd, mine[LANES * 16 + 1] = sp;
+            put8(sm.joined[warp] + lane * 8, x);
+            put8(sm.joined[warp] + 256 + lane * 8, y);
+            reinterpret_cast<float2*>(sm.joined[warp] + 512)[lane] = make_float2(sd, sp);
             __syncthreads();
             if (w.slice == 0) {
                 for (int k = 1; k < a.slices; k++) {
                     const float* src = sm.joined[warp + k];
-                    sd += src[LANES * 16];
-                    sp += src[LANES * 16 + 1];
+                    const float2 dp = reinterpret_cast<const float2*>(src + 512)[lane];
+                    float o[8], h[8];
+                    get8(src + lane * 8, o);
+                    get8(src + 256 + lane * 8, h);
+                    sd += dp.x;
+                    sp += dp.y;
 #pragma unroll
-                    for (int j = 0; j < Vec::PAIRS; j++) {
-                        const float2 o = *reinterpret_cast<const float2*>(src + d0 + 2 * j);
-                        const float2 h = *reinterpret_cast<const float2*>(src + LANES * 8 + d0 + 2 * j);
-                        x[j].x += o.x, x[j].y += o.y, y[j].x += h.x, y[j].y += h.y;
-                    }
+                    for (int j = 0; j < 8; j++) x[j] += o[j], y[j] += h[j];
                 }
             }
         }
-        if (r >= w.nr || w.slice != 0 || !w.live || !Vec::writer()) continue;
+        if (r >= w.nr || w.slice != 0 || !w.live || w.entry != 0) continue;
         const int64_t at = w.i * a.heads + w.h0 + r, n = a.queries * a.heads, row = (int64_t)blockIdx.y * n + at;
-#pragma unroll
-        for (int j = 0; j < Vec::PAIRS; j++) {
-            const int d = d0 + 2 * j;
-            if (a.part) {
-                *reinterpret_cast<float2*>(a.part + row * 2 * a.head + d) = x[j];
-                *reinterpret_cast<float2*>(a.part + (row * 2 + 1) * a.head + d) = y[j];
-            } else {
-                finish_backward(a, at, d, x[j], y[j], sd, sp);
-            }
+        if (a.part) {
+            put8(a.part + row * 2 * a.head + w.d0, x);
+            put8(a.part + (row * 2 + 1) * a.head + w.d0, y);
+            if (w.d0 == 0) reinterpret_cast<float2*>(a.part + a.splits * n * 2 * a.head)[row] = make_float2(sd, sp);
+        } else {
+            finish_backward(a, at, w.d0, x, y, sd, sp);
         }
-        if (a.part && lane == 0)
-            reinterpret_cast<float2*>(a.part + a.splits * n * 2 * a.head)[row] = make_float2(sd, sp);
     }
 }
 
@@ -809,10 +799,7 @@ __global__ void __launch_bounds__(128) k_attend_backward_join(const __grid_const
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] += joined[k][d0 + j], y[j] += joined[k][kMaxHead + d0 + j];
     }
-    if (d0 < a.head)
-#pragma unroll
-        for (int j = 0; j < 8; j += 2)
-            finish_backward(a, at, d0 + j, make_float2(x[j], x[j + 1]), make_float2(y[j], y[j + 1]), d, p);
+    if (d0 < a.head) finish_backward(a, at, d0, x, y, d, p);
 }
 
 // dbias[i][j] = sum over heads of (p dP - p D / P) / P, in head order; 0 at hidden entries.
@@ -846,21 +833,33 @@ CodeView code_view(const RowsView& r) {
     return c;
 }
 
-// How a call is laid out over blocks.  A block takes up to kMaxWarps units of
-// a query; where the calls' units do not fill the GPU, several warps of a
-// block share a unit's list, and then blocks take ranges of it; no slice is
-// below kMinSlice entries.
+// Lanes that hold a head; rows off 8 bytes take the widest form alone.
+int lanes_of(const AttendParams& p) {
+    int lanes = 1;
+    while (lanes * 8 < p.head) lanes *= 2;
+    return p.aligned ? lanes : 32;
+}
+
+// How a call is laid out over warps and blocks.  Units side by side in a warp
+// need no join, so lane groups take entries of one unit only where the GPU's
+// warps would not be filled otherwise; then several warps of a block share
+// units' lists, and then blocks take ranges of a list; no slice is below
+// kMinSlice entries.
 void lay_out(AttendParams& p) {
-    constexpr int64_t kFill = 148 * 16;  // warps
+    constexpr int64_t kFill = 148 * 12;  // warps
     p.r_blocks = (int)ceil_div(p.shared, kMaxShared);
     p.rb = (int)ceil_div(p.shared, p.r_blocks);
     p.units = p.heads / p.shared * p.r_blocks;
-    p.unit_blocks = (int)ceil_div(p.units, kMaxWarps);
-    p.block_units = (int)ceil_div(p.units, p.unit_blocks);
-    const int64_t units = std::max<int64_t>(1, p.queries * p.unit_blocks * p.block_units);
+    int side = 32 / lanes_of(p);
+    p.entries_log = 0;
+    while (side > 1 && (side / 2 >= p.units || p.queries * ceil_div(p.units, side) < kFill)) side /= 2, p.entries_log++;
+    const int64_t unit_warps = ceil_div(p.units, side);
+    p.unit_blocks = (int)ceil_div(unit_warps, kMaxWarps);
+    p.block_warps = (int)ceil_div(unit_warps, p.unit_blocks);
+    const int64_t warps = std::max<int64_t>(1, p.queries * p.unit_blocks * p.block_warps);
     p.slices = (int)std::max<int64_t>(
-        1, std::min({(int64_t)kMaxWarps / p.block_units, ceil_div(p.found, kMinSlice), ceil_div(kFill, units)}));
-    const int64_t splits = std::min(ceil_div(p.found, p.slices * kMinSlice), kFill / (units * p.slices));
+        1, std::min({(int64_t)kMaxWarps / p.block_warps, ceil_div(p.found, kMinSlice), ceil_div(kFill, warps)}));
+    const int64_t splits = std::min(ceil_div(p.found, p.slices * kMinSlice), kFill / (warps * p.slices));
     p.split_len = (int)std::max<int64_t>(1, ceil_div(p.found, std::max<int64_t>(1, splits)));
     p.splits = (int)std::max<int64_t>(1, ceil_div(p.found, p.split_len));
 }
@@ -919,19 +918,23 @@ AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const 
 }
 
 // The layout of a call from its sizes alone, for the workspace.
-AttendParams layout_of(const mdh_attend_args* a) {
+AttendParams layout_of(const mdh_attend_args* a, bool aligned) {
     AttendParams p{};
     p.queries = a->queries;
     p.found = a->found;
     p.heads = a->heads;
     p.shared = a->shared;
     p.head = a->head;
+    p.aligned = aligned;
     lay_out(p);
     return p;
 }
 bool has_sizes(const mdh_attend_args* a) {
     return a && a->queries > 0 && a->found >= 0 && a->heads > 0 && a->shared > 0 && a->heads % a->shared == 0 &&
            a->head > 0;
+}
+int64_t forward_part(const AttendParams& p) {
+    return p.splits > 1 ? p.splits * p.queries * p.heads * ((int64_t)p.head + 2) * 4 : 0;
 }
 int64_t backward_part(const AttendParams& p) {
     return p.splits > 1 ? round_up(p.splits * p.queries * p.heads * (2 * (int64_t)p.head + 2) * 4, 16) : 0;
@@ -949,17 +952,19 @@ void by_shape(const AttendParams& p, F&& fn) {
         else if (p.rb == 3) fn(lanes, integral_constant<int, 3>{}, std::true_type{});
         else fn(lanes, integral_constant<int, 4>{}, std::true_type{});
     };
-    if (p.head <= 8) heads(integral_constant<int, 1>{});
-    else if (p.head <= 16) heads(integral_constant<int, 2>{});
-    else if (p.head <= 32) heads(integral_constant<int, 4>{});
-    else if (p.head <= 64) heads(integral_constant<int, 8>{});
-    else if (p.head <= 128) heads(integral_constant<int, 16>{});
-    else heads(integral_constant<int, 32>{});
+    switch (lanes_of(p)) {
+        case 1: heads(integral_constant<int, 1>{}); break;
+        case 2: heads(integral_constant<int, 2>{}); break;
+        case 4: heads(integral_constant<int, 4>{}); break;
+        case 8: heads(integral_constant<int, 8>{}); break;
+        case 16: heads(integral_constant<int, 16>{}); break;
+        default: heads(integral_constant<int, 32>{}); break;
+    }
 }
 dim3 attend_grid(const AttendParams& p) {
     return dim3((unsigned)(p.queries * p.unit_blocks), (unsigned)p.splits);
 }
-int attend_threads(const AttendParams& p) { return 32 * p.block_units * p.slices; }
+int attend_threads(const AttendParams& p) { return 32 * p.block_warps * p.slices; }
 
 }  // namespace
 }  // namespace mdh
@@ -970,8 +975,7 @@ extern "C" {
 
 int64_t mdh_attend_workspace(const mdh_attend_args* a) {
     if (!has_sizes(a)) return 0;
-    const AttendParams p = layout_of(a);
-    return p.splits > 1 ? p.splits * p.queries * p.heads * ((int64_t)p.head + 2) * 4 : 0;
+    return std::max(forward_part(layout_of(a, true)), forward_part(layout_of(a, false)));
 }
 
 mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values, void* out, float* lse,
@@ -987,7 +991,7 @@ mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_
         const cudaStream_t st = (cudaStream_t)stream;
         p.out = out;
         p.lse = lse;
-        p.part = need ? (float*)ws : nullptr;
+        p.part = p.splits > 1 ? (float*)ws : nullptr;
         by_shape(p, [&](auto lanes, auto rb, auto aligned) {
             k_attend<lanes, rb, aligned><<<attend_grid(p), attend_threads(p), 0, st>>>(p);
         });
@@ -1001,7 +1005,7 @@ mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_
 
 int64_t mdh_attend_backward_workspace(const mdh_attend_args* a, int32_t want_dbias) {
     if (!has_sizes(a)) return 0;
-    int64_t need = backward_part(layout_of(a));
+    int64_t need = std::max(backward_part(layout_of(a, true)), backward_part(layout_of(a, false)));
     if (want_dbias) need += a->queries * a->heads * 8 + a->queries * a->heads * (int64_t)a->found * 8;
     return need;
 }
