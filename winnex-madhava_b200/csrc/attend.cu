@@ -17,8 +17,10 @@
 // entries side by side.  A block takes one query and a range of its list: it
 // first lists the range's visible entries in shared memory (ids, documents and
 // biases are read once for all units); then its warps share the units and, if
-// there are more warps, slices of that list.  STEPS entries of a lane group
-// are loaded while the previous ones are used.  The STEPS x heads partial
+// there are more warps, slices of that list.  Each lane copies the codes and
+// scales it will use into its own shared memory (cp.async), STEPS entries a
+// stage and some stages ahead: rows lie anywhere in a large cache, and what
+// bounds short lists is the latency of reaching them.  The STEPS x heads partial
 // products of a lane are summed by halving: each step sends half of the values
 // to the partner lane, so a lane ends with one finished score and the softmax
 // arithmetic is done once per score.  Entries side by side and slices are
@@ -31,6 +33,7 @@
 // 8-term sums; the affine code's offset enters as a constant times the sum of
 // the query's elements, or of the weights.
 #include <algorithm>
+#include <atomic>
 
 #include "op_rows.cuh"
 
@@ -84,32 +87,7 @@ struct AttendParams {
     float2* sum_d;         // [queries][heads] D / P and 1 / P, or null
 };
 
-using u64 = unsigned long long;
-__device__ __forceinline__ u64 pair(float a, float b) {
-    u64 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpair(u64 v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
-    u64 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ u64 add2(u64 a, u64 b) {
-    u64 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
-    u64 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
+using u64 = f32x2;
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -123,18 +101,6 @@ __device__ __forceinline__ float tanh_fast(float x) {
     return 1.0f - __fdividef(2.0f, exp2_fast(fminf(x * (2.0f * kLog2e), 126.0f)) + 1.0f);
 }
 
-// 8 codes of a row; ALIGNED: rows start and step on 8 bytes.
-template <bool ALIGNED>
-__device__ __forceinline__ uint2 load_codes(const uint8_t* p) {
-    if (ALIGNED) return __ldg(reinterpret_cast<const uint2*>(p));
-    uint2 r = make_uint2(0, 0);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        r.x |= (uint32_t)p[j] << (8 * j);
-        r.y |= (uint32_t)p[4 + j] << (8 * j);
-    }
-    return r;
-}
 // The codes c as four pairs of floats.
 __device__ __forceinline__ void code_pairs(uint2 raw, uint32_t flip, u64 (&c)[4]) {
     const uint32_t w[2] = {raw.x ^ flip, raw.y ^ flip};
@@ -250,15 +216,21 @@ __device__ __forceinline__ int entry_slot(const AttendParams& a, int64_t i, int 
     return id;
 }
 
-// The visible entries of a range, in order.
+// The visible entries of a range, in order (shared memory, kRound a warp).
 struct Entries {
-    int slot[kMaxWarps * kRound];
-    float bias[kMaxWarps * kRound];
-    int place[kMaxWarps * kRound];  // in the query's list
-    int count[kMaxWarps];
+    int* slot;
+    float* bias;
+    int* place;   // in the query's list
+    int* count;   // of each warp
 };
+constexpr int kEntriesBytes = kRound * 12 + 16;  // a warp
+__device__ __forceinline__ Entries entries_at(uint8_t* p, int warps) {
+    int* q = reinterpret_cast<int*>(p);
+    const int n = warps * kRound;
+    return {q, reinterpret_cast<float*>(q + n), q + 2 * n, q + 3 * n};
+}
 // Lists the visible entries of [j0, j1), at most kRound a warp.
-__device__ __forceinline__ int list_entries(const AttendParams& a, Entries& e, int64_t i, int32_t doc, int j0, int j1) {
+__device__ __forceinline__ int list_entries(const AttendParams& a, const Entries& e, int64_t i, int32_t doc, int j0, int j1) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int warps = min((int)blockDim.x >> 5, (j1 - j0 + kRound - 1) / kRound);  // that look at entries
     int slot[kRound / 32], n = 0;
@@ -350,8 +322,11 @@ template <int LANES, int RB>
 struct Steps {
     static constexpr int RP = RB == 3 ? 4 : RB;                    // heads, as a power of two
     static constexpr int WANT = RB > 2 ? 2 : 4;
-    static constexpr int N = WANT > LANES ? LANES : WANT;          // steps loaded at a time
+    static constexpr int N = WANT > LANES ? LANES : WANT;          // entries of a stage
+    static constexpr int STAGES = N == 4 ? 2 : 4;
+    static constexpr int RING = STAGES * N * 768;                  // bytes a warp: codes and scales of its lanes
     using Sums = Halving<LANES, N * RP>;                           // value number step * RP + head
+    static_assert(RING >= 576 * 4, "the joined vectors lie in the rings");
     // Over the lanes that hold the same head: the bits of the step and of the entry side by side.
     template <class F>
     static __device__ __forceinline__ void over_entries(int entries_log, F&& f) {
@@ -435,12 +410,6 @@ __device__ __forceinline__ void finish_backward(const AttendParams& a, int64_t a
     if (a.sum_d && d == 0) a.sum_d[at] = make_float2(sum_d, inv);
 }
 
-// The codes and scales of STEPS entries side by side, in flight.
-template <int STEPS>
-struct Rows {
-    uint2 k[STEPS], v[STEPS];
-    float ks[STEPS], vs[STEPS];
-};
 // Where a lane reads rows.
 struct Places {
     const uint8_t *k, *v;
@@ -454,35 +423,67 @@ __device__ __forceinline__ Places places_of(const AttendParams& a, const Work& w
             a.v.scales ? a.v.scales + w.e0 / a.v.group : nullptr, a.k.stride, a.v.stride, a.k.n_groups, a.v.n_groups,
             a.k.scale, a.v.scale};
 }
+// A lane's place in a stage: codes of key and value (8 bytes), their scales.
+struct Slot {
+    uint8_t* at;
+    __device__ __forceinline__ uint2* codes(int u, int value) const {
+        return reinterpret_cast<uint2*>(at + u * 768 + value * 256) + (threadIdx.x & 31);
+    }
+    __device__ __forceinline__ float* scale(int u, int value) const {
+        return reinterpret_cast<float*>(at + u * 768 + 512 + value * 128) + (threadIdx.x & 31);
+    }
+};
+// What a lane uses of one stage's keys or values.
+template <int STEPS>
+struct Taken {
+    uint2 codes[STEPS];
+    float scale[STEPS];
+    __device__ __forceinline__ void take(const Slot& s, int value, bool scales, float constant) {
+#pragma unroll
+        for (int u = 0; u < STEPS; u++) {
+            codes[u] = *s.codes(u, value);
+            scale[u] = scales ? *s.scale(u, value) : constant;
+        }
+    }
+};
+template <bool ALIGNED>
+__device__ __forceinline__ void fetch_codes(uint2* dst, const uint8_t* src, bool some) {
+    if (ALIGNED) return copy_async<8>(dst, src, some);
+    uint2 r = make_uint2(0, 0);
+    if (some) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) r.x |= (uint32_t)src[j] << (8 * j), r.y |= (uint32_t)src[4 + j] << (8 * j);
+    }
+    *dst = r;
+}
+// Starts the copies of one stage: entries first, first + (1 << entries_log), ...
 template <bool ALIGNED, int STEPS>
-__device__ __forceinline__ void load_rows(Rows<STEPS>& r, const Places& p, const int* slots, int first, int entries_log, int hi,
-                                          bool live) {
+__device__ __forceinline__ void fetch(Slot to, const Places& p, const int* slots, int first, int entries_log, int hi,
+                                      bool live) {
 #pragma unroll
     for (int u = 0; u < STEPS; u++) {
         const int e = first + (u << entries_log);
-        r.k[u] = r.v[u] = make_uint2(0, 0);
-        r.ks[u] = r.vs[u] = 0.0f;
-        if (e < hi && live) {
-            const int64_t slot = slots[e];
-            r.k[u] = load_codes<ALIGNED>(p.k + slot * p.k_stride);
-            r.v[u] = load_codes<ALIGNED>(p.v + slot * p.v_stride);
-            r.ks[u] = p.ks ? __ldg(p.ks + slot * p.kn) : p.k_scale;
-            r.vs[u] = p.vs ? __ldg(p.vs + slot * p.vn) : p.v_scale;
-        }
+        const bool some = e < hi && live;
+        const int64_t slot = some ? slots[e] : 0;
+        fetch_codes<ALIGNED>(to.codes(u, 0), p.k + slot * p.k_stride, some);
+        fetch_codes<ALIGNED>(to.codes(u, 1), p.v + slot * p.v_stride, some);
+        if (p.ks) copy_async<4>(to.scale(u, 0), p.ks + slot * p.kn, some);
+        if (p.vs) copy_async<4>(to.scale(u, 1), p.vs + slot * p.vn, some);
     }
+    copy_commit();
 }
-
 template <int LANES, int RB, bool ALIGNED>
 __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(const __grid_constant__ AttendParams a) {
     using St = Steps<LANES, RB>;
     using Sums = typename St::Sums;
     constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP;
-    __shared__ union alignas(16) {
-        Entries e;
-        float joined[kMaxWarps][32 * 8 + 64];    // of each lane: vector; m, l
-    } sm;
+    constexpr int STAGES = St::STAGES;
+    extern __shared__ uint8_t sm[];  // the warps' rings, later the vectors to join; then the entries
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = STEPS << a.entries_log;
     const Work w = work_of<LANES>(a);
+    const int warps = blockDim.x >> 5;
+    const Entries list = entries_at(sm + warps * St::RING, warps);
+    const Slot ring{sm + warp * St::RING};
     u64 q[RB][4], acc[RB][4];
     float kb[RB];
     load_heads<RB>(a.q, w.i * a.q_stride, a.q_head_stride, a.dtype, w, a.q_vec, a.scale, q, kb);
@@ -501,20 +502,31 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(cons
     const int j1 = (int)min((int64_t)j0 + a.split_len, (int64_t)a.found);
     for (int from = j0; from < j1; from += (blockDim.x >> 5) * kRound) {
         int lo, hi;
-        slice_of(list_entries(a, sm.e, w.i, doc, from, j1), w.slice, a.slices, step, lo, hi);
+        slice_of(list_entries(a, list, w.i, doc, from, j1), w.slice, a.slices, step, lo, hi);
         if (w.idle) hi = lo;
-        Rows<STEPS> next;
-        load_rows<ALIGNED, STEPS>(next, places, sm.e.slot, lo + w.entry, a.entries_log, hi, w.live);
+        copy_wait<0>();  // the previous range's last (empty) stages
+#pragma unroll
+        for (int k = 0; k < STAGES - 1; k++)
+            fetch<ALIGNED, STEPS>({ring.at + k * STEPS * 768}, places, list.slot, lo + k * step + w.entry, a.entries_log,
+                                  hi, w.live);
+        int stage = 0, ahead = STAGES - 1;
         for (int t = lo; t < hi; t += step) {
-            const Rows<STEPS> now = next;  // the next entries are loaded while these are used
-            load_rows<ALIGNED, STEPS>(next, places, sm.e.slot, t + step + w.entry, a.entries_log, hi, w.live);
+            copy_wait<STAGES - 2>();
+            const Slot now{ring.at + stage * STEPS * 768};
+            fetch<ALIGNED, STEPS>({ring.at + ahead * STEPS * 768}, places, list.slot,
+                                  t + (STAGES - 1) * step + w.entry, a.entries_log, hi, w.live);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            ahead = ahead + 1 == STAGES ? 0 : ahead + 1;
+            Taken<STEPS> key, value;
+            key.take(now, 0, places.ks, places.k_scale);
+            value.take(now, 1, places.vs, places.v_scale);
             float s[STEPS * RP];
 #pragma unroll
             for (int u = 0; u < STEPS; u++) {
                 u64 c[4];
-                code_pairs(now.k[u], a.k.flip, c);
+                code_pairs(key.codes[u], a.k.flip, c);
 #pragma unroll
-                for (int r = 0; r < RP; r++) s[u * RP + r] = r < RB ? fmaf(now.ks[u], dot_pairs(q[r < RB ? r : 0], c), kb[r < RB ? r : 0]) : 0.0f;
+                for (int r = 0; r < RP; r++) s[u * RP + r] = r < RB ? fmaf(key.scale[u], dot_pairs(q[r < RB ? r : 0], c), kb[r < RB ? r : 0]) : 0.0f;
             }
             Sums::sum(s);
             float p[KEEP], keep[KEEP];
@@ -523,7 +535,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(cons
             for (int x = 0; x < KEEP; x++) {
                 const int e = t + (Sums::value_of(x) / RP << a.entries_log) + w.entry;
                 float th;
-                p[x] = e < hi ? score_of(a, s[x], sm.e.bias[e], th) : -INFINITY;
+                p[x] = e < hi ? score_of(a, s[x], list.bias[e], th) : -INFINITY;
                 float top = p[x];
                 St::over_entries(a.entries_log, [&](int o) { top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o)); });
                 top = fmaxf(top, m[x]);
@@ -546,10 +558,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(cons
 #pragma unroll
             for (int u = 0; u < STEPS; u++) {
                 u64 c[4];
-                code_pairs(now.v[u], a.v.flip, c);
+                code_pairs(value.codes[u], a.v.flip, c);
 #pragma unroll
                 for (int r = 0; r < RB; r++) {
-                    const float pv = Sums::get(p, u * RP + r) * now.vs[u];
+                    const float pv = Sums::get(p, u * RP + r) * value.scale[u];
                     const u64 pp = pair(pv, pv);
 #pragma unroll
                     for (int j = 0; j < 4; j++) acc[r][j] = fma2(pp, c[j], acc[r][j]);
@@ -557,6 +569,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(cons
             }
         }
     }
+    copy_wait<0>();
 #pragma unroll
     for (int x = 0; x < KEEP; x++)
         St::over_entries(a.entries_log, [&](int o) { l[x] += __shfl_xor_sync(0xffffffffu, l[x], o); });
@@ -565,13 +578,14 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(cons
         float v[8], mm = Sums::get(m, r), ll = Sums::get(l, r);
         join_vectors<LANES>(acc[r], a.entries_log, v);
         if (a.slices > 1) {
-            __syncthreads();  // the list, or the previous head's vectors, have been read
-            put8(sm.joined[warp] + lane * 8, v);
-            reinterpret_cast<float2*>(sm.joined[warp] + 256)[lane] = make_float2(mm, ll);
+            __syncthreads();  // the rings, or the previous head's vectors, have been read
+            float* mine = reinterpret_cast<float*>(sm) + warp * 320;
+            put8(mine + lane * 8, v);
+            reinterpret_cast<float2*>(mine + 256)[lane] = make_float2(mm, ll);
             __syncthreads();
             if (w.slice == 0) {
                 for (int k = 1; k < a.slices; k++) {
-                    const float* src = sm.joined[warp + k];
+                    const float* src = mine + k * 320;
                     const float2 ml = reinterpret_cast<const float2*>(src + 256)[lane];
                     float o[8], f, g;
                     get8(src + lane * 8, o);
@@ -639,12 +653,13 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_back
     using St = Steps<LANES, RB>;
     using Sums = typename St::Sums;
     constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP;
-    __shared__ union alignas(16) {
-        Entries e;
-        float joined[kMaxWarps][32 * 16 + 64];   // of each lane: A, B; D, P
-    } sm;
+    constexpr int STAGES = St::STAGES;
+    extern __shared__ uint8_t sm[];  // the warps' rings, later the vectors to join; then the entries
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = STEPS << a.entries_log;
     const Work w = work_of<LANES>(a);
+    const int warps = blockDim.x >> 5;
+    const Entries list = entries_at(sm + warps * St::RING, warps);
+    const Slot ring{sm + warp * St::RING};
     u64 q[RB][4], g[RB][4], va[RB][4], vb[RB][4];
     float kb[RB], gb[RB];
     load_heads<RB>(a.q, w.i * a.q_stride, a.q_head_stride, a.dtype, w, a.q_vec, a.scale, q, kb);
@@ -670,23 +685,34 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_back
     const int j1 = (int)min((int64_t)j0 + a.split_len, (int64_t)a.found);
     for (int from = j0; from < j1; from += (blockDim.x >> 5) * kRound) {
         int lo, hi;
-        slice_of(list_entries(a, sm.e, w.i, doc, from, j1), w.slice, a.slices, step, lo, hi);
+        slice_of(list_entries(a, list, w.i, doc, from, j1), w.slice, a.slices, step, lo, hi);
         if (w.idle) hi = lo;
-        Rows<STEPS> next;
-        load_rows<ALIGNED, STEPS>(next, places, sm.e.slot, lo + w.entry, a.entries_log, hi, w.live);
+        copy_wait<0>();  // the previous range's last (empty) stages
+#pragma unroll
+        for (int k = 0; k < STAGES - 1; k++)
+            fetch<ALIGNED, STEPS>({ring.at + k * STEPS * 768}, places, list.slot, lo + k * step + w.entry, a.entries_log,
+                                  hi, w.live);
+        int stage = 0, ahead = STAGES - 1;
         for (int t = lo; t < hi; t += step) {
-            const Rows<STEPS> now = next;  // the next entries are loaded while these are used
-            load_rows<ALIGNED, STEPS>(next, places, sm.e.slot, t + step + w.entry, a.entries_log, hi, w.live);
+            copy_wait<STAGES - 2>();
+            const Slot now{ring.at + stage * STEPS * 768};
+            fetch<ALIGNED, STEPS>({ring.at + ahead * STEPS * 768}, places, list.slot,
+                                  t + (STAGES - 1) * step + w.entry, a.entries_log, hi, w.live);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            ahead = ahead + 1 == STAGES ? 0 : ahead + 1;
+            Taken<STEPS> key, value;
+            key.take(now, 0, places.ks, places.k_scale);
+            value.take(now, 1, places.vs, places.v_scale);
             float s[STEPS * RP], dp[STEPS * RP];
 #pragma unroll
             for (int u = 0; u < STEPS; u++) {
                 u64 c[4];
-                code_pairs(now.k[u], a.k.flip, c);
+                code_pairs(key.codes[u], a.k.flip, c);
 #pragma unroll
-                for (int r = 0; r < RP; r++) s[u * RP + r] = r < RB ? fmaf(now.ks[u], dot_pairs(q[r < RB ? r : 0], c), kb[r < RB ? r : 0]) : 0.0f;
-                code_pairs(now.v[u], a.v.flip, c);
+                for (int r = 0; r < RP; r++) s[u * RP + r] = r < RB ? fmaf(key.scale[u], dot_pairs(q[r < RB ? r : 0], c), kb[r < RB ? r : 0]) : 0.0f;
+                code_pairs(value.codes[u], a.v.flip, c);
 #pragma unroll
-                for (int r = 0; r < RP; r++) dp[u * RP + r] = r < RB ? fmaf(now.vs[u], dot_pairs(g[r < RB ? r : 0], c), gb[r < RB ? r : 0]) : 0.0f;
+                for (int r = 0; r < RP; r++) dp[u * RP + r] = r < RB ? fmaf(value.scale[u], dot_pairs(g[r < RB ? r : 0], c), gb[r < RB ? r : 0]) : 0.0f;
             }
             Sums::sum(s);
             Sums::sum(dp);
@@ -697,21 +723,21 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_back
                 fa[x] = fb[x] = 0.0f;
                 if (e < hi && r < w.nr) {
                     float th;
-                    const float sc = score_of(a, s[x], sm.e.bias[e], th);
+                    const float sc = score_of(a, s[x], list.bias[e], th);
                     const float p = exp_fast(sc - z[x]), pdp = p * dp[x], slope = 1.0f - th * th;
                     dsum[x] += pdp;
                     psum[x] += p;
                     fa[x] = pdp * slope;
                     fb[x] = p * slope;
                     if (a.pd && lane % Sums::DUP == 0)
-                        a.pd[(w.i * a.heads + w.h0 + r) * a.found + sm.e.place[e]] = make_float2(pdp, p);
+                        a.pd[(w.i * a.heads + w.h0 + r) * a.found + list.place[e]] = make_float2(pdp, p);
                 }
             }
 #pragma unroll
             for (int u = 0; u < STEPS; u++) {
                 u64 c[4];
-                code_pairs(now.k[u], a.k.flip, c);
-                const u64 kss = pair(now.ks[u], now.ks[u]);
+                code_pairs(key.codes[u], a.k.flip, c);
+                const u64 kss = pair(key.scale[u], key.scale[u]);
 #pragma unroll
                 for (int j = 0; j < 4; j++) c[j] = fma2(kss, c[j], kbase);  // the key's values
 #pragma unroll
@@ -727,6 +753,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_back
             }
         }
     }
+    copy_wait<0>();
 #pragma unroll
     for (int x = 0; x < KEEP; x++)
         St::over_entries(a.entries_log, [&](int o) {
@@ -739,14 +766,15 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_back
         join_vectors<LANES>(va[r], a.entries_log, x);
         join_vectors<LANES>(vb[r], a.entries_log, y);
         if (a.slices > 1) {
-            __syncthreads();  // the list, or the previous head's vectors, have been read
-            put8(sm.joined[warp] + lane * 8, x);
-            put8(sm.joined[warp] + 256 + lane * 8, y);
-            reinterpret_cast<float2*>(sm.joined[warp] + 512)[lane] = make_float2(sd, sp);
+            __syncthreads();  // the rings, or the previous head's vectors, have been read
+            float* mine = reinterpret_cast<float*>(sm) + warp * 576;
+            put8(mine + lane * 8, x);
+            put8(mine + 256 + lane * 8, y);
+            reinterpret_cast<float2*>(mine + 512)[lane] = make_float2(sd, sp);
             __syncthreads();
             if (w.slice == 0) {
                 for (int k = 1; k < a.slices; k++) {
-                    const float* src = sm.joined[warp + k];
+                    const float* src = mine + k * 576;
                     const float2 dp = reinterpret_cast<const float2*>(src + 512)[lane];
                     float o[8], h[8];
                     get8(src + lane * 8, o);
@@ -841,24 +869,26 @@ int lanes_of(const AttendParams& p) {
 }
 
 // How a call is laid out over warps and blocks.  Units side by side in a warp
-// need no join, so lane groups take entries of one unit only where the GPU's
-// warps would not be filled otherwise; then several warps of a block share
-// units' lists, and then blocks take ranges of a list; no slice is below
-// kMinSlice entries.
+// need no join, so lane groups take entries of one unit only where fewer than
+// kEnough warps would have work (2,048 queries x 4 units: 48 us with four
+// units side by side, 58 us with two and twice the warps); then several warps
+// of a block share units' lists, and then blocks take ranges of a list, up to
+// kFill warps; no slice is below kMinSlice entries.
 void lay_out(AttendParams& p) {
-    constexpr int64_t kFill = 148 * 12;  // warps
+    constexpr int64_t kEnough = 148 * 8, kFill = 148 * 16;
     p.r_blocks = (int)ceil_div(p.shared, kMaxShared);
     p.rb = (int)ceil_div(p.shared, p.r_blocks);
     p.units = p.heads / p.shared * p.r_blocks;
     int side = 32 / lanes_of(p);
     p.entries_log = 0;
-    while (side > 1 && (side / 2 >= p.units || p.queries * ceil_div(p.units, side) < kFill)) side /= 2, p.entries_log++;
+    while (side > 1 && (side / 2 >= p.units || p.queries * ceil_div(p.units, side) < kEnough))
+        side /= 2, p.entries_log++;
     const int64_t unit_warps = ceil_div(p.units, side);
     p.unit_blocks = (int)ceil_div(unit_warps, kMaxWarps);
     p.block_warps = (int)ceil_div(unit_warps, p.unit_blocks);
     const int64_t warps = std::max<int64_t>(1, p.queries * p.unit_blocks * p.block_warps);
     p.slices = (int)std::max<int64_t>(
-        1, std::min({(int64_t)kMaxWarps / p.block_warps, ceil_div(p.found, kMinSlice), ceil_div(kFill, warps)}));
+        1, std::min({(int64_t)kMaxWarps / p.block_warps, ceil_div(p.found, kMinSlice), kFill / warps}));
     const int64_t splits = std::min(ceil_div(p.found, p.slices * kMinSlice), kFill / (warps * p.slices));
     p.split_len = (int)std::max<int64_t>(1, ceil_div(p.found, std::max<int64_t>(1, splits)));
     p.splits = (int)std::max<int64_t>(1, ceil_div(p.found, p.split_len));
@@ -964,7 +994,19 @@ void by_shape(const AttendParams& p, F&& fn) {
 dim3 attend_grid(const AttendParams& p) {
     return dim3((unsigned)(p.queries * p.unit_blocks), (unsigned)p.splits);
 }
-int attend_threads(const AttendParams& p) { return 32 * p.block_warps * p.slices; }
+template <int LANES, int RB, bool ALIGNED, bool BACKWARD>
+void launch_form(const AttendParams& p, cudaStream_t st) {
+    constexpr int kWarpBytes = Steps<LANES, RB>::RING + kEntriesBytes;
+    const auto kernel = BACKWARD ? k_attend_backward<LANES, RB, ALIGNED> : k_attend<LANES, RB, ALIGNED>;
+    static std::atomic<uint64_t> set{0};  // a bit a device
+    const int dev = current_device(), warps = p.block_warps * p.slices;
+    if (!(set.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+        MDH_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxWarps * kWarpBytes));
+        set.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
+    }
+    kernel<<<attend_grid(p), 32 * warps, warps * kWarpBytes, st>>>(p);
+    check_launch();
+}
 
 }  // namespace
 }  // namespace mdh
@@ -993,9 +1035,8 @@ mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_
         p.lse = lse;
         p.part = p.splits > 1 ? (float*)ws : nullptr;
         by_shape(p, [&](auto lanes, auto rb, auto aligned) {
-            k_attend<lanes, rb, aligned><<<attend_grid(p), attend_threads(p), 0, st>>>(p);
+            launch_form<lanes, rb, aligned, false>(p, st);
         });
-        check_launch();
         if (p.splits > 1) {
             k_attend_join<<<(unsigned)(p.queries * p.heads), 128, 0, st>>>(p);
             check_launch();
@@ -1037,9 +1078,8 @@ mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, c
         p.dout_vec = aligned16(dout) && a->head * dtype_size(a->dtype) % 16 == 0;
         p.lse_in = lse;
         by_shape(p, [&](auto lanes, auto rb, auto aligned) {
-            k_attend_backward<lanes, rb, aligned><<<attend_grid(p), attend_threads(p), 0, st>>>(p);
+            launch_form<lanes, rb, aligned, true>(p, st);
         });
-        check_launch();
         if (p.splits > 1) {
             k_attend_backward_join<<<(unsigned)(p.queries * p.heads), 128, 0, st>>>(p);
             check_launch();

@@ -7,9 +7,16 @@
 //   db = sum_r dy.
 // Both are bound by memory: about ten operations an element.
 //
+// Blocks stay and take rows in turn, so the weights are read once a block.
+// What bounds them is the latency of memory: each thread copies its share of
+// the next rows, three where they fit (16-byte vectors where base, stride and width allow,
+// else one by one) into its own places of a ring in shared memory.
 // A row belongs to one warp up to 1024 elements (its sums are shuffles), to a
-// block beyond; a thread holds 8, 16 or 32 elements of the row in registers,
-// in 16-byte vectors where base, stride and width allow, else one by one.
+// group of warps beyond, 16 elements a thread; weights, and backward the
+// running sums of a thread's columns, stay in registers.
+#include <algorithm>
+#include <atomic>
+
 #include "op_common.cuh"
 
 namespace mdh {
@@ -21,17 +28,18 @@ constexpr int kWarpsPerBlock = 8;     // rows at a time of a block, warp form
 constexpr int kBlockElems = 16;       // elements of a thread, block form
 constexpr int kMaxWidth = 16384;
 
-// Sum of `v` over the threads of a row: a warp, or (WIDE) the whole block.
-template <bool WIDE>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-    v = warp_sum(v);
-    if constexpr (WIDE) {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = blockDim.x >> 5;
-        __syncthreads();  // the previous sum has been read
+// Sums over the `warps` warps of a row that share barrier `id` and red[warps].
+__device__ __forceinline__ float2 row_sums(float2 v, float2* red, int warp, int warps, int id) {
+    v.x = warp_sum(v.x);
+    v.y = warp_sum(v.y);
+    if (warps > 1) {
+        const int lane = threadIdx.x & 31;
+        asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(32 * warps) : "memory");  // the previous sums have been read
         if (lane == 0) red[warp] = v;
-        __syncthreads();
-        v = lane < n ? red[lane] : 0.0f;
-        v = warp_sum(v);
+        asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(32 * warps) : "memory");
+        v = lane < warps ? red[lane] : make_float2(0.0f, 0.0f);
+        v.x = warp_sum(v.x);
+        v.y = warp_sum(v.y);
     }
     return v;
 }
@@ -58,173 +66,253 @@ __device__ __forceinline__ void load_weights(const void* w, bool w_f32, int c, f
     }
 }
 
-template <class T, int V, int ELEMS, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? 1024 : 32 * kWarpsPerBlock)
+// A thread's places for its shares of the next rows: elements (i * nt + t) * V
+// + 0 .. V - 1 of a row.  Those past the width are 0 and stay so.
+// A ring has four stages, fewer where a block's rows are too large for them.
+constexpr int stages_of(int threads, int bytes) {
+    return threads * bytes * 4 <= 144 * 1024 ? 4 : threads * bytes * 2 <= 144 * 1024 ? 2 : 1;
+}
+template <class T, int V, int NV, int STAGES>
+struct Ring {
+    Pack<T, V>* at;  // of this thread: place i of stage s at [(s * NV + i) * threads]
+    __device__ __forceinline__ Ring(void* smem, int t, int nt, int width) : at(static_cast<Pack<T, V>*>(smem) + threadIdx.x) {
+        Pack<T, V> zero;
+#pragma unroll
+        for (int j = 0; j < V; j++) zero.v[j] = from_f32<T>(0.0f);
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            if ((i * nt + t) * V >= width)
+                for (int s = 0; s < STAGES; s++) at[(s * NV + i) * blockDim.x] = zero;
+    }
+    __device__ __forceinline__ void fetch(int stage, const T* row, int t, int nt, int width) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * nt + t) * V;
+            Pack<T, V>* to = at + (stage * NV + i) * blockDim.x;
+            if (c >= width) continue;
+            if constexpr (V * sizeof(T) >= 4) copy_async<V * sizeof(T)>(to, row + c);
+            else *to = load_pack<T, V>(row + c);
+        }
+    }
+    __device__ __forceinline__ void take(int stage, Pack<T, V> (&raw)[NV]) const {
+#pragma unroll
+        for (int i = 0; i < NV; i++) raw[i] = at[(stage * NV + i) * blockDim.x];
+    }
+};
+
+// Elements 2 p and 2 p + 1 of a thread's share as floats.
+template <class T, int V, int NV>
+__device__ __forceinline__ f32x2 pair_of(const Pack<T, V> (&raw)[NV], int p) {
+    return pair(to_f32(raw[2 * p / V].v[2 * p % V]), to_f32(raw[(2 * p + 1) / V].v[(2 * p + 1) % V]));
+}
+// Pairs -> the share's vectors in memory (those inside the width).
+template <class T, int V, int NV>
+__device__ __forceinline__ void store_row(T* row, const f32x2 (&v)[NV * V / 2], int t, int nt, int width) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * nt + t) * V;
+        Pack<T, V> p;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float2 f = unpair(v[(i * V + j) / 2]);
+            p.v[j] = from_f32<T>((i * V + j) % 2 ? f.y : f.x);
+        }
+        if (c < width) store_pack<T, V>(row + c, p);
+    }
+}
+
+// A thread's weights, `fallback` where there are none.
+template <class T, int V, int NV>
+__device__ __forceinline__ void load_share(const void* w, bool w_f32, float fallback, int t, int nt, int width,
+                                           f32x2 (&out)[NV * V / 2]) {
+    float f[NV * V];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * nt + t) * V;
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) v[j] = fallback;
+        if (w && c < width) load_weights<T, V>(w, w_f32, c, v);
+#pragma unroll
+        for (int j = 0; j < V; j++) f[i * V + j] = v[j];
+    }
+#pragma unroll
+    for (int p = 0; p < NV * V / 2; p++) out[p] = pair(f[2 * p], f[2 * p + 1]);
+}
+
+template <class T, int V, int ELEMS, bool WIDE, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
     k_norm_forward(const T* __restrict__ x, int64_t x_stride, const void* __restrict__ w, const void* __restrict__ b,
                    bool w_f32, int64_t rows, int width, float eps, T* __restrict__ y, int64_t y_stride,
                    float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    constexpr int NV = ELEMS / V;
-    __shared__ float red[32];
-    const int64_t row = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWarpsPerBlock + (threadIdx.x >> 5);
-    if (row >= rows) return;
+    constexpr int NV = ELEMS / V, PAIRS = ELEMS / 2, STAGES = stages_of(THREADS, ELEMS * sizeof(T));
+    __shared__ float2 red[32];
+    extern __shared__ float4 smem4[];  // the ring
     const int t = WIDE ? threadIdx.x : threadIdx.x & 31, nt = WIDE ? blockDim.x : 32;
-    const T* xr = x + row * x_stride;
-    float v[NV][V];
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int c = (i * nt + t) * V;
-        if (c < width) {
-            const Pack<T, V> p = load_pack<T, V>(xr + c);
-#pragma unroll
-            for (int j = 0; j < V; j++) sum += v[i][j] = to_f32(p.v[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; j++) v[i][j] = 0.0f;
-        }
+    int64_t row = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWarpsPerBlock + (threadIdx.x >> 5);
+    const int64_t step = WIDE ? gridDim.x : (int64_t)gridDim.x * kWarpsPerBlock;
+    Ring<T, V, NV, STAGES> ring(smem4, t, nt, width);
+    for (int k = 0; k < STAGES - 1; k++) {
+        if (row + k * step < rows) ring.fetch(k, x + (row + k * step) * x_stride, t, nt, width);
+        copy_commit();
     }
-    const float mean = row_sum<WIDE>(sum, red) / (float)width;
-    float sq = 0.0f;
+    f32x2 fw[PAIRS], fb[PAIRS];
+    load_share<T, V, NV>(w, w_f32, 1.0f, t, nt, width, fw);
+    load_share<T, V, NV>(b, w_f32, 0.0f, t, nt, width, fb);
+    for (int stage = 0; row < rows; row += step, stage = (stage + 1) % STAGES) {
+        if (STAGES == 1) ring.fetch(0, x + row * x_stride, t, nt, width), copy_commit();
+        copy_wait<STAGES == 1 ? 0 : STAGES - 2>();
+        Pack<T, V> raw[NV];
+        ring.take(stage, raw);
+        f32x2 v[PAIRS];
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        if ((i * nt + t) * V < width) {
+        for (int p = 0; p < PAIRS; p++) v[p] = pair_of<T, V, NV>(raw, p);
+        const int64_t ahead = row + (STAGES - 1) * step;
+        if (STAGES > 1 && ahead < rows) ring.fetch((stage + STAGES - 1) % STAGES, x + ahead * x_stride, t, nt, width);
+        copy_commit();
+        f32x2 sum = 0;
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float d = v[i][j] - mean;
-                sq += d * d;
+        for (int p = 0; p < PAIRS; p++) sum = add2(sum, v[p]);
+        const float2 s = unpair(sum);
+        const float mean =
+            row_sums(make_float2(s.x + s.y, 0.0f), red, threadIdx.x >> 5, WIDE ? nt >> 5 : 1, 0).x / (float)width;
+        const f32x2 away = pair(-mean, -mean);
+        f32x2 sq = 0;
+#pragma unroll
+        for (int p = 0; p < PAIRS; p++) {
+            v[p] = add2(v[p], away);
+            // Elements past the width deviate by 0.  A warp's share is full up to its last 8 elements.
+            if (WIDE || 2 * p >= ELEMS - 8) {
+                const float2 f = unpair(v[p]);
+                v[p] = pair((2 * p / V * nt + t) * V < width ? f.x : 0.0f,
+                            ((2 * p + 1) / V * nt + t) * V < width ? f.y : 0.0f);
             }
+            sq = fma2(v[p], v[p], sq);
         }
-    }
-    const float rstd = 1.0f / sqrtf(row_sum<WIDE>(sq, red) / (float)width + eps);
-    if (t == 0) {
-        if (mean_out) mean_out[row] = mean;
-        if (rstd_out) rstd_out[row] = rstd;
-    }
-    T* yr = y + row * y_stride;
+        const float2 q = unpair(sq);
+        const float var =
+            row_sums(make_float2(q.x + q.y, 0.0f), red, threadIdx.x >> 5, WIDE ? nt >> 5 : 1, 0).x / (float)width;
+        const float rstd = 1.0f / sqrtf(var + eps);
+        if (t == 0) {
+            if (mean_out) mean_out[row] = mean;
+            if (rstd_out) rstd_out[row] = rstd;
+        }
+        const f32x2 rr = pair(rstd, rstd);
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int c = (i * nt + t) * V;
-        if (c >= width) continue;
-        float ww[V], bb[V];
-#pragma unroll
-        for (int j = 0; j < V; j++) ww[j] = 1.0f, bb[j] = 0.0f;
-        if (w) load_weights<T, V>(w, w_f32, c, ww);
-        if (b) load_weights<T, V>(b, w_f32, c, bb);
-        Pack<T, V> p;
-#pragma unroll
-        for (int j = 0; j < V; j++) p.v[j] = from_f32<T>((v[i][j] - mean) * rstd * ww[j] + bb[j]);
-        store_pack<T, V>(yr + c, p);
+        for (int p = 0; p < PAIRS; p++) v[p] = fma2(mul2(v[p], rr), fw[p], fb[p]);
+        store_row<T, V, NV>(y + row * y_stride, v, t, nt, width);
     }
 }
 
-// Blocks take rows in turn; each thread sums dw and db of its columns over
-// its rows, the warps of a block join theirs in shared memory, and the block
-// writes one partial row of part[block][2][width].
-template <class T, int V, int ELEMS, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? 1024 : 32 * kWarpsPerBlock)
+// Each thread sums dw and db of its columns over its rows, the groups of a
+// block join theirs in shared memory in order, and the block writes one
+// partial row of part[block][2][width].  `group` threads hold a row.
+template <class T, int V, int ELEMS, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 3 : 1)
     k_norm_backward(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride,
                     const void* __restrict__ w, bool w_f32, const float* __restrict__ mean_in,
-                    const float* __restrict__ rstd_in, int64_t rows, int width, T* __restrict__ dx, int64_t dx_stride,
-                    float* __restrict__ part) {
-    constexpr int NV = ELEMS / V;
-    __shared__ float red[32];
-    extern __shared__ float joined[];  // warp form: [2][width]
-    const int warp = threadIdx.x >> 5;
-    const int t = WIDE ? threadIdx.x : threadIdx.x & 31, nt = WIDE ? blockDim.x : 32;
-    float dw[NV][V], db[NV][V];
-#pragma unroll
-    for (int i = 0; i < NV; i++)
-#pragma unroll
-        for (int j = 0; j < V; j++) dw[i][j] = db[i][j] = 0.0f;
-    const int64_t step = WIDE ? gridDim.x : (int64_t)gridDim.x * kWarpsPerBlock;
-    for (int64_t row = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWarpsPerBlock + warp; row < rows;
-         row += step) {
-        const float mean = mean_in[row], rstd = rstd_in[row];
-        float xh[NV][V], g[NV][V];
-        float sg = 0.0f, sgx = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * nt + t) * V;
-#pragma unroll
-            for (int j = 0; j < V; j++) xh[i][j] = g[i][j] = 0.0f;
-            if (c >= width) continue;
-            const Pack<T, V> px = load_pack<T, V>(x + row * x_stride + c);
-            const Pack<T, V> pd = load_pack<T, V>(dy + row * dy_stride + c);
-            float ww[V];
-#pragma unroll
-            for (int j = 0; j < V; j++) ww[j] = 1.0f;
-            if (w) load_weights<T, V>(w, w_f32, c, ww);
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float d = to_f32(pd.v[j]);
-                xh[i][j] = (to_f32(px.v[j]) - mean) * rstd;
-                g[i][j] = d * ww[j];
-                dw[i][j] += d * xh[i][j];
-                db[i][j] += d;
-                sg += g[i][j];
-                sgx += g[i][j] * xh[i][j];
-            }
+                    const float* __restrict__ rstd_in, int64_t rows, int width, int group, T* __restrict__ dx,
+                    int64_t dx_stride, float* __restrict__ part) {
+    constexpr int NV = ELEMS / V, PAIRS = ELEMS / 2, STAGES = stages_of(THREADS, 2 * ELEMS * sizeof(T));
+    __shared__ float2 red[32];
+    extern __shared__ float4 smem4[];  // the rings of x and dy, (mean, rstd); at the end the sums to join
+    const int g = threadIdx.x / group, t = threadIdx.x - g * group, groups = blockDim.x / group, warps = group >> 5;
+    int64_t row = (int64_t)blockIdx.x * groups + g;
+    const int64_t step = (int64_t)gridDim.x * groups;
+    constexpr int kRing = STAGES * ELEMS * sizeof(T);  // bytes a thread
+    uint8_t* smem = reinterpret_cast<uint8_t*>(smem4);
+    Ring<T, V, NV, STAGES> ring_x(smem, t, group, width), ring_d(smem + kRing * blockDim.x, t, group, width);
+    // (mean, rstd) of each warp's next rows.
+    float* stats = reinterpret_cast<float*>(smem + 2 * kRing * blockDim.x) + (threadIdx.x >> 5) * 2 * STAGES;
+    float* joined = reinterpret_cast<float*>(smem);  // [2][width], once the rows are done
+    auto fetch = [&](int stage, int64_t r) {
+        ring_x.fetch(stage, x + r * x_stride, t, group, width);
+        ring_d.fetch(stage, dy + r * dy_stride, t, group, width);
+        if ((threadIdx.x & 31) == 0) {
+            copy_async<4>(stats + 2 * stage, mean_in + r);
+            copy_async<4>(stats + 2 * stage + 1, rstd_in + r);
         }
+    };
+    for (int k = 0; k < STAGES - 1; k++) {
+        if (row + k * step < rows) fetch(k, row + k * step);
+        copy_commit();
+    }
+    f32x2 fw[PAIRS];
+    load_share<T, V, NV>(w, w_f32, 1.0f, t, group, width, fw);
+    f32x2 dw[PAIRS], db[PAIRS];
+#pragma unroll
+    for (int p = 0; p < PAIRS; p++) dw[p] = db[p] = 0;
+    for (int stage = 0; row < rows; row += step, stage = (stage + 1) % STAGES) {
+        if (STAGES == 1) fetch(0, row), copy_commit();
+        copy_wait<STAGES == 1 ? 0 : STAGES - 2>();
+        __syncwarp();  // lane 0 copied the statistics
+        Pack<T, V> px[NV], pd[NV];
+        ring_x.take(stage, px);
+        ring_d.take(stage, pd);
+        f32x2 xh[PAIRS], gy[PAIRS], sg = 0, sgx = 0;
+        const f32x2 away = pair(-stats[2 * stage], -stats[2 * stage]), rr = pair(stats[2 * stage + 1], stats[2 * stage + 1]);
+#pragma unroll
+        for (int p = 0; p < PAIRS; p++) {
+            // dy is 0 past the width, so whatever x and w hold there adds nothing.
+            const f32x2 d = pair_of<T, V, NV>(pd, p);
+            xh[p] = mul2(add2(pair_of<T, V, NV>(px, p), away), rr);
+            gy[p] = mul2(d, fw[p]);
+            dw[p] = fma2(d, xh[p], dw[p]);
+            db[p] = add2(db[p], d);
+            sg = add2(sg, gy[p]);
+            sgx = fma2(gy[p], xh[p], sgx);
+        }
+        __syncwarp();  // the statistics have been read
+        const int64_t ahead = row + (STAGES - 1) * step;
+        if (STAGES > 1 && ahead < rows) fetch((stage + STAGES - 1) % STAGES, ahead);
+        copy_commit();
         if (dx) {
-            const float mg = row_sum<WIDE>(sg, red) / (float)width;
-            const float mgx = row_sum<WIDE>(sgx, red) / (float)width;
+            const float2 a = unpair(sg), b = unpair(sgx);
+            const float2 s = row_sums(make_float2(a.x + a.y, b.x + b.y), red + g * warps, t >> 5, warps, 1 + g);
+            const float mg = s.x / (float)width, mgx = s.y / (float)width;
+            const f32x2 mg2 = pair(-mg, -mg), mgx2 = pair(-mgx, -mgx);
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                const int c = (i * nt + t) * V;
-                if (c >= width) continue;
-                Pack<T, V> p;
-#pragma unroll
-                for (int j = 0; j < V; j++) p.v[j] = from_f32<T>(rstd * (g[i][j] - mg - xh[i][j] * mgx));
-                store_pack<T, V>(dx + row * dx_stride + c, p);
-            }
+            for (int p = 0; p < PAIRS; p++) gy[p] = mul2(rr, fma2(xh[p], mgx2, add2(gy[p], mg2)));
+            store_row<T, V, NV>(dx + row * dx_stride, gy, t, group, width);
         }
     }
     if (!part) return;
+    copy_wait<0>();
+    __syncthreads();  // the rings are free
     float* out = part + (int64_t)blockIdx.x * 2 * width;
-    if constexpr (WIDE) {
+    for (int k = 0; k < groups; k++) {
+        float* dst = k + 1 == groups ? out : joined;
+        if (g == k) {
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * nt + t) * V;
-            if (c >= width) continue;
-#pragma unroll
-            for (int j = 0; j < V; j++) out[c + j] = dw[i][j], out[width + c + j] = db[i][j];
-        }
-    } else {
-        // The warps add theirs one after another: a fixed order.
-        for (int k = 0; k < kWarpsPerBlock; k++) {
-            if (warp == k) {
-#pragma unroll
-                for (int i = 0; i < NV; i++) {
-                    const int c = (i * nt + t) * V;
-                    if (c >= width) continue;
-#pragma unroll
-                    for (int j = 0; j < V; j++) {
-                        joined[c + j] = (k ? joined[c + j] : 0.0f) + dw[i][j];
-                        joined[width + c + j] = (k ? joined[width + c + j] : 0.0f) + db[i][j];
-                    }
-                }
+            for (int e = 0; e < ELEMS; e++) {
+                const int c = (e / V * group + t) * V + e % V;
+                if (c >= width) continue;
+                const float2 fw = unpair(dw[e / 2]), fb = unpair(db[e / 2]);
+                dst[c] = (k ? joined[c] : 0.0f) + (e % 2 ? fw.y : fw.x);
+                dst[width + c] = (k ? joined[width + c] : 0.0f) + (e % 2 ? fb.y : fb.x);
             }
-            __syncthreads();
         }
-        for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) out[c] = joined[c];
+        __syncthreads();
     }
 }
 
-// Column sums of part[n][2][width]: 32 columns of a block, its 8 warps each
-// take every eighth partial row, joined in order.
+// Column sums of part[n][2][width]: 32 columns of a block, its 32 warps each
+// take every 32nd partial row, joined in order.
 template <class W>
-__global__ void __launch_bounds__(256) k_norm_join(const float* __restrict__ part, int n, int width,
-                                                   W* __restrict__ dw, W* __restrict__ db) {
-    __shared__ float s[8][33];
+__global__ void __launch_bounds__(1024) k_norm_join(const float* __restrict__ part, int n, int width,
+                                                    W* __restrict__ dw, W* __restrict__ db) {
+    __shared__ float s[32][33];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c = blockIdx.x * 32 + lane;
     float v = 0.0f;
-    if (c < 2 * width)
-        for (int i = warp; i < n; i += 8) v += part[(int64_t)i * 2 * width + c];
+    if (c < 2 * width) {
+#pragma unroll 4
+        for (int i = warp; i < n; i += 32) v += part[(int64_t)i * 2 * width + c];
+    }
     s[warp][lane] = v;
     __syncthreads();
     if (warp == 0 && c < 2 * width) {
-        for (int k = 1; k < 8; k++) v += s[k][lane];
+        for (int k = 1; k < 32; k++) v += s[k][lane];
         if (c < width) {
             if (dw) dw[c] = from_f32<W>(v);
         } else if (db) {
@@ -233,9 +321,13 @@ __global__ void __launch_bounds__(256) k_norm_join(const float* __restrict__ par
     }
 }
 
+// Backward: threads that hold a row, such groups in a block (named barriers 1
+// .. 4 serve those of several warps), and blocks that stay.
+int backward_group(int width) { return width <= 1024 ? 32 : (int)round_up(ceil_div(width, kBlockElems), 32); }
+int backward_groups(int width) { return std::max(1, 128 / backward_group(width)); }
 int backward_blocks(int64_t rows, int width) {
-    const int64_t units = width <= 1024 ? ceil_div(rows, kWarpsPerBlock) : rows;
-    return (int)std::min<int64_t>(units, 148 * 2);
+    const int groups = backward_groups(width), stay = std::max(1, 384 / (backward_group(width) * groups));
+    return (int)std::min<int64_t>(ceil_div(rows, groups), 148 * stay);
 }
 
 void check_norm(const void* x, int64_t x_stride, int32_t dtype, int32_t w_dtype, int64_t rows, int32_t width) {
@@ -248,18 +340,33 @@ void check_norm(const void* x, int64_t x_stride, int32_t dtype, int32_t w_dtype,
     MDH_REQUIRE(rows <= 1 || x_stride >= width, MDH_ERR_INVALID_ARG, "layer norm: row stride below the width");
 }
 
-// fn(V, ELEMS, WIDE) as compile-time values.
+// Lets KERNEL have `BYTES` of dynamic shared memory on the current device.
+template <auto KERNEL, size_t BYTES>
+void allow_shared() {
+    static_assert(BYTES <= 227 * 1024, "shared memory budget");
+    static std::atomic<uint64_t> set{0};  // a bit a device
+    const uint64_t bit = uint64_t(1) << (current_device() & 63);
+    if (BYTES <= 48 * 1024 || (set.load(std::memory_order_relaxed) & bit)) return;
+    MDH_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BYTES));
+    set.fetch_or(bit, std::memory_order_relaxed);
+}
+
+// fn(V, ELEMS, WIDE, THREADS) as compile-time values.
 template <class T, class F>
 void by_shape(bool vec, int width, F&& fn) {
     constexpr int V = 16 / sizeof(T);
+    using std::integral_constant;
+    const integral_constant<int, 32 * kWarpsPerBlock> small{};
     auto elems = [&](auto v) {
-        if (width <= 256) fn(v, std::integral_constant<int, 8>{}, std::false_type{});
-        else if (width <= 512) fn(v, std::integral_constant<int, 16>{}, std::false_type{});
-        else if (width <= 1024) fn(v, std::integral_constant<int, 32>{}, std::false_type{});
-        else fn(v, std::integral_constant<int, kBlockElems>{}, std::true_type{});
+        if (width <= 256) fn(v, integral_constant<int, 8>{}, std::false_type{}, small);
+        else if (width <= 512) fn(v, integral_constant<int, 16>{}, std::false_type{}, small);
+        else if (width <= 768) fn(v, integral_constant<int, 24>{}, std::false_type{}, small);
+        else if (width <= 1024) fn(v, integral_constant<int, 32>{}, std::false_type{}, small);
+        else if (width <= 8192) fn(v, integral_constant<int, kBlockElems>{}, std::true_type{}, integral_constant<int, 512>{});
+        else fn(v, integral_constant<int, kBlockElems>{}, std::true_type{}, integral_constant<int, 1024>{});
     };
-    if (vec) elems(std::integral_constant<int, V>{});
-    else elems(std::integral_constant<int, 1>{});
+    if (vec) elems(integral_constant<int, V>{});
+    else elems(integral_constant<int, 1>{});
 }
 
 }  // namespace
@@ -283,12 +390,16 @@ mdh_status mdh_layer_norm_forward(const void* x, int64_t x_stride, int32_t dtype
             using T = decltype(zero);
             const bool vec = width % (16 / sizeof(T)) == 0 && rows_aligned(x, x_stride, sizeof(T)) &&
                              rows_aligned(y, y_stride, sizeof(T)) && aligned16(w) && aligned16(b);
-            by_shape<T>(vec, width, [&](auto v, auto elems, auto wide) {
+            by_shape<T>(vec, width, [&](auto v, auto elems, auto wide, auto most) {
                 const int threads = wide ? (int)round_up(ceil_div(width, elems), 32) : 32 * kWarpsPerBlock;
-                const int64_t blocks = wide ? rows : ceil_div(rows, kWarpsPerBlock);
-                MDH_REQUIRE(blocks <= INT32_MAX, MDH_ERR_UNSUPPORTED, "layer norm: too many rows");
-                k_norm_forward<T, v, elems, wide><<<(unsigned)blocks, threads, 0, (cudaStream_t)stream>>>(
-                    (const T*)x, x_stride, w, b, w_dtype == MDH_F32, rows, width, eps, (T*)y, y_stride, mean, rstd);
+                const int64_t units = wide ? rows : ceil_div(rows, kWarpsPerBlock);
+                const int64_t stay = 148 * std::max(1, 512 / threads);  // blocks that stay
+                constexpr int kShare = elems * sizeof(T), kRing = stages_of(most, kShare) * kShare;
+                const int smem = kRing * threads;
+                allow_shared<k_norm_forward<T, v, elems, wide, most>, most * kRing>();
+                k_norm_forward<T, v, elems, wide, most>
+                    <<<(unsigned)std::min(units, stay), threads, smem, (cudaStream_t)stream>>>((const T*)x, x_stride, w, b, w_dtype == MDH_F32, rows, width, eps, (T*)y,
+                                               y_stride, mean, rstd);
             });
         });
         check_launch();
@@ -328,18 +439,33 @@ mdh_status mdh_layer_norm_backward(const void* dy, int64_t dy_stride, const void
             const bool vec = width % (16 / sizeof(T)) == 0 && rows_aligned(x, x_stride, sizeof(T)) &&
                              rows_aligned(dy, dy_stride, sizeof(T)) && aligned16(w) &&
                              (!dx || rows_aligned(dx, dx_stride, sizeof(T)));
-            by_shape<T>(vec, width, [&](auto v, auto elems, auto wide) {
-                const int threads = wide ? (int)round_up(ceil_div(width, elems), 32) : 32 * kWarpsPerBlock;
-                k_norm_backward<T, v, elems, wide><<<blocks, threads, wide ? 0 : 2 * width * 4, st>>>(
+            const int group = backward_group(width), groups = backward_groups(width);
+            auto launch = [&](auto v, auto elems, auto most) {
+                constexpr int kShare = 2 * elems * sizeof(T), kStages = stages_of(most, kShare);
+                const int rings = group * groups * kStages * kShare + 8 * kStages * (group * groups / 32);
+                const int smem = std::max(rings, groups > 1 ? 2 * width * 4 : 0);
+                allow_shared<k_norm_backward<T, v, elems, most>, most * kStages * kShare + 8192>();
+                k_norm_backward<T, v, elems, most><<<blocks, group * groups, smem, st>>>(
                     (const T*)dy, dy_stride, (const T*)x, x_stride, w, w_dtype == MDH_F32, mean, rstd, rows, width,
-                    (T*)dx, dx_stride, sums ? (float*)ws : nullptr);
-            });
+                    group, (T*)dx, dx_stride, sums ? (float*)ws : nullptr);
+            };
+            using std::integral_constant;
+            auto by_elems = [&](auto v) {
+                if (width <= 256) launch(v, integral_constant<int, 8>{}, integral_constant<int, 128>{});
+                else if (width <= 512) launch(v, integral_constant<int, 16>{}, integral_constant<int, 128>{});
+                else if (width <= 768) launch(v, integral_constant<int, 24>{}, integral_constant<int, 128>{});
+                else if (width <= 1024) launch(v, integral_constant<int, 32>{}, integral_constant<int, 128>{});
+                else if (width <= 8192) launch(v, integral_constant<int, kBlockElems>{}, integral_constant<int, 512>{});
+                else launch(v, integral_constant<int, kBlockElems>{}, integral_constant<int, 1024>{});
+            };
+            if (vec) by_elems(std::integral_constant<int, 16 / sizeof(T)>{});
+            else by_elems(std::integral_constant<int, 1>{});
         });
         check_launch();
         if (!sums) return;
         by_dtype(w_dtype, [&](auto zero) {
             using W = decltype(zero);
-            k_norm_join<W><<<(unsigned)ceil_div(2 * (int64_t)width, 32), 256, 0, st>>>((const float*)ws, blocks, width,
+            k_norm_join<W><<<(unsigned)ceil_div(2 * (int64_t)width, 32), 1024, 0, st>>>((const float*)ws, blocks, width,
                                                                                     (W*)dw, (W*)db);
         });
         check_launch();

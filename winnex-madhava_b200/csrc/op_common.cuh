@@ -62,6 +62,48 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// Two floats in one register pair: one instruction for two operations.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Starts a copy of BYTES (4, 8 or 16) to shared memory, zeros where `some` is false.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool some = true) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+                 "n"(BYTES), "r"(some ? BYTES : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits for this thread's copies, all but those of the last PENDING commits.
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
 // ------------------------------------------------------------ host side
 inline size_t dtype_size(int32_t t) { return t == MDH_F32 ? 4 : 2; }
 inline bool dtype_ok(int32_t t) { return t == MDH_F32 || t == MDH_BF16 || t == MDH_F16; }
