@@ -847,7 +847,6 @@ __global__ void __launch_bounds__(256) k_attend_dbias(const __grid_constant__ At
     dbias[at] = v;
 }
 
-bool rows_on_8(const RowsView& r) { return reinterpret_cast<uintptr_t>(r.codes) % 8 == 0 && r.stride % 8 == 0; }
 CodeView code_view(const RowsView& r) {
     CodeView c{};
     c.codes = r.codes;

@@ -16,6 +16,9 @@ struct RowsView {
     float lo, step, inv_step;
 };
 
+// Rows start and step on 8 bytes.
+inline bool rows_on_8(const RowsView& r) { return reinterpret_cast<uintptr_t>(r.codes) % 8 == 0 && r.stride % 8 == 0; }
+
 // Checks a caller's cache and gives its view; throws MDH_ERR_INVALID_ARG.
 RowsView rows_view(const mdh_rows* c);
 

@@ -13,11 +13,109 @@ namespace {
 using namespace op;
 
 constexpr int kThreads = 256;
+constexpr int kChunk = 8;  // elements of a thread
 
-// One warp writes one row, group by group.
+// A block is x threads along a row (a power of two) by y rows; no index of
+// an element needs a division.
+dim3 row_block(int width) {
+    int x = 1;
+    while (x * kChunk < width && x < kThreads) x *= 2;
+    return dim3(x, kThreads / x);
+}
+
+// 8 elements from p, zeros past `left`; vec: one or two 16-byte loads.
+template <class T>
+__device__ __forceinline__ void load_chunk(const T* p, int left, bool vec, float (&v)[kChunk]) {
+    if (vec && left >= kChunk) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kChunk / N; i++) {
+            const Pack<T, N> x = load_pack<T, N>(p + i * N);
+#pragma unroll
+            for (int j = 0; j < N; j++) v[i * N + j] = to_f32(x.v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; j++) v[j] = j < left ? to_f32(p[j]) : 0.0f;
+    }
+}
+template <class T>
+__device__ __forceinline__ void store_chunk(T* p, int left, bool vec, const float (&v)[kChunk]) {
+    if (vec && left >= kChunk) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kChunk / N; i++) {
+            Pack<T, N> x;
+#pragma unroll
+            for (int j = 0; j < N; j++) x.v[j] = from_f32<T>(v[i * N + j]);
+            store_pack<T, N>(p + i * N, x);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; j++)
+            if (j < left) p[j] = from_f32<T>(v[j]);
+    }
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, int left, bool vec, const uint32_t (&c)[kChunk]) {
+    if (vec && left >= kChunk) {
+        uint2 w;
+        w.x = (c[0] & 255) | (c[1] & 255) << 8 | (c[2] & 255) << 16 | c[3] << 24;
+        w.y = (c[4] & 255) | (c[5] & 255) << 8 | (c[6] & 255) << 16 | c[7] << 24;
+        *reinterpret_cast<uint2*>(p) = w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; j++)
+            if (j < left) p[j] = (uint8_t)c[j];
+    }
+}
+__device__ __forceinline__ float chunk_max(const float (&v)[kChunk], float a) {
+#pragma unroll
+    for (int j = 0; j < kChunk; j++) a = max_nan(a, fabsf(v[j]));
+    return a;
+}
+__device__ __forceinline__ void encode_group(const float (&v)[kChunk], float inv, uint32_t (&c)[kChunk]) {
+#pragma unroll
+    for (int j = 0; j < kChunk; j++) c[j] = (uint32_t)group_code(v[j], inv);
+}
+
+// uint8, and int8 in groups of `lanes` = 1, 2, 4 .. 32 neighbouring chunks
+// (lanes divides the row's threads or the row is one group): the group's
+// magnitude is a few shuffles.
 template <class T, class I>
 __global__ void __launch_bounds__(kThreads)
-    k_rows_write(RowsView c, const I* __restrict__ ids, const T* __restrict__ rows, int64_t row_stride, int64_t n) {
+    k_rows_write(RowsView c, const I* __restrict__ ids, const T* __restrict__ rows, int64_t row_stride, int64_t n,
+                 int lanes, bool vec_in, bool vec_out) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    // Every thread of a warp goes through the shuffles; rows that are not written store nothing.
+    const int64_t slot = i < n ? (int64_t)ids[i] : -1;
+    const bool write = slot >= 0 && slot < c.slots;
+    const T* x = rows + (write ? i : 0) * row_stride;
+    uint8_t* out = c.codes + (write ? slot : 0) * c.stride;
+    for (int e0 = 0; e0 < c.width; e0 += blockDim.x * kChunk) {
+        const int e = e0 + threadIdx.x * kChunk, left = write ? c.width - e : 0;
+        float v[kChunk];
+        load_chunk(x + (left > 0 ? e : 0), left, vec_in, v);
+        uint32_t code[kChunk];
+        if (c.affine) {
+#pragma unroll
+            for (int j = 0; j < kChunk; j++) code[j] = affine_code(v[j], c.lo, c.inv_step);
+        } else {
+            float a = chunk_max(v, 0.0f), scale, inv;
+            for (int o = lanes / 2; o; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+            group_scale(a, scale, inv);
+            encode_group(v, inv, code);
+            if (left > 0 && threadIdx.x % lanes == 0) c.scales[slot * c.n_groups + e / c.group] = scale;
+        }
+        if (left > 0) store_codes(out + e, left, vec_out, code);
+    }
+}
+
+// int8 in groups of any other size: a warp writes a row, group by group, and
+// reads the group a second time (from the cache) for its codes.
+template <class T, class I>
+__global__ void __launch_bounds__(kThreads)
+    k_rows_write_any(RowsView c, const I* __restrict__ ids, const T* __restrict__ rows, int64_t row_stride, int64_t n,
+                     bool vec_in, bool vec_out) {
     const int lane = threadIdx.x & 31;
     const int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
     if (i >= n) return;
@@ -25,57 +123,59 @@ __global__ void __launch_bounds__(kThreads)
     if (slot < 0 || slot >= c.slots) return;
     const T* x = rows + i * row_stride;
     uint8_t* out = c.codes + slot * c.stride;
-    if (c.affine) {
-        for (int e = lane; e < c.width; e += 32) out[e] = affine_code(to_f32(x[e]), c.lo, c.inv_step);
-        return;
-    }
     for (int g = 0; g < c.n_groups; g++) {
         const int e0 = g * c.group, e1 = min(e0 + c.group, c.width);
-        float a = 0.0f;
-        for (int e = e0 + lane; e < e1; e += 32) a = max_nan(a, fabsf(to_f32(x[e])));
+        float a = 0.0f, v[kChunk], scale, inv;
+        for (int e = e0 + lane * kChunk; e < e1; e += 32 * kChunk) {
+            load_chunk(x + e, e1 - e, vec_in, v);
+            a = chunk_max(v, a);
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-        float scale, inv;
         group_scale(a, scale, inv);
-        for (int e = e0 + lane; e < e1; e += 32) out[e] = (uint8_t)group_code(to_f32(x[e]), inv);
+        for (int e = e0 + lane * kChunk; e < e1; e += 32 * kChunk) {
+            load_chunk(x + e, e1 - e, vec_in, v);
+            uint32_t code[kChunk];
+            encode_group(v, inv, code);
+            store_codes(out + e, e1 - e, vec_out, code);
+        }
         if (lane == 0) c.scales[slot * c.n_groups + g] = scale;
     }
 }
 
-// A thread reads V consecutive elements of one row.
-template <class T, class I, int V>
+template <class T, class I>
 __global__ void __launch_bounds__(kThreads)
-    k_rows_read(RowsView c, const I* __restrict__ ids, int64_t n, int chunks, T* __restrict__ out, int64_t out_stride) {
-    const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    const int64_t i = at / chunks;
+    k_rows_read(RowsView c, const I* __restrict__ ids, int64_t n, bool vec_in, T* __restrict__ out, int64_t out_stride,
+                bool vec_out) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (i >= n) return;
-    const int e = (int)(at - i * chunks) * V;
     const int64_t slot = (int64_t)ids[i];
-    Pack<T, V> p;
-    if (slot < 0 || slot >= c.slots) {
+    const bool some = slot >= 0 && slot < c.slots;
+    for (int e = threadIdx.x * kChunk; e < c.width; e += blockDim.x * kChunk) {
+        const int left = c.width - e;
+        float v[kChunk] = {};
+        if (some) {
+            const uint8_t* src = c.codes + slot * c.stride + e;
+            uint8_t code[kChunk] = {};
+            if (vec_in && left >= kChunk) {
+                *reinterpret_cast<uint2*>(code) = __ldg(reinterpret_cast<const uint2*>(src));
+            } else {
 #pragma unroll
-        for (int j = 0; j < V; j++) p.v[j] = from_f32<T>(0.0f);
-    } else {
-        const uint8_t* src = c.codes + slot * c.stride + e;
-        uint8_t code[V];
-        if constexpr (V == 8) {
-            *reinterpret_cast<uint2*>(code) = __ldg(reinterpret_cast<const uint2*>(src));
-        } else if constexpr (V == 4) {
-            *reinterpret_cast<uint32_t*>(code) = __ldg(reinterpret_cast<const uint32_t*>(src));
-        } else {
-            code[0] = src[0];
+                for (int j = 0; j < kChunk; j++)
+                    if (j < left) code[j] = src[j];
+            }
+            if (c.affine) {
+#pragma unroll
+                for (int j = 0; j < kChunk; j++) v[j] = affine_value(code[j], c.lo, c.step);
+            } else {
+                // Groups are multiples of 16 elements: the chunk has one scale.
+                const float scale = c.scales[slot * c.n_groups + e / c.group];
+#pragma unroll
+                for (int j = 0; j < kChunk; j++) v[j] = (float)(int8_t)code[j] * scale;
+            }
         }
-        if (c.affine) {
-#pragma unroll
-            for (int j = 0; j < V; j++) p.v[j] = from_f32<T>(affine_value(code[j], c.lo, c.step));
-        } else {
-            // Groups are multiples of 16 elements: the V share one scale.
-            const float scale = c.scales[slot * c.n_groups + e / c.group];
-#pragma unroll
-            for (int j = 0; j < V; j++) p.v[j] = from_f32<T>((float)(int8_t)code[j] * scale);
-        }
+        store_chunk(out + i * out_stride + e, left, vec_out, v);
     }
-    store_pack<T, V>(out + i * out_stride + e, p);
 }
 
 template <class F>
@@ -140,14 +240,23 @@ mdh_status mdh_rows_write(const mdh_rows* cache, const void* ids, int32_t id_bit
         current_device();
         if (n == 0 || c.slots == 0) return;
         MDH_REQUIRE(ids && rows, MDH_ERR_INVALID_ARG, "row cache: null ids or rows");
-        const int64_t blocks = ceil_div(n, kThreads / 32);
+        // Chunks of a group, where they are neighbouring lanes: a power of two up to 32.
+        const int lanes = c.affine ? 1 : c.group % kChunk == 0 ? c.group / kChunk : 0;
+        const dim3 block = row_block(c.width);
+        const bool shuffled = lanes >= 1 && lanes <= 32 && (lanes & (lanes - 1)) == 0 && lanes <= (int)block.x;
+        const int64_t blocks = ceil_div(n, shuffled ? block.y : kThreads / 32);
         MDH_REQUIRE(blocks <= INT32_MAX, MDH_ERR_UNSUPPORTED, "row cache: too many rows in one call");
+        const bool vec_in = rows_aligned(rows, row_stride, dtype_size(dtype)), vec_out = rows_on_8(c);
         by_dtype(dtype, [&](auto zero) {
             using T = decltype(zero);
             by_id(id_bits, [&](auto id) {
                 using I = decltype(id);
-                k_rows_write<T, I><<<(unsigned)blocks, kThreads, 0, (cudaStream_t)stream>>>(
-                    c, (const I*)ids, (const T*)rows, row_stride, n);
+                if (shuffled)
+                    k_rows_write<T, I><<<(unsigned)blocks, block, 0, (cudaStream_t)stream>>>(
+                        c, (const I*)ids, (const T*)rows, row_stride, n, lanes, vec_in, vec_out);
+                else
+                    k_rows_write_any<T, I><<<(unsigned)blocks, kThreads, 0, (cudaStream_t)stream>>>(
+                        c, (const I*)ids, (const T*)rows, row_stride, n, vec_in, vec_out);
             });
         });
         check_launch();
@@ -165,22 +274,16 @@ mdh_status mdh_rows_read(const mdh_rows* cache, const void* ids, int32_t id_bits
         current_device();
         if (n == 0) return;
         MDH_REQUIRE(ids && out, MDH_ERR_INVALID_ARG, "row cache: null ids or output");
+        const dim3 block = row_block(c.width);
+        const int64_t blocks = ceil_div(n, block.y);
+        MDH_REQUIRE(blocks <= INT32_MAX, MDH_ERR_UNSUPPORTED, "row cache: too many rows in one call");
+        const bool vec_in = rows_on_8(c), vec_out = rows_aligned(out, out_stride, dtype_size(dtype));
         by_dtype(dtype, [&](auto zero) {
             using T = decltype(zero);
-            constexpr int V = 16 / sizeof(T);
-            const bool vec = c.width % V == 0 && c.stride % V == 0 &&
-                             reinterpret_cast<uintptr_t>(c.codes) % V == 0 && rows_aligned(out, out_stride, sizeof(T));
-            const int chunks = vec ? c.width / V : c.width;
-            const int64_t blocks = ceil_div(n * chunks, kThreads);
-            MDH_REQUIRE(blocks <= INT32_MAX, MDH_ERR_UNSUPPORTED, "row cache: too many rows in one call");
             by_id(id_bits, [&](auto id) {
                 using I = decltype(id);
-                if (vec)
-                    k_rows_read<T, I, V><<<(unsigned)blocks, kThreads, 0, (cudaStream_t)stream>>>(
-                        c, (const I*)ids, n, chunks, (T*)out, out_stride);
-                else
-                    k_rows_read<T, I, 1><<<(unsigned)blocks, kThreads, 0, (cudaStream_t)stream>>>(
-                        c, (const I*)ids, n, chunks, (T*)out, out_stride);
+                k_rows_read<T, I><<<(unsigned)blocks, block, 0, (cudaStream_t)stream>>>(c, (const I*)ids, n, vec_in, (T*)out,
+                                                                                     out_stride, vec_out);
             });
         });
         check_launch();
