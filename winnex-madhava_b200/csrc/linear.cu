@@ -12,48 +12,120 @@ namespace {
 
 using namespace op;
 
-__device__ __forceinline__ float activation_slope(float z, int act) {
-    switch (act) {
-        case MDH_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-        case MDH_ACT_GELU:
-            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-        case MDH_ACT_SILU: {
-            const float e = 1.0f / (1.0f + expf(-z));
-            return e * (1.0f + z * (1.0f - e));
-        }
-        default: return 1.0f;
-    }
-}
-
 // dz [rows][n] = dy act'(z) (dz null: not stored), and part[block][n] = the
-// column sums of a block's rows.
+// column sums of a block's rows.  A lane holds 8 columns, a warp every eighth
+// of the block's rows.  Bound by memory: three passes over [rows][n].
 constexpr int kSlopeRows = 64;
 template <class T>
 __global__ void __launch_bounds__(256)
     k_slope(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z, int act, int64_t rows, int64_t n,
-            T* __restrict__ dz, int64_t dz_stride, float* __restrict__ part) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= n) return;
-    const int64_t r0 = (int64_t)blockIdx.y * kSlopeRows, r1 = min(r0 + kSlopeRows, rows);
-    float sum = 0.0f;
-    for (int64_t r = r0; r < r1; r++) {
-        float v = to_f32(dy[r * dy_stride + c]);
-        if (act != MDH_ACT_NONE) v *= activation_slope(to_f32(z[r * n + c]), act);
-        sum += v;
-        if (dz) dz[r * dz_stride + c] = from_f32<T>(v);
+            T* __restrict__ dz, int64_t dz_stride, float* __restrict__ part, bool vec_dy, bool vec_z) {
+    __shared__ float sums[8][32 * kChunk];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t c = ((int64_t)blockIdx.y * 32 + lane) * kChunk;
+    const int left = (int)min((int64_t)kChunk, n - c);
+    const int64_t r0 = (int64_t)blockIdx.x * kSlopeRows, r1 = min(r0 + kSlopeRows, rows);
+    f32x2 sum[kChunk / 2] = {};
+    auto run = [&](auto known) {  // the activation as a compile-time value
+        constexpr int ACT = decltype(known)::value;
+#pragma unroll 2
+        for (int64_t r = r0 + warp; r < r1; r += 8) {
+            float v[kChunk], zz[kChunk];
+            load_chunk(dy + r * dy_stride + c, left, vec_dy, v);
+            if (ACT != MDH_ACT_NONE) load_chunk(z + r * n + c, left, vec_z, zz);
+#pragma unroll
+            for (int j = 0; j < kChunk / 2; j++) {
+                f32x2 d = pair(v[2 * j], v[2 * j + 1]);
+                if (ACT != MDH_ACT_NONE) d = mul2(d, activation_slope(pair(zz[2 * j], zz[2 * j + 1]), ACT));
+                sum[j] = add2(sum[j], d);
+                const float2 f = unpair(d);
+                v[2 * j] = f.x, v[2 * j + 1] = f.y;
+            }
+            if (dz) store_chunk(dz + r * dz_stride + c, left, true, v);
+        }
+    };
+    if (left > 0) {
+        if (act == MDH_ACT_RELU) run(std::integral_constant<int, MDH_ACT_RELU>{});
+        else if (act == MDH_ACT_GELU) run(std::integral_constant<int, MDH_ACT_GELU>{});
+        else if (act == MDH_ACT_SILU) run(std::integral_constant<int, MDH_ACT_SILU>{});
+        else run(std::integral_constant<int, MDH_ACT_NONE>{});
     }
-    if (part) part[blockIdx.y * n + c] = sum;
+    if (!part) return;
+#pragma unroll
+    for (int j = 0; j < kChunk / 2; j++) *reinterpret_cast<float2*>(&sums[warp][lane * kChunk + 2 * j]) = unpair(sum[j]);
+    __syncthreads();
+    const int64_t at = (int64_t)blockIdx.y * 32 * kChunk + threadIdx.x;
+    if (at < n) {
+        float v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) v += sums[k][threadIdx.x];
+        part[blockIdx.x * n + at] = v;
+    }
 }
 
+// Column sums of part[blocks][n]: 32 columns of a block, its 32 warps each
+// take every 32nd partial row, joined in order.
 template <class T>
-__global__ void __launch_bounds__(256) k_join(const float* __restrict__ part, int64_t blocks, int64_t n,
-                                              T* __restrict__ out) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= n) return;
+__global__ void __launch_bounds__(1024) k_join(const float* __restrict__ part, int64_t blocks, int64_t n,
+                                               T* __restrict__ out) {
+    __shared__ float s[32][33];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     float v = 0.0f;
-    for (int64_t i = 0; i < blocks; i++) v += part[i * n + c];
+    if (c < n) {
+#pragma unroll 4
+        for (int64_t i = warp; i < blocks; i += 32) v += part[i * n + c];
+    }
+    s[warp][lane] = v;
+    __syncthreads();
+    if (warp != 0 || c >= n) return;
+    for (int k = 1; k < 32; k++) v += s[k][lane];
     out[c] = from_f32<T>(v);
 }
+
+// The forward pass of a few rows (a query, a token): bound by reading w once
+// and by latency.  A warp forms one output column for up to ROWS rows; x and w
+// are read 8 elements a lane.
+template <class T, int ROWS>
+__global__ void __launch_bounds__(128)
+    k_linear_rows(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ w, int64_t w_stride,
+                  const T* __restrict__ bias, const T* __restrict__ residual, int64_t residual_stride, int act, int rows,
+                  int inner, int outer, T* __restrict__ y, int64_t y_stride, T* __restrict__ z, bool vec_x, bool vec_w) {
+    const int lane = threadIdx.x & 31;
+    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int m0 = blockIdx.y * ROWS, mine = m0 + lane;
+    if (n >= outer) return;
+    const bool writes = lane < ROWS && mine < rows;
+    const float b = bias ? to_f32(bias[n]) : 0.0f;
+    const float res = residual && writes ? to_f32(residual[mine * residual_stride + n]) : 0.0f;
+    float acc[ROWS] = {};
+#pragma unroll 2
+    for (int k = lane * kChunk; k < inner; k += 32 * kChunk) {
+        float wv[kChunk];
+        load_chunk(w + n * w_stride + k, inner - k, vec_w, wv);
+#pragma unroll
+        for (int m = 0; m < ROWS; m++) {
+            if (m0 + m >= rows) break;
+            float xv[kChunk];
+            load_chunk(x + (m0 + m) * x_stride + k, inner - k, vec_x, xv);
+#pragma unroll
+            for (int j = 0; j < kChunk; j++) acc[m] = fmaf(xv[j], wv[j], acc[m]);
+        }
+    }
+    float v = 0.0f;
+#pragma unroll
+    for (int m = 0; m < ROWS; m++) {
+        const float s = warp_sum(acc[m]);
+        if (lane == m) v = s;
+    }
+    if (!writes) return;
+    v += b;
+    if (z) z[(int64_t)mine * outer + n] = from_f32<T>(v);
+    y[mine * y_stride + n] = from_f32<T>(activate(v, act) + res);
+}
+// Rows up to which the row form is taken (2,048 x 2,048 and smaller weights;
+// each 4 rows read w again, from the cache).
+constexpr int64_t kFewRows = 8;
 
 void check_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int32_t dtype, int32_t act,
                   int64_t rows, int32_t inner, int32_t outer) {
@@ -107,7 +179,7 @@ extern "C" {
 
 int64_t mdh_linear_forward_workspace(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t rows,
                                      int32_t inner, int32_t outer) {
-    return product_workspace({x, x_stride, true}, {w, w_stride, true}, rows, outer, inner);
+    return rows <= kFewRows ? 0 : product_workspace({x, x_stride, true}, {w, w_stride, true}, rows, outer, inner);
 }
 
 mdh_status mdh_linear_forward(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
@@ -121,6 +193,22 @@ mdh_status mdh_linear_forward(const void* x, int64_t x_stride, const void* w, in
         current_device();
         if (rows == 0) return;
         MDH_REQUIRE(y, MDH_ERR_INVALID_ARG, "linear: null output");
+        if (rows <= kFewRows) {
+            by_half(dtype, [&](auto zero) {
+                using T = decltype(zero);
+                auto run = [&](auto group) {
+                    const dim3 grid((unsigned)ceil_div(outer, 4), (unsigned)ceil_div(rows, group));
+                    k_linear_rows<T, group><<<grid, 128, 0, (cudaStream_t)stream>>>(
+                        (const T*)x, x_stride, (const T*)w, w_stride, (const T*)bias, (const T*)residual,
+                        residual_stride, activation, (int)rows, inner, outer, (T*)y, y_stride, (T*)z_out,
+                        rows_aligned(x, x_stride, 2), rows_aligned(w, w_stride, 2));
+                };
+                if (rows == 1) run(std::integral_constant<int, 1>{});
+                else run(std::integral_constant<int, 4>{});
+            });
+            check_launch();
+            return;
+        }
         check_product_status();
         MDH_REQUIRE(enough(ws, ws_bytes, mdh_linear_forward_workspace(x, x_stride, w, w_stride, rows, inner, outer)),
                     MDH_ERR_INVALID_ARG, "linear: workspace too small or not 16-byte aligned");
@@ -170,13 +258,14 @@ mdh_status mdh_linear_backward(const void* dy, int64_t dy_stride, const void* x,
             float* part = reinterpret_cast<float*>(base + lay.part);
             const int64_t blocks = ceil_div(rows, kSlopeRows);
             if (dz || db) {
-                const dim3 grid((unsigned)ceil_div(outer, 256), (unsigned)blocks);
+                const dim3 grid((unsigned)blocks, (unsigned)ceil_div(outer, 32 * kChunk));
                 k_slope<T><<<grid, 256, 0, st>>>((const T*)dy, dy_stride, (const T*)z, activation, rows, outer, dz,
-                                                 lay.dz_stride, db ? part : nullptr);
+                                                 lay.dz_stride, db ? part : nullptr, rows_aligned(dy, dy_stride, 2),
+                                                 rows_aligned(z, outer, 2));
                 check_launch();
             }
             if (db) {
-                k_join<T><<<(unsigned)ceil_div(outer, 256), 256, 0, st>>>(part, blocks, outer, (T*)db);
+                k_join<T><<<(unsigned)ceil_div(outer, 32), 1024, 0, st>>>(part, blocks, outer, (T*)db);
                 check_launch();
             }
             const void* g = dz ? dz : dy;

@@ -56,6 +56,40 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& r) {
     }
 }
 
+constexpr int kChunk = 8;  // elements of a thread
+// 8 elements from p, zeros past `left`; vec: one or two 16-byte loads.
+template <class T>
+__device__ __forceinline__ void load_chunk(const T* p, int left, bool vec, float (&v)[kChunk]) {
+    if (vec && left >= kChunk) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kChunk / N; i++) {
+            const Pack<T, N> x = load_pack<T, N>(p + i * N);
+#pragma unroll
+            for (int j = 0; j < N; j++) v[i * N + j] = to_f32(x.v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; j++) v[j] = j < left ? to_f32(p[j]) : 0.0f;
+    }
+}
+template <class T>
+__device__ __forceinline__ void store_chunk(T* p, int left, bool vec, const float (&v)[kChunk]) {
+    if (vec && left >= kChunk) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kChunk / N; i++) {
+            Pack<T, N> x;
+#pragma unroll
+            for (int j = 0; j < N; j++) x.v[j] = from_f32<T>(v[i * N + j]);
+            store_pack<T, N>(p + i * N, x);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; j++)
+            if (j < left) p[j] = from_f32<T>(v[j]);
+    }
+}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

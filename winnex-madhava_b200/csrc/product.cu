@@ -26,12 +26,11 @@ using namespace op;
 using namespace tc;
 
 constexpr int BM = 128, KB = 64;
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;
 constexpr int PRODUCER_WARP = EPI_WARPS, MMA_WARP = EPI_WARPS + 1;
 constexpr int NUM_THREADS = 32 * (EPI_WARPS + 2);
 constexpr uint32_t A_BYTES = BM * KB * 2;
-constexpr uint32_t STAGING = 32 * 64;      // a warp's 32 x 32 chunk of 16-bit values
-constexpr uint32_t WARP_SMEM = STAGING + 128;  // and 32 bias values
+constexpr uint32_t WARP_SMEM = 32 * 64;  // a warp's 32 x 32 chunk of 16-bit values
 
 template <int BN>
 struct Shape {
@@ -62,7 +61,7 @@ struct ProductParams {
     void* z;
     float* part;            // splits > 1: [splits][m][pitch]
     int64_t pitch;
-    bool y_vec, z_vec, r_vec;  // rows can be accessed 16 bytes at a time
+    bool y_vec, z_vec, r_vec, b_vec;  // rows can be accessed 16 bytes at a time
     int32_t* status;
 };
 
@@ -153,39 +152,51 @@ __device__ __forceinline__ void chunk_in(uint8_t* stage, const void* p, int64_t 
         *reinterpret_cast<uint4*>(stage + staged(r, piece)) = v;
     }
 }
-__device__ __forceinline__ void stage_row(uint8_t* stage, const float (&v)[32], bool f16, int lane) {
+__device__ __forceinline__ void stage_row(uint8_t* stage, const f32x2 (&v)[16], bool f16, int lane) {
 #pragma unroll
     for (int piece = 0; piece < 4; piece++) {
-        const float* e = v + piece * 8;
-        *reinterpret_cast<uint4*>(stage + staged(lane, piece)) = make_uint4(
-            pack2(e[0], e[1], f16), pack2(e[2], e[3], f16), pack2(e[4], e[5], f16), pack2(e[6], e[7], f16));
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = unpair(v[piece * 4 + j]);
+            w[j] = pack2(f.x, f.y, f16);
+        }
+        *reinterpret_cast<uint4*>(stage + staged(lane, piece)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
-__device__ __forceinline__ void activate32(float (&v)[32], int act) {
-    if (act == MDH_ACT_RELU) {
+template <int ACT>
+__device__ __forceinline__ void activate32(f32x2 (&v)[16]) {
 #pragma unroll
-        for (int j = 0; j < 32; j++) v[j] = activate(v[j], MDH_ACT_RELU);
-    } else if (act == MDH_ACT_GELU) {
+    for (int j = 0; j < 16; j++) v[j] = activate(v[j], ACT);
+}
+
+// Adds 8 16-bit values to four pairs.
+__device__ __forceinline__ void add8(f32x2* v, uint4 x, bool f16) {
+    const uint32_t e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int j = 0; j < 32; j++) v[j] = activate(v[j], MDH_ACT_GELU);
-    } else if (act == MDH_ACT_SILU) {
-#pragma unroll
-        for (int j = 0; j < 32; j++) v[j] = activate(v[j], MDH_ACT_SILU);
+    for (int j = 0; j < 4; j++) {
+        const float2 f = unpack2(e[j], f16);
+        v[j] = add2(v[j], pair(f.x, f.y));
     }
 }
 
 // One 32 x 32 chunk of sums, a row a lane: bias, z, activation, residual, y.
-__device__ __forceinline__ void finish_chunk(const ProductParams& p, float (&v)[32], int row0, int col0, uint8_t* stage,
+__device__ __forceinline__ void finish_chunk(const ProductParams& p, f32x2 (&v)[16], int row0, int col0, uint8_t* stage,
                                              int lane) {
-    float* sbias = reinterpret_cast<float*>(stage + STAGING);
     if (p.bias) {
-        sbias[lane] = col0 + lane < p.n ? half_at(p.bias, col0 + lane, p.f16) : 0.0f;
-        __syncwarp();
+        // The same 32 values for every lane.
+        const uint16_t* b = static_cast<const uint16_t*>(p.bias) + col0;
+        if (p.b_vec && col0 + 32 <= p.n) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float4 b = *reinterpret_cast<const float4*>(sbias + 4 * j);
-            v[4 * j] += b.x, v[4 * j + 1] += b.y, v[4 * j + 2] += b.z, v[4 * j + 3] += b.w;
+            for (int piece = 0; piece < 4; piece++) add8(v + 4 * piece, __ldg(reinterpret_cast<const uint4*>(b) + piece), p.f16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int c = col0 + 2 * j;
+                v[j] = add2(v[j], pair(c < p.n ? half_at(b, 2 * j, p.f16) : 0.0f,
+                                       c + 1 < p.n ? half_at(b, 2 * j + 1, p.f16) : 0.0f));
+            }
         }
     }
     if (p.z) {
@@ -194,21 +205,15 @@ __device__ __forceinline__ void finish_chunk(const ProductParams& p, float (&v)[
         chunk_out(stage, p.z, p.n, p.z_vec, row0, col0, p.m, p.n, lane);
         __syncwarp();
     }
-    activate32(v, p.act);
+    if (p.act == MDH_ACT_RELU) activate32<MDH_ACT_RELU>(v);
+    else if (p.act == MDH_ACT_GELU) activate32<MDH_ACT_GELU>(v);
+    else if (p.act == MDH_ACT_SILU) activate32<MDH_ACT_SILU>(v);
     if (p.residual) {
         chunk_in(stage, p.residual, p.residual_stride, p.r_vec, row0, col0, p.m, p.n, lane);
         __syncwarp();
 #pragma unroll
-        for (int piece = 0; piece < 4; piece++) {
-            const uint4 r = *reinterpret_cast<const uint4*>(stage + staged(lane, piece));
-            const uint32_t e[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float2 f = unpack2(e[j], p.f16);
-                v[piece * 8 + 2 * j] += f.x;
-                v[piece * 8 + 2 * j + 1] += f.y;
-            }
-        }
+        for (int piece = 0; piece < 4; piece++)
+            add8(v + 4 * piece, *reinterpret_cast<const uint4*>(stage + staged(lane, piece)), p.f16);
         __syncwarp();
     }
     stage_row(stage, v, p.f16, lane);
@@ -344,8 +349,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             }
         }
     } else {
-        const int quarter = warp & 3, half = warp >> 2;
-        constexpr int CHUNKS = BN / 64;  // chunks of 32 columns of this warp's half
+        const int quarter = warp & 3, part = warp >> 2;
+        // Chunks of 32 columns of this warp; a tile of 64 columns has none for the last 8 warps.
+        constexpr int CHUNKS = BN >= 128 ? BN / 128 : 1;
+        const bool works = part * 32 < BN;
         uint8_t* stage = smem + S::OFF_EPI + warp * WARP_SMEM;
         int acc = 0;
         uint32_t acc_phase = 0;
@@ -356,21 +363,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             const int row0 = t.m0 + quarter * 32;
 #pragma unroll 1
             for (int c = 0; c < CHUNKS; c++) {
-                const int off = half * (BN / 2) + c * 32;
+                const int off = (part * CHUNKS + c) * 32;
                 uint32_t raw[32];
                 __syncwarp();
-                tmem_ld32_issue(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN + off), raw);
-                tmem_ld_wait(raw);
+                if (works) {
+                    tmem_ld32_issue(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN + off), raw);
+                    tmem_ld_wait(raw);
+                }
                 if (c == CHUNKS - 1) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bars + 8 * (S::BAR_ACC_EMPTY + acc));
                 }
                 const int col0 = t.n0 + off;
-                if (row0 >= p.m || col0 >= p.n) continue;
-                float v[32];
-#pragma unroll
-                for (int j = 0; j < 32; j++) v[j] = __uint_as_float(raw[j]);
+                if (!works || row0 >= p.m || col0 >= p.n) continue;
                 if (p.part) {
                     if (row0 + lane < p.m) {
                         float* dst = p.part + ((int64_t)t.split * p.m + row0 + lane) * p.pitch + col0;
@@ -378,9 +384,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                         for (int j = 0; j < 8; j++)
                             if (col0 + 4 * j < p.n)  // the pitch is a multiple of 4
                                 *reinterpret_cast<float4*>(dst + 4 * j) =
-                                    make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                                    make_float4(__uint_as_float(raw[4 * j]), __uint_as_float(raw[4 * j + 1]),
+                                                __uint_as_float(raw[4 * j + 2]), __uint_as_float(raw[4 * j + 3]));
                     }
                 } else {
+                    f32x2 v[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] = pair(__uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1]));
                     finish_chunk(p, v, row0, col0, stage, lane);
                 }
             }
@@ -560,6 +570,7 @@ void product(const ProductOperand& a0, const ProductOperand& b0, int64_t m, int6
     p.y_vec = rows_aligned(ep.y, ep.y_stride, 2);
     p.z_vec = rows_aligned(ep.z, n, 2);
     p.r_vec = rows_aligned(ep.residual, ep.residual_stride, 2);
+    p.b_vec = aligned16(ep.bias);
     p.pitch = round_up(n, 4);
     p.part = p.splits > 1 ? reinterpret_cast<float*>(at) : nullptr;
     p.status = status_word();

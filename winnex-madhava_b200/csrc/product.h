@@ -35,14 +35,71 @@ void product(const ProductOperand& a, const ProductOperand& b, int64_t m, int64_
 // Throws MDH_ERR_TIMEOUT when an earlier product gave up one of its waits.
 void check_product_status();
 
-__device__ __forceinline__ float activate(float z, int act) {
-    switch (act) {
-        case MDH_ACT_RELU: return z < 0.0f ? 0.0f : z;  // NaN stays NaN
-        case MDH_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case MDH_ACT_SILU: return z / (1.0f + expf(-z));
-        default: return z;
-    }
+// 2^x and 1 / x by the hardware (relative errors about 2^-22 and 2^-23).
+__device__ __forceinline__ float fast_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
+__device__ __forceinline__ float fast_inverse(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ f32x2 both(float v) { return pair(v, v); }
+// e^x of both values.
+__device__ __forceinline__ f32x2 exp_of(f32x2 x) {
+    const float2 f = unpair(mul2(x, both(1.44269504088896341f)));
+    return pair(fast_exp2(f.x), fast_exp2(f.y));
+}
+// The normal distribution's Phi(z), with e = e^(-z^2 / 2), by the rational
+// approximation 7.1.26 of Abramowitz and Stegun for the error function
+// (|error| <= 1.5e-7): half the instructions of the library's erff, whose
+// last bits the 16-bit results do not show.
+__device__ __forceinline__ f32x2 normal_cdf(f32x2 z, f32x2 e) {
+    const float2 f = unpair(z);
+    const f32x2 x = pair(fabsf(f.x), fabsf(f.y));
+    const float2 d = unpair(fma2(x, both(0.3275911f * 0.70710678118654752f), both(1.0f)));
+    const f32x2 t = pair(fast_inverse(d.x), fast_inverse(d.y));
+    f32x2 p = fma2(both(1.061405429f), t, both(-1.453152027f));
+    p = fma2(p, t, both(1.421413741f));
+    p = fma2(p, t, both(-0.284496736f));
+    p = fma2(p, t, both(0.254829592f));
+    const float2 tail = unpair(mul2(mul2(p, t), mul2(e, both(0.5f))));  // of the side away from 0
+    return pair(f.x < 0.0f ? tail.x : 1.0f - tail.x, f.y < 0.0f ? tail.y : 1.0f - tail.y);
+}
+__device__ __forceinline__ f32x2 logistic(f32x2 z) {
+    const float2 d = unpair(add2(exp_of(mul2(z, both(-1.0f))), both(1.0f)));
+    return pair(fast_inverse(d.x), fast_inverse(d.y));
+}
+__device__ __forceinline__ f32x2 activate(f32x2 z, int act) {
+    if (act == MDH_ACT_RELU) {
+        const float2 f = unpair(z);
+        return pair(f.x < 0.0f ? 0.0f : f.x, f.y < 0.0f ? 0.0f : f.y);  // NaN stays NaN
+    }
+    if (act == MDH_ACT_GELU) return mul2(z, normal_cdf(z, exp_of(mul2(mul2(z, z), both(-0.5f)))));
+    if (act == MDH_ACT_SILU) {
+        // z logistic(z); where e^-z leaves the float range the factor is 0 and so is the value.
+        return mul2(z, logistic(z));
+    }
+    return z;
+}
+__device__ __forceinline__ f32x2 activation_slope(f32x2 z, int act) {
+    if (act == MDH_ACT_RELU) {
+        const float2 f = unpair(z);
+        return pair(f.x > 0.0f ? 1.0f : 0.0f, f.y > 0.0f ? 1.0f : 0.0f);
+    }
+    if (act == MDH_ACT_GELU) {
+        const f32x2 e = exp_of(mul2(mul2(z, z), both(-0.5f)));
+        return fma2(mul2(z, both(0.39894228040143268f)), e, normal_cdf(z, e));
+    }
+    if (act == MDH_ACT_SILU) {
+        const f32x2 g = logistic(z);  // g (1 + z (1 - g))
+        return fma2(mul2(g, z), add2(both(1.0f), mul2(g, both(-1.0f))), g);
+    }
+    return both(1.0f);
+}
+__device__ __forceinline__ float activate(float z, int act) { return unpair(activate(both(z), act)).x; }
 
 }  // namespace op
 }  // namespace mdh

@@ -13,7 +13,6 @@ namespace {
 using namespace op;
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 8;  // elements of a thread
 
 // A block is x threads along a row (a power of two) by y rows; no index of
 // an element needs a division.
@@ -23,39 +22,6 @@ dim3 row_block(int width) {
     return dim3(x, kThreads / x);
 }
 
-// 8 elements from p, zeros past `left`; vec: one or two 16-byte loads.
-template <class T>
-__device__ __forceinline__ void load_chunk(const T* p, int left, bool vec, float (&v)[kChunk]) {
-    if (vec && left >= kChunk) {
-        constexpr int N = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < kChunk / N; i++) {
-            const Pack<T, N> x = load_pack<T, N>(p + i * N);
-#pragma unroll
-            for (int j = 0; j < N; j++) v[i * N + j] = to_f32(x.v[j]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < kChunk; j++) v[j] = j < left ? to_f32(p[j]) : 0.0f;
-    }
-}
-template <class T>
-__device__ __forceinline__ void store_chunk(T* p, int left, bool vec, const float (&v)[kChunk]) {
-    if (vec && left >= kChunk) {
-        constexpr int N = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < kChunk / N; i++) {
-            Pack<T, N> x;
-#pragma unroll
-            for (int j = 0; j < N; j++) x.v[j] = from_f32<T>(v[i * N + j]);
-            store_pack<T, N>(p + i * N, x);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < kChunk; j++)
-            if (j < left) p[j] = from_f32<T>(v[j]);
-    }
-}
 __device__ __forceinline__ void store_codes(uint8_t* p, int left, bool vec, const uint32_t (&c)[kChunk]) {
     if (vec && left >= kChunk) {
         uint2 w;
