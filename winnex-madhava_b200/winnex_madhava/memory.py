@@ -36,56 +36,67 @@ def _require(ok, message):
 
 def _dtype(t, name):
     code = _DTYPES.get(t.dtype)
-    _require(code is not None, f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
     return code
 
 
-def _on(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
+def _device(t, name):
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return index
+
+
+def _on(index, t, name):
+    if t is not None and t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
 
 
 def _rows(t, name):
-    """``t`` as rows of its last dimension: a 2-D view (rows may be strided)."""
-    _require(t.is_cuda, f"{name} must be a CUDA tensor")
-    _require(t.dim() >= 1, f"{name} must have at least one dimension")
-    if t.dim() != 2:
-        try:
-            t = t.view(-1, t.shape[-1]) if t.shape[-1] else t.view(0, 0)
-        except RuntimeError:
-            raise ValueError(f"{name}: its leading dimensions cannot be viewed as rows of one stride") from None
-    _require(t.shape[1] <= 1 or t.stride(1) == 1, f"{name}: the last dimension must be contiguous")
-    _require(t.shape[0] <= 1 or t.stride(0) >= t.shape[1], f"{name}: rows must not overlap")
-    return t
+    """``(rows, width, stride, t)`` of ``t`` as rows of its last dimension
+    (2-D rows may be strided); ``t`` is a view of the argument."""
+    dims = t.dim()
+    if dims == 2:
+        rows, width = t.shape
+        stride, inner = t.stride()
+        if width > 1 and inner != 1:
+            raise ValueError(f"{name}: the last dimension must be contiguous")
+        if rows > 1 and stride < width:
+            raise ValueError(f"{name}: rows must not overlap")
+        return rows, width, stride, t
+    if dims == 0:
+        raise ValueError(f"{name} must have at least one dimension")
+    width = t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // width if width else 0, width, width, t
+    try:
+        return _rows(t.view(-1, width), name)
+    except RuntimeError:
+        raise ValueError(f"{name}: its leading dimensions cannot be viewed as rows of one stride") from None
 
 
 def _vector(t, size, name):
-    if t is not None:
-        _require(t.dim() == 1 and t.shape[0] == size and t.is_contiguous(),
-                 f"{name} must be a contiguous vector of {size}")
-    return t
+    if t.dim() != 1 or t.shape[0] != size or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of {size}")
 
 
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
-class _Call:
-    """The device of a call, made current, and torch's stream there."""
+# The handle of torch's current stream on a device, without building a Stream.
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-        self.device = device
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(index, fn, *args):
+    """fn(*args, stream) with device ``index`` current and torch's stream there."""
+    if index == torch.cuda.current_device():
+        fn(*args, _stream_of(index))
+    else:
+        with torch.cuda.device(index):
+            fn(*args, _stream_of(index))
 
 
 def _workspace(size, device):
@@ -93,31 +104,34 @@ def _workspace(size, device):
 
 
 # ------------------------------------------------------------------ layer norm
-def _norm_weights(x2, weight, bias):
-    width = x2.shape[1]
-    _vector(weight, width, "weight")
-    _vector(bias, width, "bias")
-    _on(x2.device, weight=weight, bias=bias)
-    kinds = {t.dtype for t in (weight, bias) if t is not None}
-    _require(len(kinds) <= 1, "weight and bias must have one type")
-    kind = kinds.pop() if kinds else x2.dtype
-    _require(kind in (torch.float32, x2.dtype), "weight and bias must be float32 or of x's type")
-    return kind
+def _norm_weights(index, width, kind, weight, bias):
+    """The type of the weights."""
+    of = kind
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _vector(t, width, name)
+            _on(index, t, name)
+            of = t.dtype
+            if of != kind and of != torch.float32:
+                raise ValueError("weight and bias must be float32 or of x's type")
+    if weight is not None and weight.dtype != of:
+        raise ValueError("weight and bias must have one type")
+    return of
 
 
 def _norm_forward(x, weight, bias, eps, keep):
-    x2 = _rows(x, "x")
-    code = _dtype(x2, "x")
-    rows, width = x2.shape
-    _require(width >= 1, "x must have a last dimension of at least 1")
-    kind = _norm_weights(x2, weight, bias)
+    index = _device(x, "x")
+    code = _dtype(x, "x")
+    rows, width, stride, x2 = _rows(x, "x")
+    if width < 1:
+        raise ValueError("x must have a last dimension of at least 1")
+    kind = _norm_weights(index, width, x.dtype, weight, bias)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     mean = rstd = None
     if keep:
         mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    with _Call(x.device) as stream:
-        _native._layer_norm_forward(x2.data_ptr(), x2.stride(0), code, _ptr(weight), _ptr(bias), _DTYPES[kind], rows,
-                                    width, eps, y.data_ptr(), width, _ptr(mean), _ptr(rstd), stream)
+    _call(index, _native._layer_norm_forward, x2.data_ptr(), stride, code, _ptr(weight), _ptr(bias), _DTYPES[kind],
+          rows, width, eps, y.data_ptr(), width, _ptr(mean), _ptr(rstd))
     return y, mean, rstd
 
 
@@ -132,25 +146,31 @@ def layer_norm_backward(dy, x, weight, mean, rstd, *, weight_dtype=None):
 
     dweight and dbias have the weight's type (``weight_dtype`` where there is
     no weight; default x's type)."""
-    x2, dy2 = _rows(x, "x"), _rows(dy, "dy")
-    code = _dtype(x2, "x")
-    _require(dy.shape == x.shape and dy.dtype == x.dtype, "dy must have x's shape and type")
-    rows, width = x2.shape
-    _require(width >= 1, "x must have a last dimension of at least 1")
-    kind = _norm_weights(x2, weight, None) if weight is not None else weight_dtype or x.dtype
-    _require(kind in (torch.float32, x.dtype), "weight_dtype must be float32 or x's type")
-    for name, t in (("mean", mean), ("rstd", rstd)):
+    index = _device(x, "x")
+    code = _dtype(x, "x")
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("dy must have x's shape and type")
+    rows, width, stride, x2 = _rows(x, "x")
+    _, _, dy_stride, dy2 = _rows(dy, "dy")
+    if width < 1:
+        raise ValueError("x must have a last dimension of at least 1")
+    if weight is not None:
+        kind = _norm_weights(index, width, x.dtype, weight, None)
+    else:
+        kind = weight_dtype or x.dtype
+        _require(kind in (torch.float32, x.dtype), "weight_dtype must be float32 or x's type")
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
         _vector(t, rows, name)
-        _require(t is not None and t.dtype == torch.float32, f"{name} must be float32")
-    _on(x.device, dy=dy, weight=weight, mean=mean, rstd=rstd)
+        _require(t.dtype == torch.float32, f"{name} must be float32")
+        _on(index, t, name)
+    _on(index, dy, "dy")
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dw, db = torch.empty((2, width), dtype=kind, device=x.device)
     size = _native._layer_norm_backward_workspace(rows, width)
     ws = _workspace(size, x.device)
-    with _Call(x.device) as stream:
-        _native._layer_norm_backward(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), code, _ptr(weight),
-                                     _DTYPES[kind], mean.data_ptr(), rstd.data_ptr(), rows, width, dx.data_ptr(),
-                                     width, dw.data_ptr(), db.data_ptr(), _ptr(ws), size, stream)
+    _call(index, _native._layer_norm_backward, dy2.data_ptr(), dy_stride, x2.data_ptr(), stride, code, _ptr(weight),
+          _DTYPES[kind], mean.data_ptr(), rstd.data_ptr(), rows, width, dx.data_ptr(), width, dw.data_ptr(),
+          db.data_ptr(), _ptr(ws), size)
     return dx, dw, db
 
 
@@ -172,7 +192,11 @@ class _LayerNorm(torch.autograd.Function):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def layer_norm(x, weight=None, bias=None, *, eps=1e-5):
@@ -194,41 +218,49 @@ def _activation(name):
 
 
 def _linear_operands(x, weight):
-    x2 = _rows(x, "x")
-    _require(x2.dtype in (torch.bfloat16, torch.float16), f"x must be bfloat16 or float16, not {x.dtype}")
-    _require(weight.dim() == 2 and weight.dtype == x.dtype, "weight must be a matrix of x's type")
-    w2 = _rows(weight, "weight")
-    _require(w2.shape[1] == x2.shape[1], f"weight has {w2.shape[1]} columns, x rows of {x2.shape[1]}")
-    _require(w2.shape[0] >= 1 and w2.shape[1] >= 1, "weight must not be empty")
-    _on(x.device, weight=weight)
-    return x2, w2
+    """(device, x's rows, weight's rows) as :func:`_rows` gives them."""
+    index = _device(x, "x")
+    kind = x.dtype
+    if kind != torch.bfloat16 and kind != torch.float16:
+        raise ValueError(f"x must be bfloat16 or float16, not {kind}")
+    if weight.dim() != 2 or weight.dtype != kind:
+        raise ValueError("weight must be a matrix of x's type")
+    xr, wr = _rows(x, "x"), _rows(weight, "weight")
+    if wr[1] != xr[1]:
+        raise ValueError(f"weight has {wr[1]} columns, x rows of {xr[1]}")
+    if wr[0] < 1 or wr[1] < 1:
+        raise ValueError("weight must not be empty")
+    _on(index, weight, "weight")
+    return index, xr, wr
 
 
 def linear_forward(x, weight, bias=None, *, activation=None, residual=None, keep_preactivation=False):
     """``(y, z)``: :func:`linear`, and with ``keep_preactivation`` the value
     before the activation, in x's type, that :func:`linear_backward` takes
     (None without an activation: its slope is 1)."""
-    x2, w2 = _linear_operands(x, weight)
+    index, (rows, inner, xs, x2), (outer, _, ws, w2) = _linear_operands(x, weight)
     act = _activation(activation)
-    (rows, inner), outer = x2.shape, w2.shape[0]
+    kind = x.dtype
     shape = x.shape[:-1] + (outer,)
-    r2 = None
+    res = res_stride = 0
     if bias is not None:
         _vector(bias, outer, "bias")
-        _require(bias.dtype == x.dtype, "bias must have x's type")
+        if bias.dtype != kind:
+            raise ValueError("bias must have x's type")
+        _on(index, bias, "bias")
     if residual is not None:
-        _require(residual.shape == shape and residual.dtype == x.dtype, "residual must have y's shape and x's type")
-        r2 = _rows(residual, "residual")
-    _on(x.device, bias=bias, residual=residual)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    z = torch.empty(shape, dtype=x.dtype, device=x.device) if keep_preactivation and act else None
-    size = _native._linear_forward_workspace(x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), rows, inner,
-                                             outer)
-    ws = _workspace(size, x.device)
-    with _Call(x.device) as stream:
-        _native._linear_forward(x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _ptr(bias), _ptr(r2),
-                                0 if r2 is None else r2.stride(0), _DTYPES[x.dtype], act, rows, inner, outer,
-                                y.data_ptr(), outer, _ptr(z), _ptr(ws), size, stream)
+        if residual.shape != shape or residual.dtype != kind:
+            raise ValueError("residual must have y's shape and x's type")
+        _on(index, residual, "residual")
+        _, _, res_stride, r2 = _rows(residual, "residual")
+        res = r2.data_ptr()
+    y = torch.empty(shape, dtype=kind, device=x.device)
+    z = torch.empty(shape, dtype=kind, device=x.device) if keep_preactivation and act else None
+    xp, wp = x2.data_ptr(), w2.data_ptr()
+    size = _native._linear_forward_workspace(xp, xs, wp, ws, rows, inner, outer)
+    space = _workspace(size, x.device)
+    _call(index, _native._linear_forward, xp, xs, wp, ws, _ptr(bias), res, res_stride, _DTYPES[kind], act, rows, inner,
+          outer, y.data_ptr(), outer, _ptr(z), _ptr(space), size)
     return y, z
 
 
@@ -237,26 +269,26 @@ def linear_backward(dy, x, weight, z=None, *, activation=None, need=(True, True,
 
     z: from :func:`linear_forward` (with an activation).  ``need`` says which
     of the three to form; the others are None.  The residual's gradient is dy."""
-    x2, w2 = _linear_operands(x, weight)
+    index, (rows, inner, xs, x2), (outer, _, ws, w2) = _linear_operands(x, weight)
     act = _activation(activation)
-    (rows, inner), outer = x2.shape, w2.shape[0]
+    kind = x.dtype
     shape = x.shape[:-1] + (outer,)
-    _require(dy.shape == shape and dy.dtype == x.dtype, "dy must have y's shape and x's type")
-    dy2 = _rows(dy, "dy")
+    if dy.shape != shape or dy.dtype != kind:
+        raise ValueError("dy must have y's shape and x's type")
+    _on(index, dy, "dy")
+    _, _, dys, dy2 = _rows(dy, "dy")
     if act:
-        _require(z is not None and z.shape == shape and z.dtype == x.dtype and z.is_contiguous(),
-                 "z must be what linear_forward kept: y's shape, x's type, contiguous")
-    _on(x.device, dy=dy, z=z)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    dw = torch.empty((outer, inner), dtype=x.dtype, device=x.device) if need[1] else None
-    db = torch.empty(outer, dtype=x.dtype, device=x.device) if need[2] else None
-    size = _native._linear_backward_workspace(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0),
-                                              w2.data_ptr(), w2.stride(0), act, rows, inner, outer)
-    ws = _workspace(size, x.device)
-    with _Call(x.device) as stream:
-        _native._linear_backward(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), w2.data_ptr(),
-                                 w2.stride(0), _ptr(z if act else None), _DTYPES[x.dtype], act, rows, inner, outer,
-                                 _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), size, stream)
+        if z is None or z.shape != shape or z.dtype != kind or not z.is_contiguous():
+            raise ValueError("z must be what linear_forward kept: y's shape, x's type, contiguous")
+        _on(index, z, "z")
+    dx = torch.empty(x.shape, dtype=kind, device=x.device) if need[0] else None
+    dw = torch.empty((outer, inner), dtype=kind, device=x.device) if need[1] else None
+    db = torch.empty(outer, dtype=kind, device=x.device) if need[2] else None
+    xp, wp, dp = x2.data_ptr(), w2.data_ptr(), dy2.data_ptr()
+    size = _native._linear_backward_workspace(dp, dys, xp, xs, wp, ws, act, rows, inner, outer)
+    space = _workspace(size, x.device)
+    _call(index, _native._linear_backward, dp, dys, xp, xs, wp, ws, _ptr(z if act else None), _DTYPES[kind], act, rows,
+          inner, outer, _ptr(dx), _ptr(dw), _ptr(db), _ptr(space), size)
     return dx, dw, db
 
 
@@ -300,25 +332,29 @@ class RowCache:
     """
 
     def __init__(self, codes, scales=None, *, group=0, lo=0.0, step=1.0):
-        _require(codes.is_cuda and codes.dim() == 2 and codes.dtype in (torch.int8, torch.uint8),
-                 "codes must be an int8 or uint8 CUDA matrix")
-        slots, width = codes.shape
-        _require(width >= 1 and (width == 1 or codes.stride(1) == 1) and (slots <= 1 or codes.stride(0) >= width),
-                 "codes must be rows of contiguous elements that do not overlap")
+        index = _device(codes, "codes")
         affine = codes.dtype == torch.uint8
+        if codes.dim() != 2 or not (affine or codes.dtype == torch.int8):
+            raise ValueError("codes must be an int8 or uint8 matrix")
+        slots, width = codes.shape
+        stride, inner = codes.stride()
+        if width < 1 or (width > 1 and inner != 1) or (slots > 1 and stride < width):
+            raise ValueError("codes must be rows of contiguous elements that do not overlap")
         if affine:
             _require(scales is None, "uint8 codes have no scales")
             _require(step > 0, "step must be positive")
+            group = 0
         else:
             _require(group >= 0 and group % 16 == 0, "group must be 0 or a multiple of 16")
-            groups = 1 if group == 0 else -(-width // group)
-            _require(scales is not None and scales.dtype == torch.float32 and scales.shape == (slots, groups) and
-                     scales.is_contiguous(), f"scales must be a contiguous float32 matrix of {slots} x {groups}")
-            _on(codes.device, scales=scales)
+            groups = -(-width // group) if group else 1
+            if scales is None or scales.dtype != torch.float32 or scales.shape != (slots, groups) or \
+                    not scales.is_contiguous():
+                raise ValueError(f"scales must be a contiguous float32 matrix of {slots} x {groups}")
+            _on(index, scales, "scales")
         self.codes, self.scales, self.group, self.lo, self.step = codes, scales, group, lo, step
-        self.slots, self.width, self.device = slots, width, codes.device
-        self._native = _native._Rows(codes.data_ptr(), _ptr(scales), slots, max(codes.stride(0), width), width,
-                                     0 if affine else group, int(affine), lo, step)
+        self.slots, self.width, self.index = slots, width, index
+        self._native = _native._Rows(codes.data_ptr(), _ptr(scales), slots, stride if stride > width else width, width,
+                                     group, affine, lo, step)
 
     @classmethod
     def empty(cls, slots, width, *, code="int8", group=64, lo=0.0, step=1.0, device="cuda"):
@@ -333,81 +369,95 @@ class RowCache:
         groups = 1 if group == 0 else -(-width // group)
         return cls(codes, torch.zeros((slots, groups), device=device), group=group)
 
-    def _ids(self, ids, name, dims=1):
-        _require(ids.dtype in (torch.int32, torch.int64) and ids.is_contiguous() and (not dims or ids.dim() == dims),
-                 f"{name} must be contiguous int32 or int64" + (" and one-dimensional" if dims else ""))
-        _on(self.device, **{name: ids})
-        return 32 if ids.dtype == torch.int32 else 64
+    def _ids(self, ids, name):
+        wide = ids.dtype == torch.int64
+        if not (wide or ids.dtype == torch.int32) or not ids.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int32 or int64")
+        _on(self.index, ids, name)
+        return 64 if wide else 32
 
     def write(self, slots, rows):
         """Quantises rows [n, width] (float32, bfloat16 or float16) into the
         given slots; a slot outside [0, slots) (-1, say) writes nothing.  The
         slots of one call that are inside must differ from one another."""
         bits = self._ids(slots, "slots")
-        _require(rows.dim() == 2 and rows.shape == (slots.shape[0], self.width),
-                 f"rows must be {slots.shape[0]} x {self.width}")
-        r2 = _rows(rows, "rows")
-        code = _dtype(r2, "rows")
-        _on(self.device, rows=rows)
-        with _Call(self.device) as stream:
-            _native._rows_write(self._native, slots.data_ptr(), bits, r2.data_ptr(), r2.stride(0), code,
-                                slots.shape[0], stream)
+        if slots.dim() != 1 or rows.dim() != 2 or rows.shape != (slots.shape[0], self.width):
+            raise ValueError(f"slots must be one-dimensional and rows must be {slots.shape[0]} x {self.width}")
+        code = _dtype(rows, "rows")
+        _on(self.index, rows, "rows")
+        n, _, stride, _ = _rows(rows, "rows")
+        _call(self.index, _native._rows_write, self._native, slots.data_ptr(), bits, rows.data_ptr(), stride, code, n)
 
     def read(self, ids, dtype=torch.float32):
         """The rows of ids [...] as [..., width] of ``dtype``: what the codes
         stand for, zeros where an id is outside [0, slots)."""
-        bits = self._ids(ids, "ids", 0)
-        _require(dtype in _DTYPES, f"dtype must be float32, bfloat16 or float16, not {dtype}")
-        out = torch.empty(ids.shape + (self.width,), dtype=dtype, device=self.device)
-        with _Call(self.device) as stream:
-            _native._rows_read(self._native, ids.data_ptr(), bits, ids.numel(), out.data_ptr(), self.width,
-                               _DTYPES[dtype], stream)
+        bits = self._ids(ids, "ids")
+        code = _DTYPES.get(dtype)
+        if code is None:
+            raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+        out = torch.empty(ids.shape + (self.width,), dtype=dtype, device=self.codes.device)
+        _call(self.index, _native._rows_read, self._native, ids.data_ptr(), bits, ids.numel(), out.data_ptr(),
+              self.width, code)
         return out
 
 
 # ------------------------------------------------------------------ attention over found rows
+def _list_stride(t, queries, found, name):
+    """The row stride of lists [queries, found]; 0 gives every query the same."""
+    stride, inner = t.stride()
+    if (found > 1 and inner != 1) or (queries > 1 and stride < found and stride != 0):
+        raise ValueError(f"{name} must be rows of contiguous entries")
+    return stride
+
+
 def _attend_args(q, ids, keys, values, scale, cap, bias, query_docs, row_docs):
-    _require(q.is_cuda and q.dim() == 3, "q must be a CUDA tensor [queries, heads, head]")
+    index = _device(q, "q")
     code = _dtype(q, "q")
+    if q.dim() != 3:
+        raise ValueError("q must be [queries, heads, head]")
     queries, heads, head = q.shape
-    _require(heads >= 1 and head >= 8 and head % 8 == 0 and head <= 256,
-             "q: the head size must be a multiple of 8 up to 256")
-    _require(q.stride(2) == 1, "q: the last dimension must be contiguous")
-    _require(keys.width == values.width and keys.slots == values.slots, "keys and values must have one shape")
-    _require(keys.width % head == 0 and heads % (keys.width // head) == 0,
-             f"cache rows of {keys.width} do not hold heads of {head} that {heads} query heads share")
-    _require(ids.dim() == 2 and ids.shape[0] == queries and ids.dtype == torch.int32,
-             "ids must be int32 [queries, found]")
+    q_stride, head_stride, inner = q.stride()
+    if heads < 1 or head < 8 or head % 8 or head > 256:
+        raise ValueError("q: the head size must be a multiple of 8 up to 256")
+    if inner != 1:
+        raise ValueError("q: the last dimension must be contiguous")
+    width, slots = keys.width, keys.slots
+    if values.width != width or values.slots != slots:
+        raise ValueError("keys and values must have one shape")
+    if width % head or heads % (width // head):
+        raise ValueError(f"cache rows of {width} do not hold heads of {head} that {heads} query heads share")
+    if keys.index != index or values.index != index:
+        raise ValueError(f"keys and values must be on cuda:{index}")
+    if ids.dim() != 2 or ids.shape[0] != queries or ids.dtype != torch.int32:
+        raise ValueError("ids must be int32 [queries, found]")
     found = ids.shape[1]
-
-    def lists(t):  # one list may serve every query (stride 0)
-        return (found <= 1 or t.stride(1) == 1) and (queries <= 1 or t.stride(0) >= found or t.stride(0) == 0)
-
-    _require(lists(ids), "ids must be rows of contiguous entries")
+    _on(index, ids, "ids")
+    ids_stride, bias_stride = _list_stride(ids, queries, found, "ids"), 0
     if bias is not None:
-        _require(bias.shape == ids.shape and bias.dtype == torch.float32 and lists(bias),
-                 "bias must be float32 of ids' shape, its rows contiguous")
-    _require((query_docs is None) == (row_docs is None), "query_docs and row_docs go together")
-    if query_docs is not None:
-        for name, t, n in (("query_docs", query_docs, queries), ("row_docs", row_docs, keys.slots)):
+        if bias.shape != ids.shape or bias.dtype != torch.float32:
+            raise ValueError("bias must be float32 of ids' shape")
+        bias_stride = _list_stride(bias, queries, found, "bias")
+        _on(index, bias, "bias")
+    if query_docs is not None or row_docs is not None:
+        _require(query_docs is not None and row_docs is not None, "query_docs and row_docs go together")
+        for t, name, n in ((query_docs, "query_docs", queries), (row_docs, "row_docs", slots)):
             _vector(t, n, name)
             _require(t.dtype == torch.int32, f"{name} must be int32")
-    _on(q.device, ids=ids, bias=bias, query_docs=query_docs, row_docs=row_docs, keys=keys, values=values)
-    _require(cap >= 0, "cap must be >= 0")
-    return _native._AttendArgs(q.data_ptr(), ids.data_ptr(), _ptr(bias), _ptr(query_docs), _ptr(row_docs),
-                               q.stride(0), q.stride(1), ids.stride(0), 0 if bias is None else bias.stride(0),
-                               queries, found, heads,
-                               heads * head // keys.width, head, code, head ** -0.5 if scale is None else scale, cap)
+            _on(index, t, name)
+    if not cap >= 0:
+        raise ValueError("cap must be >= 0")
+    return index, _native._AttendArgs(q.data_ptr(), ids.data_ptr(), _ptr(bias), _ptr(query_docs), _ptr(row_docs),
+                                      q_stride, head_stride, ids_stride, bias_stride, queries, found, heads,
+                                      heads * head // width, head, code, head ** -0.5 if scale is None else scale, cap)
 
 
 def _attend(q, ids, keys, values, scale, cap, bias, query_docs, row_docs):
-    args = _attend_args(q, ids, keys, values, scale, cap, bias, query_docs, row_docs)
+    index, args = _attend_args(q, ids, keys, values, scale, cap, bias, query_docs, row_docs)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     size = _native._attend_workspace(args)
     ws = _workspace(size, q.device)
-    with _Call(q.device) as stream:
-        _native._attend(args, keys._native, values._native, out.data_ptr(), lse.data_ptr(), _ptr(ws), size, stream)
+    _call(index, _native._attend, args, keys._native, values._native, out.data_ptr(), lse.data_ptr(), _ptr(ws), size)
     return out, lse
 
 
@@ -416,19 +466,19 @@ def attend_backward(dout, q, ids, keys, values, lse, *, scale=None, cap=0.0, bia
     """``(dq, dbias)`` of :func:`attend` from the gradient of its output and
     its lse; dbias (float32, summed over the heads) is None without a bias.
     The caches are constants."""
-    args = _attend_args(q, ids, keys, values, scale, cap, bias, query_docs, row_docs)
-    _require(dout.shape == q.shape and dout.dtype == q.dtype and dout.is_contiguous(),
-             "dout must be contiguous, of q's shape and type")
-    _require(lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous(),
-             "lse must be what attend returned")
-    _on(q.device, dout=dout, lse=lse)
+    index, args = _attend_args(q, ids, keys, values, scale, cap, bias, query_docs, row_docs)
+    if dout.shape != q.shape or dout.dtype != q.dtype or not dout.is_contiguous():
+        raise ValueError("dout must be contiguous, of q's shape and type")
+    if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError("lse must be what attend returned")
+    _on(index, dout, "dout")
+    _on(index, lse, "lse")
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dbias = None if bias is None else torch.empty(ids.shape, dtype=torch.float32, device=q.device)
     size = _native._attend_backward_workspace(args, dbias is not None)
     ws = _workspace(size, q.device)
-    with _Call(q.device) as stream:
-        _native._attend_backward(args, keys._native, values._native, dout.data_ptr(), lse.data_ptr(), dq.data_ptr(),
-                                 _ptr(dbias), _ptr(ws), size, stream)
+    _call(index, _native._attend_backward, args, keys._native, values._native, dout.data_ptr(), lse.data_ptr(),
+          dq.data_ptr(), _ptr(dbias), _ptr(ws), size)
     return dq, dbias
 
 
