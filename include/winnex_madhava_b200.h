@@ -431,7 +431,9 @@ mdh_status mdh_rows_read(const mdh_rows* cache, const void* ids, int32_t id_bits
  * in q's type; lse (float32 [queries][heads]) = log sum_j exp(s).  A query
  * with every entry hidden gives out = 0, lse = -infinity.  head: a multiple
  * of 8 up to 256; key and value caches have the same slots and width (and
- * may differ in code).  A list stride of 0 gives every query the same list. */
+ * may differ in code).  A list stride of 0 gives every query the same list.
+ * out and dq are contiguous and 16-byte aligned; the caches' row stride is
+ * below 2^31. */
 typedef struct {
     const void* q;          /* [queries][heads][head], strides below, `head` contiguous */
     const int32_t* ids;     /* [queries][found], ids_stride */

@@ -42,7 +42,8 @@ namespace {
 
 using namespace op;
 
-constexpr int kMaxWarps = 8;          // of a block
+constexpr int kMaxWarps = 8;          // of a block, forward
+constexpr int kMaxWarpsBack = 4;      // backward: its warps hold twice the vectors
 constexpr int kRound = 128;           // entries of the list that a warp looks at at a time
 constexpr int kMaxHead = 256;
 constexpr int kMaxShared = 4;         // query heads of a unit
@@ -51,7 +52,7 @@ constexpr int kMinSlice = 16;         // entries below which a list is not cut f
 struct CodeView {
     const uint8_t* codes;
     const float* scales;  // null: affine
-    int64_t stride;
+    uint32_t stride;
     int group, n_groups;
     uint32_t flip;        // 0x80808080 for int8: the stored byte becomes c + 128
     float scale, base;    // affine: value = base + scale c
@@ -414,13 +415,13 @@ __device__ __forceinline__ void finish_backward(const AttendParams& a, int64_t a
 struct Places {
     const uint8_t *k, *v;
     const float *ks, *vs;
-    int64_t k_stride, v_stride;
-    int kn, vn;
+    uint32_t k_stride, v_stride, kn, vn;
     float k_scale, v_scale;
 };
 __device__ __forceinline__ Places places_of(const AttendParams& a, const Work& w) {
     return {a.k.codes + w.e0, a.v.codes + w.e0, a.k.scales ? a.k.scales + w.e0 / a.k.group : nullptr,
-            a.v.scales ? a.v.scales + w.e0 / a.v.group : nullptr, a.k.stride, a.v.stride, a.k.n_groups, a.v.n_groups,
+            a.v.scales ? a.v.scales + w.e0 / a.v.group : nullptr, a.k.stride, a.v.stride, (uint32_t)a.k.n_groups,
+            (uint32_t)a.v.n_groups,
             a.k.scale, a.v.scale};
 }
 // A lane's place in a stage: codes of key and value (8 bytes), their scales.
@@ -464,7 +465,7 @@ __device__ __forceinline__ void fetch(Slot to, const Places& p, const int* slots
     for (int u = 0; u < STEPS; u++) {
         const int e = first + (u << entries_log);
         const bool some = e < hi && live;
-        const int64_t slot = some ? slots[e] : 0;
+        const uint64_t slot = some ? (uint32_t)slots[e] : 0u;  // 32 x 32 bits: rows may lie past 4 GB
         fetch_codes<ALIGNED>(to.codes(u, 0), p.k + slot * p.k_stride, some);
         fetch_codes<ALIGNED>(to.codes(u, 1), p.v + slot * p.v_stride, some);
         if (p.ks) copy_async<4>(to.scale(u, 0), p.ks + slot * p.kn, some);
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(128) k_attend_join(const __grid_constant__ Att
 // P is 1 up to rounding, except where lse cannot hold its own digits beside
 // scores of 1e9 and more (a mask of the type's lowest value throughout).
 template <int LANES, int RB, bool ALIGNED>
-__global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 2 : 1) k_attend_backward(const __grid_constant__ AttendParams a) {
+__global__ void __launch_bounds__(32 * kMaxWarpsBack, RB == 1 ? 3 : 2) k_attend_backward(const __grid_constant__ AttendParams a) {
     using St = Steps<LANES, RB>;
     using Sums = typename St::Sums;
     constexpr int STEPS = St::N, RP = St::RP, KEEP = Sums::KEEP;
@@ -851,7 +852,8 @@ CodeView code_view(const RowsView& r) {
     CodeView c{};
     c.codes = r.codes;
     c.scales = r.affine ? nullptr : r.scales;
-    c.stride = r.stride;
+    MDH_REQUIRE(r.stride <= INT32_MAX, MDH_ERR_UNSUPPORTED, "attend: the caches' row stride is limited to 2^31 - 1 bytes");
+    c.stride = (uint32_t)r.stride;
     c.group = r.group;
     c.n_groups = r.n_groups;
     c.flip = r.affine ? 0u : 0x80808080u;
@@ -873,7 +875,7 @@ int lanes_of(const AttendParams& p) {
 // units side by side, 58 us with two and twice the warps); then several warps
 // of a block share units' lists, and then blocks take ranges of a list, up to
 // kFill warps; no slice is below kMinSlice entries.
-void lay_out(AttendParams& p) {
+void lay_out(AttendParams& p, int max_warps) {
     constexpr int64_t kEnough = 148 * 8, kFill = 148 * 16;
     p.r_blocks = (int)ceil_div(p.shared, kMaxShared);
     p.rb = (int)ceil_div(p.shared, p.r_blocks);
@@ -883,17 +885,17 @@ void lay_out(AttendParams& p) {
     while (side > 1 && (side / 2 >= p.units || p.queries * ceil_div(p.units, side) < kEnough))
         side /= 2, p.entries_log++;
     const int64_t unit_warps = ceil_div(p.units, side);
-    p.unit_blocks = (int)ceil_div(unit_warps, kMaxWarps);
+    p.unit_blocks = (int)ceil_div(unit_warps, max_warps);
     p.block_warps = (int)ceil_div(unit_warps, p.unit_blocks);
     const int64_t warps = std::max<int64_t>(1, p.queries * p.unit_blocks * p.block_warps);
     p.slices = (int)std::max<int64_t>(
-        1, std::min({(int64_t)kMaxWarps / p.block_warps, ceil_div(p.found, kMinSlice), kFill / warps}));
+        1, std::min({(int64_t)max_warps / p.block_warps, ceil_div(p.found, kMinSlice), kFill / warps}));
     const int64_t splits = std::min(ceil_div(p.found, p.slices * kMinSlice), kFill / (warps * p.slices));
     p.split_len = (int)std::max<int64_t>(1, ceil_div(p.found, std::max<int64_t>(1, splits)));
     p.splits = (int)std::max<int64_t>(1, ceil_div(p.found, p.split_len));
 }
 
-AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values) {
+AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values, int max_warps) {
     MDH_REQUIRE(a, MDH_ERR_INVALID_ARG, "attend: null arguments");
     AttendParams p{};
     const RowsView k = rows_view(keys), v = rows_view(values);
@@ -941,13 +943,13 @@ AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const 
     p.scale = a->scale;
     p.cap = a->cap;
     p.inv_cap = a->cap > 0.0f ? 1.0f / a->cap : 0.0f;
-    lay_out(p);
+    lay_out(p, max_warps);
     MDH_REQUIRE(p.queries * p.unit_blocks <= INT32_MAX && p.queries * p.heads <= INT32_MAX, MDH_ERR_UNSUPPORTED, "attend: too many queries");
     return p;
 }
 
 // The layout of a call from its sizes alone, for the workspace.
-AttendParams layout_of(const mdh_attend_args* a, bool aligned) {
+AttendParams layout_of(const mdh_attend_args* a, bool aligned, int max_warps) {
     AttendParams p{};
     p.queries = a->queries;
     p.found = a->found;
@@ -955,7 +957,7 @@ AttendParams layout_of(const mdh_attend_args* a, bool aligned) {
     p.shared = a->shared;
     p.head = a->head;
     p.aligned = aligned;
-    lay_out(p);
+    lay_out(p, max_warps);
     return p;
 }
 bool has_sizes(const mdh_attend_args* a) {
@@ -1000,7 +1002,8 @@ void launch_form(const AttendParams& p, cudaStream_t st) {
     static std::atomic<uint64_t> set{0};  // a bit a device
     const int dev = current_device(), warps = p.block_warps * p.slices;
     if (!(set.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-        MDH_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxWarps * kWarpBytes));
+        MDH_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (BACKWARD ? kMaxWarpsBack : kMaxWarps) * kWarpBytes));
         set.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
     }
     kernel<<<attend_grid(p), 32 * warps, warps * kWarpBytes, st>>>(p);
@@ -1016,13 +1019,13 @@ extern "C" {
 
 int64_t mdh_attend_workspace(const mdh_attend_args* a) {
     if (!has_sizes(a)) return 0;
-    return std::max(forward_part(layout_of(a, true)), forward_part(layout_of(a, false)));
+    return std::max(forward_part(layout_of(a, true, kMaxWarps)), forward_part(layout_of(a, false, kMaxWarps)));
 }
 
 mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values, void* out, float* lse,
                       void* ws, int64_t ws_bytes, void* stream) {
     return guarded([&] {
-        AttendParams p = check_attend(a, keys, values);
+        AttendParams p = check_attend(a, keys, values, kMaxWarps);
         current_device();
         if (p.queries == 0) return;
         MDH_REQUIRE(out && lse && aligned16(out), MDH_ERR_INVALID_ARG, "attend: output null or not 16-byte aligned");
@@ -1045,7 +1048,7 @@ mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_
 
 int64_t mdh_attend_backward_workspace(const mdh_attend_args* a, int32_t want_dbias) {
     if (!has_sizes(a)) return 0;
-    int64_t need = std::max(backward_part(layout_of(a, true)), backward_part(layout_of(a, false)));
+    int64_t need = std::max(backward_part(layout_of(a, true, kMaxWarpsBack)), backward_part(layout_of(a, false, kMaxWarpsBack)));
     if (want_dbias) need += a->queries * a->heads * 8 + a->queries * a->heads * (int64_t)a->found * 8;
     return need;
 }
@@ -1054,7 +1057,7 @@ mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, c
                                const void* dout, const float* lse, void* dq, float* dbias, void* ws, int64_t ws_bytes,
                                void* stream) {
     return guarded([&] {
-        AttendParams p = check_attend(a, keys, values);
+        AttendParams p = check_attend(a, keys, values, kMaxWarpsBack);
         current_device();
         if (p.queries == 0) return;
         MDH_REQUIRE(dout && lse && dq && aligned16(dq), MDH_ERR_INVALID_ARG,

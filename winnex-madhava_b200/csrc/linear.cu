@@ -14,12 +14,28 @@ using namespace op;
 
 // dz [rows][n] = dy act'(z) (dz null: not stored), and part[block][n] = the
 // column sums of a block's rows.  A lane holds 8 columns, a warp every eighth
-// of the block's rows.  Bound by memory: three passes over [rows][n].
-constexpr int kSlopeRows = 64;
+// of the block's rows; the next three are on their way into the thread's own
+// shared memory.  Bound by memory: three passes over [rows][n].
+constexpr int kSlopeRows = 64, kSlopeStages = 4;
+// 8 16-bit elements as they lie in memory, zeros past `left`.
 template <class T>
-__global__ void __launch_bounds__(256)
+struct Chunk {
+    Pack<T, kChunk> raw;
+    __device__ __forceinline__ void load(const T* p, int left, bool vec) {
+        if (vec && left >= kChunk) {
+            raw = load_pack<T, kChunk>(p);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kChunk; j++) raw.v[j] = j < left ? p[j] : from_f32<T>(0.0f);
+        }
+    }
+    __device__ __forceinline__ f32x2 pair_at(int j) const { return pair(to_f32(raw.v[2 * j]), to_f32(raw.v[2 * j + 1])); }
+};
+template <class T>
+__global__ void __launch_bounds__(256, 4)
     k_slope(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ z, int act, int64_t rows, int64_t n,
             T* __restrict__ dz, int64_t dz_stride, float* __restrict__ part, bool vec_dy, bool vec_z) {
+    __shared__ Pack<T, kChunk> ring[kSlopeStages][2][256];
     __shared__ float sums[8][32 * kChunk];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t c = ((int64_t)blockIdx.y * 32 + lane) * kChunk;
@@ -28,21 +44,40 @@ __global__ void __launch_bounds__(256)
     f32x2 sum[kChunk / 2] = {};
     auto run = [&](auto known) {  // the activation as a compile-time value
         constexpr int ACT = decltype(known)::value;
-#pragma unroll 2
+        const bool whole = vec_dy && vec_z && left == kChunk;
+        auto fetch = [&](int stage, int64_t r) {
+            if (whole && r < r1) {
+                copy_async<16>(&ring[stage][0][threadIdx.x], dy + r * dy_stride + c);
+                if (ACT != MDH_ACT_NONE) copy_async<16>(&ring[stage][1][threadIdx.x], z + r * n + c);
+            }
+            copy_commit();
+        };
+        for (int k = 0; k < kSlopeStages - 1; k++) fetch(k, r0 + warp + 8 * k);
+        int stage = 0;
         for (int64_t r = r0 + warp; r < r1; r += 8) {
-            float v[kChunk], zz[kChunk];
-            load_chunk(dy + r * dy_stride + c, left, vec_dy, v);
-            if (ACT != MDH_ACT_NONE) load_chunk(z + r * n + c, left, vec_z, zz);
+            Chunk<T> dd, zz;
+            copy_wait<kSlopeStages - 2>();
+            if (whole) {
+                dd.raw = ring[stage][0][threadIdx.x];
+                if (ACT != MDH_ACT_NONE) zz.raw = ring[stage][1][threadIdx.x];
+            } else {
+                dd.load(dy + r * dy_stride + c, left, vec_dy);
+                if (ACT != MDH_ACT_NONE) zz.load(z + r * n + c, left, vec_z);
+            }
+            fetch((stage + kSlopeStages - 1) % kSlopeStages, r + 8 * (kSlopeStages - 1));
+            stage = (stage + 1) % kSlopeStages;
+            float v[kChunk];
 #pragma unroll
             for (int j = 0; j < kChunk / 2; j++) {
-                f32x2 d = pair(v[2 * j], v[2 * j + 1]);
-                if (ACT != MDH_ACT_NONE) d = mul2(d, activation_slope(pair(zz[2 * j], zz[2 * j + 1]), ACT));
+                f32x2 d = dd.pair_at(j);
+                if (ACT != MDH_ACT_NONE) d = mul2(d, activation_slope(zz.pair_at(j), ACT));
                 sum[j] = add2(sum[j], d);
                 const float2 f = unpair(d);
                 v[2 * j] = f.x, v[2 * j + 1] = f.y;
             }
             if (dz) store_chunk(dz + r * dz_stride + c, left, true, v);
         }
+        copy_wait<0>();
     };
     if (left > 0) {
         if (act == MDH_ACT_RELU) run(std::integral_constant<int, MDH_ACT_RELU>{});

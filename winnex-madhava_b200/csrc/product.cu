@@ -61,7 +61,8 @@ struct ProductParams {
     void* z;
     float* part;            // splits > 1: [splits][m][pitch]
     int64_t pitch;
-    bool y_vec, z_vec, r_vec, b_vec;  // rows can be accessed 16 bytes at a time
+    int y_width, z_width, r_width;  // bytes that every row starts on: 16, 8, 4 or 2
+    bool b_vec;                     // the bias starts on 16 bytes
     int32_t* status;
 };
 
@@ -110,8 +111,9 @@ __device__ __forceinline__ float half_at(const void* p, int64_t i, bool f16) {
 // Offset of 16-byte piece `piece` of row `row` in a warp's staging chunk.
 __device__ __forceinline__ uint32_t staged(int row, int piece) { return row * 64 + ((piece ^ (row >> 1)) & 3) * 16; }
 
-// Staging chunk -> 32 rows x 32 columns of p at (row0, col0), clipped to m x n.
-__device__ __forceinline__ void chunk_out(const uint8_t* stage, void* p, int64_t stride, bool vec, int row0, int col0,
+// Staging chunk -> 32 rows x 32 columns of p at (row0, col0), clipped to m x
+// n; rows start on `width` bytes (16, 8, 4 or 2).
+__device__ __forceinline__ void chunk_out(const uint8_t* stage, void* p, int64_t stride, int width, int row0, int col0,
                                           int m, int n, int lane) {
     uint16_t* out = static_cast<uint16_t*>(p);
 #pragma unroll
@@ -120,8 +122,15 @@ __device__ __forceinline__ void chunk_out(const uint8_t* stage, void* p, int64_t
         if (row0 + r >= m || col >= n) continue;
         uint16_t* dst = out + (int64_t)(row0 + r) * stride + col;
         const uint4 v = *reinterpret_cast<const uint4*>(stage + staged(r, piece));
-        if (vec && col + 8 <= n) {
+        if (width == 16 && col + 8 <= n) {
             *reinterpret_cast<uint4*>(dst) = v;
+        } else if (width == 8 && col + 8 <= n) {
+            reinterpret_cast<uint2*>(dst)[0] = make_uint2(v.x, v.y);
+            reinterpret_cast<uint2*>(dst)[1] = make_uint2(v.z, v.w);
+        } else if (width >= 4 && col + 8 <= n) {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) reinterpret_cast<uint32_t*>(dst)[j] = w[j];
         } else {
             const uint16_t* e = reinterpret_cast<const uint16_t*>(&v);
 #pragma unroll
@@ -131,7 +140,7 @@ __device__ __forceinline__ void chunk_out(const uint8_t* stage, void* p, int64_t
     }
 }
 // The reverse: zeros outside m x n.
-__device__ __forceinline__ void chunk_in(uint8_t* stage, const void* p, int64_t stride, bool vec, int row0, int col0,
+__device__ __forceinline__ void chunk_in(uint8_t* stage, const void* p, int64_t stride, int width, int row0, int col0,
                                          int m, int n, int lane) {
     const uint16_t* in = static_cast<const uint16_t*>(p);
 #pragma unroll
@@ -140,8 +149,11 @@ __device__ __forceinline__ void chunk_in(uint8_t* stage, const void* p, int64_t 
         uint4 v = make_uint4(0, 0, 0, 0);
         if (row0 + r < m && col < n) {
             const uint16_t* src = in + (int64_t)(row0 + r) * stride + col;
-            if (vec && col + 8 <= n) {
+            if (width == 16 && col + 8 <= n) {
                 v = __ldg(reinterpret_cast<const uint4*>(src));
+            } else if (width == 8 && col + 8 <= n) {
+                const uint2 a = __ldg(reinterpret_cast<const uint2*>(src)), b = __ldg(reinterpret_cast<const uint2*>(src) + 1);
+                v = make_uint4(a.x, a.y, b.x, b.y);
             } else {
                 uint16_t e[8];
 #pragma unroll
@@ -202,14 +214,14 @@ __device__ __forceinline__ void finish_chunk(const ProductParams& p, f32x2 (&v)[
     if (p.z) {
         stage_row(stage, v, p.f16, lane);
         __syncwarp();
-        chunk_out(stage, p.z, p.n, p.z_vec, row0, col0, p.m, p.n, lane);
+        chunk_out(stage, p.z, p.n, p.z_width, row0, col0, p.m, p.n, lane);
         __syncwarp();
     }
     if (p.act == MDH_ACT_RELU) activate32<MDH_ACT_RELU>(v);
     else if (p.act == MDH_ACT_GELU) activate32<MDH_ACT_GELU>(v);
     else if (p.act == MDH_ACT_SILU) activate32<MDH_ACT_SILU>(v);
     if (p.residual) {
-        chunk_in(stage, p.residual, p.residual_stride, p.r_vec, row0, col0, p.m, p.n, lane);
+        chunk_in(stage, p.residual, p.residual_stride, p.r_width, row0, col0, p.m, p.n, lane);
         __syncwarp();
 #pragma unroll
         for (int piece = 0; piece < 4; piece++)
@@ -218,7 +230,7 @@ __device__ __forceinline__ void finish_chunk(const ProductParams& p, f32x2 (&v)[
     }
     stage_row(stage, v, p.f16, lane);
     __syncwarp();
-    chunk_out(stage, p.y, p.y_stride, p.y_vec, row0, col0, p.m, p.n, lane);
+    chunk_out(stage, p.y, p.y_stride, p.y_width, row0, col0, p.m, p.n, lane);
     __syncwarp();
 }
 
@@ -487,6 +499,12 @@ Plan plan_product(int64_t m, int64_t n, int64_t nkb) {
     return best;
 }
 
+// The bytes, 16 at most, that every row of 16-bit elements starts on.
+int row_width(const void* p, int64_t stride) {
+    const uint64_t bits = reinterpret_cast<uintptr_t>(p) | (uint64_t)stride * 2 | 16;
+    return (int)(bits & (~bits + 1));
+}
+
 // Whether TMA reads the operand in place.
 bool readable(const ProductOperand& o) { return rows_aligned(o.p, o.stride, 2); }
 int64_t lines(const ProductOperand& o, int64_t rows, int64_t k) { return o.k_major ? rows : k; }
@@ -567,9 +585,9 @@ void product(const ProductOperand& a0, const ProductOperand& b0, int64_t m, int6
     p.y = ep.y;
     p.y_stride = ep.y_stride;
     p.z = ep.z;
-    p.y_vec = rows_aligned(ep.y, ep.y_stride, 2);
-    p.z_vec = rows_aligned(ep.z, n, 2);
-    p.r_vec = rows_aligned(ep.residual, ep.residual_stride, 2);
+    p.y_width = row_width(ep.y, ep.y_stride);
+    p.z_width = row_width(ep.z, n);
+    p.r_width = row_width(ep.residual, ep.residual_stride);
     p.b_vec = aligned16(ep.bias);
     p.pitch = round_up(n, 4);
     p.part = p.splits > 1 ? reinterpret_cast<float*>(at) : nullptr;
