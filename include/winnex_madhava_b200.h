@@ -393,8 +393,8 @@ mdh_status mdh_linear_backward(const void* dy, int64_t dy_stride, const void* x,
  *   code 0, int8: `group` (a positive multiple of 16, or 0 for the whole row)
  *   elements share one float32 scale, scales [slots][ceil(width / group)];
  *   an element reads back as code * scale.  Writing takes the group's
- *   largest magnitude a: scale = a / 127, code = round(x * (127 / a)), each
- *   rounded to float32, halves to even.  a < 2^-100 stores zeros; a group
+ *   largest magnitude a: scale = a * (1 / 127), code = round(x * (127 * (1 /
+ *   a))), each operation rounded to float32, halves to even.  a < 2^-100 stores zeros; a group
  *   with an infinity or NaN reads back as NaN throughout.
  *   code 1, uint8: one affine map for the cache: code = round((x - lo) *
  *   (1 / step)) limited to [0, 255] (NaN to 0), read back as lo + step *

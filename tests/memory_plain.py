@@ -133,10 +133,10 @@ def quantise(x, group):
         part = x[:, g * group:(g + 1) * group]
         top = part.abs().amax(1)  # NaN where one is
         some = torch.isfinite(top) & (top >= 2.0 ** -100)
-        inv = torch.where(some, (127 / top.double()).float(), 0.0)
+        inv = torch.where(some, (1 / top.double()).float() * 127, 0.0)
         code = (part * inv[:, None]).round()
         codes[:, g * group:(g + 1) * group] = torch.where(some[:, None], code, 0.0).to(torch.int8)
-        scales[:, g] = torch.where(some, (top.double() / 127).float(), torch.where(torch.isfinite(top), 0.0, top))
+        scales[:, g] = torch.where(some, top * torch.tensor(1 / 127), torch.where(torch.isfinite(top), 0.0, top))
     return codes, scales
 
 

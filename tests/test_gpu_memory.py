@@ -552,3 +552,16 @@ def test_attend_lowest_value_everywhere_weighs_alike():
     want = head ** -0.5 * torch.einsum("qhk,qkd->qhd", ds, k)
     assert_close(dq, want, room * head ** -0.5 * k.abs().mean(1)[:, None], "dq")
     assert_close(dbias, ds.sum(1), (room / found).sum(1).expand(2, found), "dbias")
+
+
+def test_example_runs_them_together():
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "memory.py")
+    spec = importlib.util.spec_from_file_location("memory_example", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, hit = example.run(stored=3_000, queries=32, steps=6)
+    assert hit == 1.0                     # the asked state is nearest by far (noise 0.1 of its size)
+    assert all(math.isfinite(x) for x in losses) and losses[-1] < losses[0]

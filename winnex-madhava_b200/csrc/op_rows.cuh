@@ -35,8 +35,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // reads back as NaN.
 __device__ __forceinline__ void group_scale(float a, float& scale, float& inv) {
     const bool finite = a < INFINITY, some = a >= 0x1p-100f;
-    scale = !finite ? a : some ? __fdiv_rn(a, 127.0f) : 0.0f;
-    inv = finite && some ? __fdiv_rn(127.0f, a) : 0.0f;
+    scale = !finite ? a : some ? __fmul_rn(a, 1.0f / 127.0f) : 0.0f;
+    inv = finite && some ? __fmul_rn(127.0f, __frcp_rn(a)) : 0.0f;
 }
 // In a group without a finite inverse x may be infinite or NaN: 0 * x is then
 // NaN, which converts to 0.

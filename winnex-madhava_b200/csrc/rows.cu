@@ -1,10 +1,10 @@
 // A cache of 8-bit rows: quantised as they are written, read back by id.
 //
 // int8: a group of elements with largest magnitude a is stored as code =
-// round(x (127 / a)) with the scale a / 127; uint8: code = round((x - lo)
-// (1 / step)) limited to [0, 255].  Quotients, products and differences are
-// each rounded to float32 (no fused multiply-add), so a row's codes are the
-// same wherever they are computed.  Both directions are bound by memory.
+// round(x (127 (1 / a))) with the scale a (1 / 127); uint8: code = round((x -
+// lo) (1 / step)) limited to [0, 255].  Inverses, products and differences
+// are each rounded to float32 (no fused multiply-add), so a row's codes are
+// the same wherever they are computed.  Both directions are bound by memory.
 #include "op_rows.cuh"
 
 namespace mdh {
