@@ -565,3 +565,22 @@ def test_example_runs_them_together():
     losses, hit = example.run(stored=3_000, queries=32, steps=6)
     assert hit == 1.0                     # the asked state is nearest by far (noise 0.1 of its size)
     assert all(math.isfinite(x) for x in losses) and losses[-1] < losses[0]
+
+
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("width", [1, 2, 3, 31, 255, 301, 769, 1030, 2047])
+def test_layer_norm_rows_that_start_inside_words(kind, width):
+    """Contiguous 16-bit rows of odd and even widths, more of them than a launch has warps; the arrays around the
+    outputs stay as they are."""
+    rows = 5001
+    check_norm(rand(1, rows, width, kind=kind), rand(2, width, scale=0.2, shift=1.0), rand(3, width), 1e-5,
+               rand(4, rows, width, kind=kind))
+
+
+@pytest.mark.parametrize("kind", [BF16, F16])
+def test_layer_norm_mixed_strides(kind):
+    """Rows of odd and even strides together, and bases off a word."""
+    x, dy = rand(1, 33, 102, kind=kind)[:, :101], rand(2, 33, 101, kind=kind)
+    check_norm(x, None, None, 1e-5, dy)
+    check_norm(dy, rand(3, 101, kind=kind), None, 1e-5, x.contiguous())
+    check_norm(rand(4, 33, 102, kind=kind)[:, 1:], None, None, 1e-5, rand(5, 33, 104, kind=kind)[:, 2:103])

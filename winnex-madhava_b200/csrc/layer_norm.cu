@@ -9,13 +9,18 @@
 //
 // Blocks stay and take rows in turn, so the weights are read once a block.
 // What bounds them is the latency of memory: each thread copies its share of
-// the next rows, three where they fit (16-byte vectors where base, stride and width allow,
-// else one by one) into its own places of a ring in shared memory.
+// the next rows, three where they fit, into its own places of a ring in shared
+// memory.  Its vectors are of 16 bytes where base, stride and width allow;
+// 16-bit rows of any other width go by 4 bytes: such a row may start in the
+// middle of a word, and then its pairs begin one element earlier (`shift`).
+// Rows an even distance apart start alike, so a warp has one shift.
 // A row belongs to one warp up to 1024 elements (its sums are shuffles), to a
 // group of warps beyond, 16 elements a thread; weights, and backward the
 // running sums of a thread's columns, stay in registers.
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
+#include <utility>
 
 #include "op_common.cuh"
 
@@ -44,59 +49,52 @@ __device__ __forceinline__ float2 row_sums(float2 v, float2* red, int warp, int 
     return v;
 }
 
-// Weights are float32 or of the rows' type.
-template <class T, int V>
-__device__ __forceinline__ void load_weights(const void* w, bool w_f32, int c, float (&out)[V]) {
-    if (w_f32) {
-        const float* p = static_cast<const float*>(w) + c;
-        if constexpr (V >= 4) {
-#pragma unroll
-            for (int i = 0; i < V / 4; i++) {
-                const Pack<float, 4> r = load_pack<float, 4>(p + 4 * i);
-#pragma unroll
-                for (int j = 0; j < 4; j++) out[4 * i + j] = r.v[j];
-            }
-        } else {
-            out[0] = p[0];
-        }
-    } else {
-        const Pack<T, V> r = load_pack<T, V>(static_cast<const T*>(w) + c);
-#pragma unroll
-        for (int j = 0; j < V; j++) out[j] = to_f32(r.v[j]);
-    }
+// Weight c, float32 or of the rows' type.
+template <class T>
+__device__ __forceinline__ float weight_at(const void* w, bool w_f32, int c) {
+    return w_f32 ? static_cast<const float*>(w)[c] : to_f32(static_cast<const T*>(w)[c]);
 }
 
 // A thread's places for its shares of the next rows: elements (i * nt + t) * V
-// + 0 .. V - 1 of a row.  Those past the width are 0 and stay so.
-// A ring has four stages, fewer where a block's rows are too large for them.
+// - shift + 0 .. V - 1 of a row.  Those outside the row are 0.
+// A ring has four stages, fewer where a block's rows are too large for them:
+// three small blocks share an SM, larger ones have it for themselves.
 constexpr int stages_of(int threads, int bytes) {
-    return threads * bytes * 4 <= 144 * 1024 ? 4 : threads * bytes * 2 <= 144 * 1024 ? 2 : 1;
+    const int most = (threads <= 256 ? 72 : 144) * 1024;
+    return threads * bytes * 4 <= most ? 4 : threads * bytes * 2 <= most ? 2 : 1;
 }
-template <class T, int V, int NV, int STAGES>
+// Blocks of `smem` bytes that an SM holds.
+constexpr int blocks_that_fit(int smem) { return std::max(1, 227 * 1024 / (smem + 1024)); }
+template <class T, int V, int NV, int STAGES, int THREADS>
 struct Ring {
-    Pack<T, V>* at;  // of this thread: place i of stage s at [(s * NV + i) * threads]
-    __device__ __forceinline__ Ring(void* smem, int t, int nt, int width) : at(static_cast<Pack<T, V>*>(smem) + threadIdx.x) {
+    Pack<T, V>* at;  // of this thread: place i of stage s at [(s * NV + i) * THREADS]
+    int t, nt, width, shift;
+    __device__ __forceinline__ Ring(void* smem, int t, int nt, int width, int shift)
+        : at(static_cast<Pack<T, V>*>(smem) + threadIdx.x), t(t), nt(nt), width(width), shift(shift) {
         Pack<T, V> zero;
 #pragma unroll
         for (int j = 0; j < V; j++) zero.v[j] = from_f32<T>(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; i++)
-            if ((i * nt + t) * V >= width)
-                for (int s = 0; s < STAGES; s++) at[(s * NV + i) * blockDim.x] = zero;
+            if ((i * nt + t) * V - shift >= width)
+                for (int s = 0; s < STAGES; s++) at[(s * NV + i) * THREADS] = zero;
     }
-    __device__ __forceinline__ void fetch(int stage, const T* row, int t, int nt, int width) {
+    __device__ __forceinline__ void fetch(int stage, const T* row) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int c = (i * nt + t) * V;
-            Pack<T, V>* to = at + (stage * NV + i) * blockDim.x;
+            const int c = (i * nt + t) * V - shift;
+            Pack<T, V>* to = at + (stage * NV + i) * THREADS;
             if (c >= width) continue;
-            if constexpr (V * sizeof(T) >= 4) copy_async<V * sizeof(T)>(to, row + c);
+            // A last word may hold one element of the row: the copy fills the other with zero.
+            if constexpr (V == 2 && sizeof(T) == 2) copy_async_part<4>(to, row + c, c + 1 < width ? 4 : 2);
+            else if constexpr (V * sizeof(T) >= 4) copy_async<V * sizeof(T)>(to, row + c);
             else *to = load_pack<T, V>(row + c);
         }
     }
     __device__ __forceinline__ void take(int stage, Pack<T, V> (&raw)[NV]) const {
 #pragma unroll
-        for (int i = 0; i < NV; i++) raw[i] = at[(stage * NV + i) * blockDim.x];
+        for (int i = 0; i < NV; i++) raw[i] = at[(stage * NV + i) * THREADS];
+        if (V == 2 && shift && t == 0) raw[0].v[0] = from_f32<T>(0.0f);  // the element before the row
     }
 };
 
@@ -105,39 +103,65 @@ template <class T, int V, int NV>
 __device__ __forceinline__ f32x2 pair_of(const Pack<T, V> (&raw)[NV], int p) {
     return pair(to_f32(raw[2 * p / V].v[2 * p % V]), to_f32(raw[(2 * p + 1) / V].v[(2 * p + 1) % V]));
 }
-// Pairs -> the share's vectors in memory (those inside the width).
+// Pairs -> the share's vectors in memory (what of them lies in the row).
 template <class T, int V, int NV>
-__device__ __forceinline__ void store_row(T* row, const f32x2 (&v)[NV * V / 2], int t, int nt, int width) {
+__device__ __forceinline__ void store_row(T* row, const f32x2 (&v)[NV * V / 2], int t, int nt, int width, int shift) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        const int c = (i * nt + t) * V;
+        const int c = (i * nt + t) * V - shift;
         Pack<T, V> p;
 #pragma unroll
         for (int j = 0; j < V; j++) {
             const float2 f = unpair(v[(i * V + j) / 2]);
             p.v[j] = from_f32<T>((i * V + j) % 2 ? f.y : f.x);
         }
-        if (c < width) store_pack<T, V>(row + c, p);
+        if constexpr (V == 2) {
+            if (c >= 0 && c + 1 < width) *reinterpret_cast<Pack<T, 2>*>(row + c) = p;
+            else if (c >= 0 && c < width) row[c] = p.v[0];
+            else if (c == -1) row[0] = p.v[1];
+        } else {
+            if (c < width) store_pack<T, V>(row + c, p);
+        }
     }
 }
 
 // A thread's weights, `fallback` where there are none.
 template <class T, int V, int NV>
-__device__ __forceinline__ void load_share(const void* w, bool w_f32, float fallback, int t, int nt, int width,
+__device__ __forceinline__ void load_share(const void* w, bool w_f32, float fallback, int t, int nt, int width, int shift,
                                            f32x2 (&out)[NV * V / 2]) {
     float f[NV * V];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        const int c = (i * nt + t) * V;
-        float v[V];
+        const int c0 = (i * nt + t) * V - shift;
+        if (V >= 4 && w && c0 < width) {  // whole vectors
+            if (w_f32) {
 #pragma unroll
-        for (int j = 0; j < V; j++) v[j] = fallback;
-        if (w && c < width) load_weights<T, V>(w, w_f32, c, v);
+                for (int j = 0; j < V / 4; j++) {
+                    const Pack<float, 4> r = load_pack<float, 4>(static_cast<const float*>(w) + c0 + 4 * j);
 #pragma unroll
-        for (int j = 0; j < V; j++) f[i * V + j] = v[j];
+                    for (int k = 0; k < 4; k++) f[i * V + 4 * j + k] = r.v[k];
+                }
+            } else {
+                const Pack<T, V> r = load_pack<T, V>(static_cast<const T*>(w) + c0);
+#pragma unroll
+                for (int j = 0; j < V; j++) f[i * V + j] = to_f32(r.v[j]);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const int c = c0 + j;
+            f[i * V + j] = w && c >= 0 && c < width ? weight_at<T>(w, w_f32, c) : fallback;
+        }
     }
 #pragma unroll
     for (int p = 0; p < NV * V / 2; p++) out[p] = pair(f[2 * p], f[2 * p + 1]);
+}
+
+// Where this thread's rows start in a word of two elements.
+template <class T, int V>
+__device__ __forceinline__ int shift_of(int64_t row, int64_t stride) {
+    return V == 2 && sizeof(T) == 2 ? (int)((row * stride) & 1) : 0;
 }
 
 template <class T, int V, int ELEMS, bool WIDE, int THREADS>
@@ -151,16 +175,17 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
     const int t = WIDE ? threadIdx.x : threadIdx.x & 31, nt = WIDE ? blockDim.x : 32;
     int64_t row = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWarpsPerBlock + (threadIdx.x >> 5);
     const int64_t step = WIDE ? gridDim.x : (int64_t)gridDim.x * kWarpsPerBlock;
-    Ring<T, V, NV, STAGES> ring(smem4, t, nt, width);
+    const int shift = shift_of<T, V>(row, x_stride);
+    Ring<T, V, NV, STAGES, THREADS> ring(smem4, t, nt, width, shift);
     for (int k = 0; k < STAGES - 1; k++) {
-        if (row + k * step < rows) ring.fetch(k, x + (row + k * step) * x_stride, t, nt, width);
+        if (row + k * step < rows) ring.fetch(k, x + (row + k * step) * x_stride);
         copy_commit();
     }
     f32x2 fw[PAIRS], fb[PAIRS];
-    load_share<T, V, NV>(w, w_f32, 1.0f, t, nt, width, fw);
-    load_share<T, V, NV>(b, w_f32, 0.0f, t, nt, width, fb);
+    load_share<T, V, NV>(w, w_f32, 1.0f, t, nt, width, shift, fw);
+    load_share<T, V, NV>(b, w_f32, 0.0f, t, nt, width, shift, fb);
     for (int stage = 0; row < rows; row += step, stage = (stage + 1) % STAGES) {
-        if (STAGES == 1) ring.fetch(0, x + row * x_stride, t, nt, width), copy_commit();
+        if (STAGES == 1) ring.fetch(0, x + row * x_stride), copy_commit();
         copy_wait<STAGES == 1 ? 0 : STAGES - 2>();
         Pack<T, V> raw[NV];
         ring.take(stage, raw);
@@ -168,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
 #pragma unroll
         for (int p = 0; p < PAIRS; p++) v[p] = pair_of<T, V, NV>(raw, p);
         const int64_t ahead = row + (STAGES - 1) * step;
-        if (STAGES > 1 && ahead < rows) ring.fetch((stage + STAGES - 1) % STAGES, x + ahead * x_stride, t, nt, width);
+        if (STAGES > 1 && ahead < rows) ring.fetch((stage + STAGES - 1) % STAGES, x + ahead * x_stride);
         copy_commit();
         f32x2 sum = 0;
 #pragma unroll
@@ -181,11 +206,13 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
 #pragma unroll
         for (int p = 0; p < PAIRS; p++) {
             v[p] = add2(v[p], away);
-            // Elements past the width deviate by 0.  A warp's share is full up to its last 8 elements.
-            if (WIDE || 2 * p >= ELEMS - 8) {
+            // Elements outside the row deviate by 0.  A warp's share is full up to its last 8 elements,
+            // but for the element before a shifted row.
+            if (WIDE || V == 2 || 2 * p >= ELEMS - 8) {
                 const float2 f = unpair(v[p]);
-                v[p] = pair((2 * p / V * nt + t) * V < width ? f.x : 0.0f,
-                            ((2 * p + 1) / V * nt + t) * V < width ? f.y : 0.0f);
+                const int c0 = (2 * p / V * nt + t) * V + 2 * p % V - shift;
+                const int c1 = ((2 * p + 1) / V * nt + t) * V + (2 * p + 1) % V - shift;
+                v[p] = pair(c0 >= 0 && c0 < width ? f.x : 0.0f, c1 < width ? f.y : 0.0f);
             }
             sq = fma2(v[p], v[p], sq);
         }
@@ -200,7 +227,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
         const f32x2 rr = pair(rstd, rstd);
 #pragma unroll
         for (int p = 0; p < PAIRS; p++) v[p] = fma2(mul2(v[p], rr), fw[p], fb[p]);
-        store_row<T, V, NV>(y + row * y_stride, v, t, nt, width);
+        store_row<T, V, NV>(y + row * y_stride, v, t, nt, width, shift);
     }
 }
 
@@ -221,13 +248,15 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 3 : 1)
     const int64_t step = (int64_t)gridDim.x * groups;
     constexpr int kRing = STAGES * ELEMS * sizeof(T);  // bytes a thread
     uint8_t* smem = reinterpret_cast<uint8_t*>(smem4);
-    Ring<T, V, NV, STAGES> ring_x(smem, t, group, width), ring_d(smem + kRing * blockDim.x, t, group, width);
+    const int shift = shift_of<T, V>(row, x_stride);
+    Ring<T, V, NV, STAGES, THREADS> ring_x(smem, t, group, width, shift),
+        ring_d(smem + kRing * THREADS, t, group, width, shift);
     // (mean, rstd) of each warp's next rows.
-    float* stats = reinterpret_cast<float*>(smem + 2 * kRing * blockDim.x) + (threadIdx.x >> 5) * 2 * STAGES;
+    float* stats = reinterpret_cast<float*>(smem + 2 * kRing * THREADS) + (threadIdx.x >> 5) * 2 * STAGES;
     float* joined = reinterpret_cast<float*>(smem);  // [2][width], once the rows are done
     auto fetch = [&](int stage, int64_t r) {
-        ring_x.fetch(stage, x + r * x_stride, t, group, width);
-        ring_d.fetch(stage, dy + r * dy_stride, t, group, width);
+        ring_x.fetch(stage, x + r * x_stride);
+        ring_d.fetch(stage, dy + r * dy_stride);
         if ((threadIdx.x & 31) == 0) {
             copy_async<4>(stats + 2 * stage, mean_in + r);
             copy_async<4>(stats + 2 * stage + 1, rstd_in + r);
@@ -238,7 +267,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 3 : 1)
         copy_commit();
     }
     f32x2 fw[PAIRS];
-    load_share<T, V, NV>(w, w_f32, 1.0f, t, group, width, fw);
+    load_share<T, V, NV>(w, w_f32, 1.0f, t, group, width, shift, fw);
     f32x2 dw[PAIRS], db[PAIRS];
 #pragma unroll
     for (int p = 0; p < PAIRS; p++) dw[p] = db[p] = 0;
@@ -253,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 3 : 1)
         const f32x2 away = pair(-stats[2 * stage], -stats[2 * stage]), rr = pair(stats[2 * stage + 1], stats[2 * stage + 1]);
 #pragma unroll
         for (int p = 0; p < PAIRS; p++) {
-            // dy is 0 past the width, so whatever x and w hold there adds nothing.
+            // dy is 0 outside the row, so whatever x and w hold there adds nothing.
             const f32x2 d = pair_of<T, V, NV>(pd, p);
             xh[p] = mul2(add2(pair_of<T, V, NV>(px, p), away), rr);
             gy[p] = mul2(d, fw[p]);
@@ -273,7 +302,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 3 : 1)
             const f32x2 mg2 = pair(-mg, -mg), mgx2 = pair(-mgx, -mgx);
 #pragma unroll
             for (int p = 0; p < PAIRS; p++) gy[p] = mul2(rr, fma2(xh[p], mgx2, add2(gy[p], mg2)));
-            store_row<T, V, NV>(dx + row * dx_stride, gy, t, group, width);
+            store_row<T, V, NV>(dx + row * dx_stride, gy, t, group, width, shift);
         }
     }
     if (!part) return;
@@ -285,8 +314,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 3 : 1)
         if (g == k) {
 #pragma unroll
             for (int e = 0; e < ELEMS; e++) {
-                const int c = (e / V * group + t) * V + e % V;
-                if (c >= width) continue;
+                const int c = (e / V * group + t) * V + e % V - shift;
+                if (c < 0 || c >= width) continue;
                 const float2 fw = unpair(dw[e / 2]), fb = unpair(db[e / 2]);
                 dst[c] = (k ? joined[c] : 0.0f) + (e % 2 ? fw.y : fw.x);
                 dst[width + c] = (k ? joined[width + c] : 0.0f) + (e % 2 ? fb.y : fb.x);
@@ -351,10 +380,33 @@ void allow_shared() {
     set.fetch_or(bit, std::memory_order_relaxed);
 }
 
+// Elements of a vector: 16 bytes of them, 2 of 16 bits, or 1.  A null
+// array does not count.
+template <class T>
+int vector_of(int width, std::initializer_list<std::pair<const void*, int64_t>> arrays, bool weights_aligned) {
+    constexpr int V = 16 / sizeof(T);
+    bool whole = width % V == 0 && weights_aligned, words = sizeof(T) == 2;
+    int64_t parity = -1;
+    for (const auto& [p, stride] : arrays) {
+        if (!p) continue;
+        whole = whole && rows_aligned(p, stride, sizeof(T));
+        // Every array's rows start alike in words of 4 bytes.
+        words = words && reinterpret_cast<uintptr_t>(p) % 4 == 0 && (parity < 0 || parity == (stride & 1));
+        parity = stride & 1;
+    }
+    return whole ? V : words ? 2 : 1;
+}
+template <class T, class F>
+void by_vector(int v, F&& fn) {
+    if (v == 16 / (int)sizeof(T)) return fn(std::integral_constant<int, 16 / sizeof(T)>{});
+    if constexpr (sizeof(T) == 2)
+        if (v == 2) return fn(std::integral_constant<int, 2>{});
+    fn(std::integral_constant<int, 1>{});
+}
+
 // fn(V, ELEMS, WIDE, THREADS) as compile-time values.
 template <class T, class F>
-void by_shape(bool vec, int width, F&& fn) {
-    constexpr int V = 16 / sizeof(T);
+void by_shape(int vec, int width, F&& fn) {
     using std::integral_constant;
     const integral_constant<int, 32 * kWarpsPerBlock> small{};
     auto elems = [&](auto v) {
@@ -362,11 +414,11 @@ void by_shape(bool vec, int width, F&& fn) {
         else if (width <= 512) fn(v, integral_constant<int, 16>{}, std::false_type{}, small);
         else if (width <= 768) fn(v, integral_constant<int, 24>{}, std::false_type{}, small);
         else if (width <= 1024) fn(v, integral_constant<int, 32>{}, std::false_type{}, small);
+        else if (width <= 4096) fn(v, integral_constant<int, kBlockElems>{}, std::true_type{}, small);
         else if (width <= 8192) fn(v, integral_constant<int, kBlockElems>{}, std::true_type{}, integral_constant<int, 512>{});
         else fn(v, integral_constant<int, kBlockElems>{}, std::true_type{}, integral_constant<int, 1024>{});
     };
-    if (vec) elems(integral_constant<int, V>{});
-    else elems(integral_constant<int, 1>{});
+    by_vector<T>(vec, elems);
 }
 
 }  // namespace
@@ -388,14 +440,16 @@ mdh_status mdh_layer_norm_forward(const void* x, int64_t x_stride, int32_t dtype
         MDH_REQUIRE(y, MDH_ERR_INVALID_ARG, "layer norm: null output");
         by_dtype(dtype, [&](auto zero) {
             using T = decltype(zero);
-            const bool vec = width % (16 / sizeof(T)) == 0 && rows_aligned(x, x_stride, sizeof(T)) &&
-                             rows_aligned(y, y_stride, sizeof(T)) && aligned16(w) && aligned16(b);
+            // One row has no stride of its own.
+            const auto at = [&](const void* p, int64_t stride) { return std::make_pair(p, rows > 1 ? stride : (int64_t)width); };
+            const int vec = vector_of<T>(width, {at(x, x_stride), at(y, y_stride)}, aligned16(w) && aligned16(b));
             by_shape<T>(vec, width, [&](auto v, auto elems, auto wide, auto most) {
                 const int threads = wide ? (int)round_up(ceil_div(width, elems), 32) : 32 * kWarpsPerBlock;
                 const int64_t units = wide ? rows : ceil_div(rows, kWarpsPerBlock);
-                const int64_t stay = 148 * std::max(1, 512 / threads);  // blocks that stay
                 constexpr int kShare = elems * sizeof(T), kRing = stages_of(most, kShare) * kShare;
-                const int smem = kRing * threads;
+                const int smem = kRing * most;
+                // Blocks that stay: 512 threads an SM, as far as their rings fit.
+                const int64_t stay = 148 * std::min(std::max(1, 512 / threads), blocks_that_fit(smem));
                 allow_shared<k_norm_forward<T, v, elems, wide, most>, most * kRing>();
                 k_norm_forward<T, v, elems, wide, most>
                     <<<(unsigned)std::min(units, stay), threads, smem, (cudaStream_t)stream>>>((const T*)x, x_stride, w, b, w_dtype == MDH_F32, rows, width, eps, (T*)y,
@@ -433,17 +487,19 @@ mdh_status mdh_layer_norm_backward(const void* dy, int64_t dy_stride, const void
         const bool sums = dw || db;
         MDH_REQUIRE(!sums || (ws && aligned16(ws) && ws_bytes >= mdh_layer_norm_backward_workspace(rows, width)),
                     MDH_ERR_INVALID_ARG, "layer norm: workspace too small or not 16-byte aligned");
-        const int blocks = backward_blocks(rows, width);
+        const int most_blocks = backward_blocks(rows, width);
+        int parts = 0;
         by_dtype(dtype, [&](auto zero) {
             using T = decltype(zero);
-            const bool vec = width % (16 / sizeof(T)) == 0 && rows_aligned(x, x_stride, sizeof(T)) &&
-                             rows_aligned(dy, dy_stride, sizeof(T)) && aligned16(w) &&
-                             (!dx || rows_aligned(dx, dx_stride, sizeof(T)));
+            const auto at = [&](const void* p, int64_t stride) { return std::make_pair(p, rows > 1 ? stride : (int64_t)width); };
+            const int vec = vector_of<T>(width, {at(x, x_stride), at(dy, dy_stride), at(dx, dx_stride)}, aligned16(w));
             const int group = backward_group(width), groups = backward_groups(width);
             auto launch = [&](auto v, auto elems, auto most) {
                 constexpr int kShare = 2 * elems * sizeof(T), kStages = stages_of(most, kShare);
-                const int rings = group * groups * kStages * kShare + 8 * kStages * (group * groups / 32);
+                const int rings = most * kStages * kShare + 8 * kStages * (group * groups / 32);
                 const int smem = std::max(rings, groups > 1 ? 2 * width * 4 : 0);
+                const int blocks = std::min(most_blocks, 148 * blocks_that_fit(smem));
+                if (sums) parts = blocks;
                 allow_shared<k_norm_backward<T, v, elems, most>, most * kStages * kShare + 8192>();
                 k_norm_backward<T, v, elems, most><<<blocks, group * groups, smem, st>>>(
                     (const T*)dy, dy_stride, (const T*)x, x_stride, w, w_dtype == MDH_F32, mean, rstd, rows, width,
@@ -455,17 +511,17 @@ mdh_status mdh_layer_norm_backward(const void* dy, int64_t dy_stride, const void
                 else if (width <= 512) launch(v, integral_constant<int, 16>{}, integral_constant<int, 128>{});
                 else if (width <= 768) launch(v, integral_constant<int, 24>{}, integral_constant<int, 128>{});
                 else if (width <= 1024) launch(v, integral_constant<int, 32>{}, integral_constant<int, 128>{});
+                else if (width <= 4096) launch(v, integral_constant<int, kBlockElems>{}, integral_constant<int, 256>{});
                 else if (width <= 8192) launch(v, integral_constant<int, kBlockElems>{}, integral_constant<int, 512>{});
                 else launch(v, integral_constant<int, kBlockElems>{}, integral_constant<int, 1024>{});
             };
-            if (vec) by_elems(std::integral_constant<int, 16 / sizeof(T)>{});
-            else by_elems(std::integral_constant<int, 1>{});
+            by_vector<T>(vec, by_elems);
         });
         check_launch();
         if (!sums) return;
         by_dtype(w_dtype, [&](auto zero) {
             using W = decltype(zero);
-            k_norm_join<W><<<(unsigned)ceil_div(2 * (int64_t)width, 32), 1024, 0, st>>>((const float*)ws, blocks, width,
+            k_norm_join<W><<<(unsigned)ceil_div(2 * (int64_t)width, 32), 1024, 0, st>>>((const float*)ws, parts, width,
                                                                                     (W*)dw, (W*)db);
         });
         check_launch();

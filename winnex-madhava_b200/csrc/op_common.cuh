@@ -131,6 +131,13 @@ __device__ __forceinline__ void copy_async(void* dst, const void* src, bool some
                  "n"(BYTES), "r"(some ? BYTES : 0)
                  : "memory");
 }
+// The first `bytes` of BYTES, the rest zeros.
+template <int BYTES>
+__device__ __forceinline__ void copy_async_part(void* dst, const void* src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+                 "n"(BYTES), "r"(bytes)
+                 : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Waits for this thread's copies, all but those of the last PENDING commits.
 template <int PENDING>
