@@ -47,6 +47,7 @@ constexpr int kMaxWarpsBack = 4;      // backward: its warps hold twice the vect
 constexpr int kRound = 128;           // entries of the list that a warp looks at at a time
 constexpr int kMaxHead = 256;
 constexpr int kMaxShared = 4;         // query heads of a unit
+constexpr int kMaxSharedMma = 8;      // ... in the matrix form
 constexpr int kMinSlice = 16;         // entries below which a list is not cut further
 
 struct CodeView {
@@ -57,6 +58,9 @@ struct CodeView {
     uint32_t flip;        // 0x80808080 for int8: the stored byte becomes c + 128
     float scale, base;    // affine: value = base + scale c
 };
+
+// How a call's rows are read: byte by byte, 8 bytes a lane, or by the matrix form.
+enum { kFormBytes = 0, kFormLanes = 1, kFormMma = 2 };
 
 struct AttendParams {
     CodeView k, v;
@@ -76,7 +80,7 @@ struct AttendParams {
     int unit_blocks;       // blocks that share a query's units
     int slices;            // warps of a block that share their units
     int splits, split_len; // ranges of a list over blocks, entries of each
-    bool aligned;          // rows of both caches start and step on 8 bytes
+    int form;              // kForm*
     void* out;
     float* lse;
     float* part;           // splits > 1: vectors [splits][queries][heads][head] (backward: two of them), then float2
@@ -161,6 +165,48 @@ __device__ __forceinline__ void store_elements(void* p, int64_t i, int dtype, co
         }
     }
     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 4 elements of q's type at p + i; vec: on the bytes they take.
+__device__ __forceinline__ void load4(const void* p, int64_t i, int dtype, bool vec, float (&v)[4]) {
+    if (dtype == MDH_F32) {
+        const float* f = static_cast<const float*>(p) + i;
+        if (vec) {
+            const float4 x = __ldg(reinterpret_cast<const float4*>(f));
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = f[j];
+        }
+        return;
+    }
+    const uint16_t* h = static_cast<const uint16_t*>(p) + i;
+    uint2 w;
+    if (vec) w = __ldg(reinterpret_cast<const uint2*>(h));
+    else w = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+    if (dtype == MDH_BF16) {
+        v[0] = __uint_as_float(w.x << 16), v[1] = __uint_as_float(w.x & 0xffff0000u);
+        v[2] = __uint_as_float(w.y << 16), v[3] = __uint_as_float(w.y & 0xffff0000u);
+    } else {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+        v[0] = x.x, v[1] = x.y, v[2] = y.x, v[3] = y.y;
+    }
+}
+// 4 elements at place i (a multiple of 4) of an aligned output.
+__device__ __forceinline__ void store4(void* p, int64_t i, int dtype, float4 v) {
+    if (dtype == MDH_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = v;
+        return;
+    }
+    uint2 w;
+    if (dtype == MDH_BF16) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+        w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    } else {
+        const __half2 x = __floats2half2_rn(v.x, v.y), y = __floats2half2_rn(v.z, v.w);
+        w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = w;
 }
 
 // What a lane works on.
@@ -599,6 +645,299 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(cons
     }
 }
 
+// ------------------------------------------------------------ matrix form
+// Where two or more query heads share a row, the tensor cores take both
+// products (mma.sync m16n8k16, float32 sums): a warp holds one unit, up to 8
+// heads, and 16 entries at a time.
+//
+// Scores: A rows 0-7 are the heads' queries rounded to float16 (scaled by a
+// power of two to use its range), rows 8-15 what the rounding left, so their
+// sum carries 22 bits; B are the key codes, exact in float16, as bytes of
+// 1024 + (c + 128) less 1152.  Values: A are the value codes with dimensions
+// as rows, exact in bfloat16 (a byte's low 7 bits over 128 less 128 or 256,
+// its top bit), B the weights p times the row's scale as three bfloat16 parts:
+// 24 bits at any size, since a weight may count where the larger ones' values
+// are 0.  A lane finds its codes as 32-bit words: which
+// dimension a word's bytes stand for is the same on both sides of a product,
+// so no byte moves between lanes.  Each entry's head lies in shared memory
+// 16 bytes past a multiple of the bank width, so those words hit all banks.
+constexpr int kMmaEntries = 16;
+template <int NS>  // of 16 dimensions
+struct Mma {
+    static constexpr int HEAD = NS * 16;
+    static constexpr int ROW = HEAD + 16;                         // bytes of an entry
+    static constexpr int STAGE = 2 * kMmaEntries * ROW + 2 * kMmaEntries * 4;
+    static constexpr int STAGES = 3;
+    static constexpr int RING = STAGES * STAGE;
+    static constexpr int JOIN = kMaxSharedMma * (HEAD + 2) * 4;   // vectors, m, l of a warp
+    static_assert(JOIN <= RING && STAGE % 16 == 0, "the joined vectors lie in the rings");
+};
+
+__device__ __forceinline__ void mma16816_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Bytes c (two's complement) split into low 7 bits and top bit -> the pair of
+// bfloat16 c: bytes 0 and 1, or 2 and 3.
+__device__ __forceinline__ uint32_t bf16_codes(uint32_t low, uint32_t top, bool high) {
+    const uint32_t x = __byte_perm(low, 0x43434343u, high ? 0x4342 : 0x4140), y = __byte_perm(top, 0x43434343u, high ? 0x4342 : 0x4140);
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Two floats as three bfloat16 parts each.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&part)[3]) {
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        part[k] = *reinterpret_cast<const uint32_t*>(&h);
+        x -= __uint_as_float(part[k] << 16);
+        y -= __uint_as_float(part[k] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Bytes c + 128 -> the pair of float16 c: bytes 0 and 1, or 2 and 3.
+__device__ __forceinline__ uint32_t half_codes(uint32_t w, bool high) {
+    const uint32_t x = __byte_perm(w, 0x64646464u, high ? 0x4342 : 0x4140);
+    const __half2 off = __half2half2(__ushort_as_half(0xE480));  // -1152
+    const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&x), off);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Two floats as float16 and what is left of them.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// The power of two at x > 0 or just below; 1 where x is 0 or not finite.
+__device__ __forceinline__ float power_of_two(float x) {
+    const uint32_t e = __float_as_uint(x) & 0x7f800000u;
+    return e == 0 || e == 0x7f800000u ? 1.0f : __uint_as_float(e);
+}
+
+template <int NS>
+__global__ void __launch_bounds__(32 * kMaxWarps, NS > 4 ? 1 : 2) k_attend_mma(const __grid_constant__ AttendParams a) {
+    using M = Mma<NS>;
+    extern __shared__ uint8_t sm[];  // the warps' rings, later the vectors to join; then the entries
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int warps = blockDim.x >> 5;
+    const Entries list = entries_at(sm + warps * M::RING, warps);
+    uint8_t* ring = sm + warp * M::RING;
+    // Lanes of one unit: work_of with a lane group of 32 (its own elements are not used).
+    const Work w = work_of<32>(a);
+    const int e0 = min(w.h0 / a.shared, a.heads / a.shared - 1) * M::HEAD;
+    const bool mine = g < w.nr;  // this lane's score rows are a head
+
+    // Queries: head g, dimensions 16 s + 4 c + 0 .. 3.
+    uint32_t q[NS][4];
+    float unscale, kb;
+    {
+        float x[NS][4], top = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            if (mine) load4(a.q, w.i * a.q_stride + (w.h0 + g) * a.q_head_stride + 16 * s + 4 * c, a.dtype, a.q_vec, x[s]);
+            else x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                top = fmaxf(top, fabsf(x[s][j]));
+                sum += x[s][j];
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        const float unit = power_of_two(fmaxf(top, 0x1p-100f)), up = 1024.0f / unit;  // the largest lies in [1024, 2048)
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            split2(x[s][0] * up, x[s][1] * up, q[s][0], q[s][1]);
+            split2(x[s][2] * up, x[s][3] * up, q[s][2], q[s][3]);
+        }
+        unscale = a.scale * unit * (1.0f / 1024.0f);
+        kb = a.scale * a.k.base * sum;
+    }
+    float acc[NS][4];  // dimensions x heads 2 c, 2 c + 1
+#pragma unroll
+    for (int t = 0; t < NS; t++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[t][j] = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // of head g; l of this lane's entries
+
+    const uint8_t *kp = a.k.codes + e0, *vp = a.v.codes + e0;
+    const float* ksp = a.k.scales ? a.k.scales + e0 / a.k.group : nullptr;
+    const float* vsp = a.v.scales ? a.v.scales + e0 / a.v.group : nullptr;
+    auto fetch = [&](int stage, int first, int hi) {
+        uint8_t* to = ring + stage * M::STAGE;
+#pragma unroll
+        for (int k = 0; k < NS; k++) {
+            const int x = lane + 32 * k, value = x / (kMmaEntries * NS), y = x % (kMmaEntries * NS);
+            const int e = first + y / NS, at = y % NS * 16;
+            const bool some = e < hi;
+            const uint64_t slot = some ? (uint32_t)list.slot[e] : 0u;
+            copy_async<16>(to + value * kMmaEntries * M::ROW + y / NS * M::ROW + at,
+                           (value ? vp + slot * a.v.stride : kp + slot * a.k.stride) + at, some);
+        }
+        const int e = first + (lane & 15);
+        const bool some = e < hi, value = lane >= 16;
+        const uint64_t slot = some ? (uint32_t)list.slot[e] : 0u;
+        const float* from = value ? vsp : ksp;
+        if (from) copy_async<4>(to + 2 * kMmaEntries * M::ROW + lane * 4, from + slot * (uint32_t)(value ? a.v.n_groups : a.k.n_groups), some);
+        copy_commit();
+    };
+
+    const uint32_t v_flip = a.v.flip ^ 0x80808080u;  // bytes c here, c + 128 with the keys
+    const int32_t doc = a.query_docs ? a.query_docs[w.i] : 0;
+    const int j0 = (int)min((int64_t)blockIdx.y * a.split_len, (int64_t)a.found);
+    const int j1 = (int)min((int64_t)j0 + a.split_len, (int64_t)a.found);
+    for (int from = j0; from < j1; from += warps * kRound) {
+        int lo, hi;
+        slice_of(list_entries(a, list, w.i, doc, from, j1), w.slice, a.slices, kMmaEntries, lo, hi);
+        if (w.idle) hi = lo;
+        copy_wait<0>();
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < M::STAGES - 1; k++) fetch(k, lo + k * kMmaEntries, hi);
+        int stage = 0;
+        for (int t = lo; t < hi; t += kMmaEntries) {
+            copy_wait<M::STAGES - 2>();
+            __syncwarp();  // every lane's copies of this stage are there, and its reads of the one before are done
+            fetch(stage == 0 ? M::STAGES - 1 : stage - 1, t + (M::STAGES - 1) * kMmaEntries, hi);
+            const uint8_t* at = ring + stage * M::STAGE;
+            const float* scales = reinterpret_cast<const float*>(at + 2 * kMmaEntries * M::ROW);
+            stage = stage + 1 == M::STAGES ? 0 : stage + 1;
+            // Scores of entries 8 n + 2 c, + 1 for head g.
+            float p[4];
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint32_t* row = reinterpret_cast<const uint32_t*>(at + (8 * n + g) * M::ROW);
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+                    const uint32_t word = row[4 * s + c] ^ a.k.flip;
+                    mma16816(d, q[s], half_codes(word, false), half_codes(word, true));
+                }
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int e = 8 * n + 2 * c + j;
+                    const float ks = ksp ? scales[e] : a.k.scale;
+                    float th;
+                    p[2 * n + j] = t + e < hi ? score_of(a, fmaf((d[j] + d[2 + j]) * unscale, ks, kb), list.bias[t + e], th)
+                                              : -INFINITY;
+                }
+            }
+            float top = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), m);
+            const float ref = top == -INFINITY ? 0.0f : top, keep = m == top ? 1.0f : expf(m - ref);
+            m = top;
+            if (__any_sync(0xffffffffu, keep != 1.0f)) {
+                const float s0 = __shfl_sync(0xffffffffu, keep, 8 * c), s1 = __shfl_sync(0xffffffffu, keep, 8 * c + 4);
+#pragma unroll
+                for (int k = 0; k < NS; k++) acc[k][0] *= s0, acc[k][1] *= s1, acc[k][2] *= s0, acc[k][3] *= s1;
+            }
+            l *= keep;
+            float weight[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                p[j] = expf(p[j] - ref);
+                l += p[j];
+                weight[j] = p[j] * (vsp ? scales[kMmaEntries + 8 * (j >> 1) + 2 * c + (j & 1)] : a.v.scale);
+            }
+            uint32_t w0[3], w1[3];
+            split3(weight[0], weight[1], w0);
+            split3(weight[2], weight[3], w1);
+            // Values: word 8 k + g of an entry holds the rows g and g + 8 of two products.
+            const uint8_t* values = at + kMmaEntries * M::ROW + 2 * c * M::ROW;
+#pragma unroll
+            for (int k = 0; k < NS / 2; k++) {
+                const int off = (8 * k + g) * 4;
+                uint32_t v[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    v[j] = *reinterpret_cast<const uint32_t*>(values + ((j >> 1) * 8 + (j & 1)) * M::ROW + off) ^ v_flip;
+                const uint32_t x0 = __byte_perm(v[0], v[1], 0x5140), y0 = __byte_perm(v[0], v[1], 0x7362);
+                const uint32_t x1 = __byte_perm(v[2], v[3], 0x5140), y1 = __byte_perm(v[2], v[3], 0x7362);
+                constexpr uint32_t kLow = 0x7f7f7f7fu, kTop = 0x80808080u;
+                const uint32_t first[4] = {bf16_codes(x0 & kLow, x0 & kTop, false), bf16_codes(x0 & kLow, x0 & kTop, true),
+                                           bf16_codes(x1 & kLow, x1 & kTop, false), bf16_codes(x1 & kLow, x1 & kTop, true)};
+                const uint32_t second[4] = {bf16_codes(y0 & kLow, y0 & kTop, false), bf16_codes(y0 & kLow, y0 & kTop, true),
+                                            bf16_codes(y1 & kLow, y1 & kTop, false), bf16_codes(y1 & kLow, y1 & kTop, true)};
+#pragma unroll
+                for (int j = 2; j >= 0; j--) {  // the small parts first
+                    mma16816_bf16(acc[2 * k], first, w0[j], w1[j]);
+                    mma16816_bf16(acc[2 * k + 1], second, w0[j], w1[j]);
+                }
+            }
+        }
+    }
+    copy_wait<0>();
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    // This lane's vectors: heads 2 c and 2 c + 1, dimensions 32 k + 4 g + 0 .. 3.
+    float* mine_at = reinterpret_cast<float*>(sm + warp * M::RING);
+    float mm[2], ll[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int from = 8 * c + 4 * h;
+        mm[h] = __shfl_sync(0xffffffffu, m, from);
+        ll[h] = __shfl_sync(0xffffffffu, l, from);
+    }
+    if (a.slices > 1) {
+        __syncthreads();  // the rings have been read
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float* dst = mine_at + (2 * c + h) * (M::HEAD + 2);
+#pragma unroll
+            for (int k = 0; k < NS; k++) dst[32 * (k / 2) + 4 * g + 2 * (k & 1)] = acc[k][h], dst[32 * (k / 2) + 4 * g + 2 * (k & 1) + 1] = acc[k][2 + h];
+            if (g == 0) dst[M::HEAD] = mm[h], dst[M::HEAD + 1] = ll[h];
+        }
+        __syncthreads();
+        if (w.slice == 0) {
+            for (int k2 = 1; k2 < a.slices; k2++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float* src = mine_at + k2 * (M::RING / 4) + (2 * c + h) * (M::HEAD + 2);
+                    float f, o;
+                    mm[h] = join(mm[h], src[M::HEAD], f, o);
+                    ll[h] = ll[h] * f + src[M::HEAD + 1] * o;
+#pragma unroll
+                    for (int k = 0; k < NS; k++) {
+                        const int d = 32 * (k / 2) + 4 * g + 2 * (k & 1);
+                        acc[k][h] = acc[k][h] * f + src[d] * o;
+                        acc[k][2 + h] = acc[k][2 + h] * f + src[d + 1] * o;
+                    }
+                }
+        }
+    }
+    if (w.slice != 0) return;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (2 * c + h >= w.nr) continue;
+        const int64_t at = w.i * a.heads + w.h0 + 2 * c + h, n = a.queries * a.heads, row = (int64_t)blockIdx.y * n + at;
+        const float inv = a.part ? 1.0f : ll[h] != 0.0f ? 1.0f / ll[h] : 0.0f, base = a.part || ll[h] == 0.0f ? 0.0f : a.v.base;
+#pragma unroll
+        for (int k = 0; k < NS / 2; k++) {
+            const float4 v = make_float4(fmaf(acc[2 * k][h], inv, base), fmaf(acc[2 * k][2 + h], inv, base),
+                                         fmaf(acc[2 * k + 1][h], inv, base), fmaf(acc[2 * k + 1][2 + h], inv, base));
+            const int d = 32 * k + 4 * g;
+            if (a.part) *reinterpret_cast<float4*>(a.part + row * a.head + d) = v;
+            else store4(a.out, at * a.head + d, a.dtype, v);
+        }
+        if (g != 0) continue;
+        if (a.part) reinterpret_cast<float2*>(a.part + a.splits * n * a.head)[row] = make_float2(mm[h], ll[h]);
+        else a.lse[at] = ll[h] != 0.0f ? mm[h] + logf(ll[h]) : -INFINITY;
+    }
+}
+
 // Joins the ranges of a list: a block for each (query, head), 8 elements a
 // lane group of 4 warps, each every fourth range; the warps' sums in order.
 __global__ void __launch_bounds__(128) k_attend_join(const __grid_constant__ AttendParams a) {
@@ -853,11 +1192,12 @@ CodeView code_view(const RowsView& r) {
     return c;
 }
 
-// Lanes that hold a head; rows off 8 bytes take the widest form alone.
+// Lanes that hold a head; rows off 8 bytes take the widest form alone, the
+// matrix form a warp.
 int lanes_of(const AttendParams& p) {
     int lanes = 1;
     while (lanes * 8 < p.head) lanes *= 2;
-    return p.aligned ? lanes : 32;
+    return p.form == kFormLanes ? lanes : 32;
 }
 
 // How a call is laid out over warps and blocks.  Units side by side in a warp
@@ -867,8 +1207,9 @@ int lanes_of(const AttendParams& p) {
 // of a block share units' lists, and then blocks take ranges of a list, up to
 // kFill warps; no slice is below kMinSlice entries.
 void lay_out(AttendParams& p, int max_warps) {
-    constexpr int64_t kEnough = 148 * 8, kFill = 148 * 16;
-    p.r_blocks = (int)ceil_div(p.shared, kMaxShared);
+    // The matrix form of heads past 64 has room for 8 warps an SM.
+    const int64_t kEnough = 148 * 8, kFill = p.form == kFormMma && p.head > 64 ? 148 * 8 : 148 * 16;
+    p.r_blocks = (int)ceil_div(p.shared, p.form == kFormMma ? kMaxSharedMma : kMaxShared);
     p.rb = (int)ceil_div(p.shared, p.r_blocks);
     p.units = p.heads / p.shared * p.r_blocks;
     int side = 32 / lanes_of(p);
@@ -886,7 +1227,7 @@ void lay_out(AttendParams& p, int max_warps) {
     p.splits = (int)std::max<int64_t>(1, ceil_div(p.found, p.split_len));
 }
 
-AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values, int max_warps) {
+AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values, bool forward) {
     MDH_REQUIRE(a, MDH_ERR_INVALID_ARG, "attend: null arguments");
     AttendParams p{};
     const RowsView k = rows_view(keys), v = rows_view(values);
@@ -911,7 +1252,13 @@ AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const 
                 "attend: list stride below its length (0: one list for every query)");
     p.k = code_view(k);
     p.v = code_view(v);
-    p.aligned = rows_on_8(k) && rows_on_8(v);
+    // The matrix form takes heads of 32 .. 128 that start on 16 bytes and have one scale each; a head of its own
+    // gains nothing from it (4,096 queries x 12 heads of 64, 25 entries seen: 82 us by lanes).
+    auto one_scale = [&](const RowsView& c) { return c.affine || c.n_groups == 1 || c.group % a->head == 0; };
+    auto on_16 = [](const RowsView& c) { return aligned16(c.codes) && c.stride % 16 == 0; };
+    const bool matrix = forward && a->shared >= 2 && a->head % 32 == 0 && a->head <= 128 && one_scale(k) && one_scale(v) &&
+                        on_16(k) && on_16(v);
+    p.form = matrix ? kFormMma : rows_on_8(k) && rows_on_8(v) ? kFormLanes : kFormBytes;
     const size_t size = dtype_size(a->dtype);
     p.q_vec = rows_aligned(a->q, a->q_stride, size) && rows_aligned(a->q, a->q_head_stride, size) &&
               a->head * size % 16 == 0;
@@ -934,20 +1281,20 @@ AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const 
     p.scale = a->scale;
     p.cap = a->cap;
     p.inv_cap = a->cap > 0.0f ? 1.0f / a->cap : 0.0f;
-    lay_out(p, max_warps);
+    lay_out(p, forward ? kMaxWarps : kMaxWarpsBack);
     MDH_REQUIRE(p.queries * p.unit_blocks <= INT32_MAX && p.queries * p.heads <= INT32_MAX, MDH_ERR_UNSUPPORTED, "attend: too many queries");
     return p;
 }
 
 // The layout of a call from its sizes alone, for the workspace.
-AttendParams layout_of(const mdh_attend_args* a, bool aligned, int max_warps) {
+AttendParams layout_of(const mdh_attend_args* a, int form, int max_warps) {
     AttendParams p{};
     p.queries = a->queries;
     p.found = a->found;
     p.heads = a->heads;
     p.shared = a->shared;
     p.head = a->head;
-    p.aligned = aligned;
+    p.form = form;
     lay_out(p, max_warps);
     return p;
 }
@@ -967,7 +1314,7 @@ int64_t backward_part(const AttendParams& p) {
 template <class F>
 void by_shape(const AttendParams& p, F&& fn) {
     using std::integral_constant;
-    if (!p.aligned) return fn(integral_constant<int, 32>{}, integral_constant<int, 4>{}, std::false_type{});
+    if (p.form == kFormBytes) return fn(integral_constant<int, 32>{}, integral_constant<int, 4>{}, std::false_type{});
     auto heads = [&](auto lanes) {
         if (p.rb == 1) fn(lanes, integral_constant<int, 1>{}, std::true_type{});
         else if (p.rb == 2) fn(lanes, integral_constant<int, 2>{}, std::true_type{});
@@ -986,19 +1333,31 @@ void by_shape(const AttendParams& p, F&& fn) {
 dim3 attend_grid(const AttendParams& p) {
     return dim3((unsigned)(p.queries * p.unit_blocks), (unsigned)p.splits);
 }
-template <int LANES, int RB, bool ALIGNED, bool BACKWARD>
-void launch_form(const AttendParams& p, cudaStream_t st) {
-    constexpr int kWarpBytes = Steps<LANES, RB>::RING + kEntriesBytes;
-    const auto kernel = BACKWARD ? k_attend_backward<LANES, RB, ALIGNED> : k_attend<LANES, RB, ALIGNED>;
+// Launches KERNEL with `WARP_BYTES` of shared memory for each of its warps.
+template <auto KERNEL, int WARP_BYTES, int MAX_WARPS>
+void launch_warps(const AttendParams& p, cudaStream_t st) {
     static std::atomic<uint64_t> set{0};  // a bit a device
     const int dev = current_device(), warps = p.block_warps * p.slices;
     if (!(set.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-        MDH_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (BACKWARD ? kMaxWarpsBack : kMaxWarps) * kWarpBytes));
+        MDH_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_WARPS * WARP_BYTES));
         set.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_relaxed);
     }
-    kernel<<<attend_grid(p), 32 * warps, warps * kWarpBytes, st>>>(p);
+    KERNEL<<<attend_grid(p), 32 * warps, warps * WARP_BYTES, st>>>(p);
     check_launch();
+}
+template <int LANES, int RB, bool ALIGNED, bool BACKWARD>
+void launch_lanes(const AttendParams& p, cudaStream_t st) {
+    constexpr int kWarpBytes = Steps<LANES, RB>::RING + kEntriesBytes;
+    if constexpr (BACKWARD) launch_warps<k_attend_backward<LANES, RB, ALIGNED>, kWarpBytes, kMaxWarpsBack>(p, st);
+    else launch_warps<k_attend<LANES, RB, ALIGNED>, kWarpBytes, kMaxWarps>(p, st);
+}
+void launch_mma(const AttendParams& p, cudaStream_t st) {
+    switch (p.head) {
+        case 32: launch_warps<k_attend_mma<2>, Mma<2>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
+        case 64: launch_warps<k_attend_mma<4>, Mma<4>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
+        case 96: launch_warps<k_attend_mma<6>, Mma<6>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
+        default: launch_warps<k_attend_mma<8>, Mma<8>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
+    }
 }
 
 }  // namespace
@@ -1010,13 +1369,14 @@ extern "C" {
 
 int64_t mdh_attend_workspace(const mdh_attend_args* a) {
     if (!has_sizes(a)) return 0;
-    return std::max(forward_part(layout_of(a, true, kMaxWarps)), forward_part(layout_of(a, false, kMaxWarps)));
+    return std::max({forward_part(layout_of(a, kFormBytes, kMaxWarps)), forward_part(layout_of(a, kFormLanes, kMaxWarps)),
+                     forward_part(layout_of(a, kFormMma, kMaxWarps))});
 }
 
 mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values, void* out, float* lse,
                       void* ws, int64_t ws_bytes, void* stream) {
     return guarded([&] {
-        AttendParams p = check_attend(a, keys, values, kMaxWarps);
+        AttendParams p = check_attend(a, keys, values, true);
         current_device();
         if (p.queries == 0) return;
         MDH_REQUIRE(out && lse && aligned16(out), MDH_ERR_INVALID_ARG, "attend: output null or not 16-byte aligned");
@@ -1027,9 +1387,8 @@ mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_
         p.out = out;
         p.lse = lse;
         p.part = p.splits > 1 ? (float*)ws : nullptr;
-        by_shape(p, [&](auto lanes, auto rb, auto aligned) {
-            launch_form<lanes, rb, aligned, false>(p, st);
-        });
+        if (p.form == kFormMma) launch_mma(p, st);
+        else by_shape(p, [&](auto lanes, auto rb, auto aligned) { launch_lanes<lanes, rb, aligned, false>(p, st); });
         if (p.splits > 1) {
             k_attend_join<<<(unsigned)(p.queries * p.heads), 128, 0, st>>>(p);
             check_launch();
@@ -1039,7 +1398,8 @@ mdh_status mdh_attend(const mdh_attend_args* a, const mdh_rows* keys, const mdh_
 
 int64_t mdh_attend_backward_workspace(const mdh_attend_args* a, int32_t want_dbias) {
     if (!has_sizes(a)) return 0;
-    int64_t need = std::max(backward_part(layout_of(a, true, kMaxWarpsBack)), backward_part(layout_of(a, false, kMaxWarpsBack)));
+    int64_t need = std::max(backward_part(layout_of(a, kFormBytes, kMaxWarpsBack)),
+                            backward_part(layout_of(a, kFormLanes, kMaxWarpsBack)));
     if (want_dbias) need += a->queries * a->heads * 8 + a->queries * a->heads * (int64_t)a->found * 8;
     return need;
 }
@@ -1048,7 +1408,7 @@ mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, c
                                const void* dout, const float* lse, void* dq, float* dbias, void* ws, int64_t ws_bytes,
                                void* stream) {
     return guarded([&] {
-        AttendParams p = check_attend(a, keys, values, kMaxWarpsBack);
+        AttendParams p = check_attend(a, keys, values, false);
         current_device();
         if (p.queries == 0) return;
         MDH_REQUIRE(dout && lse && dq && aligned16(dq), MDH_ERR_INVALID_ARG,
@@ -1071,7 +1431,7 @@ mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, c
         p.dout_vec = aligned16(dout) && a->head * dtype_size(a->dtype) % 16 == 0;
         p.lse_in = lse;
         by_shape(p, [&](auto lanes, auto rb, auto aligned) {
-            launch_form<lanes, rb, aligned, true>(p, st);
+            launch_lanes<lanes, rb, aligned, true>(p, st);
         });
         if (p.splits > 1) {
             k_attend_backward_join<<<(unsigned)(p.queries * p.heads), 128, 0, st>>>(p);
