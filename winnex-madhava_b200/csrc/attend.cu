@@ -1252,11 +1252,15 @@ AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const 
                 "attend: list stride below its length (0: one list for every query)");
     p.k = code_view(k);
     p.v = code_view(v);
-    // The matrix form takes heads of 32 .. 128 that start on 16 bytes and have one scale each; a head of its own
-    // gains nothing from it (4,096 queries x 12 heads of 64, 25 entries seen: 82 us by lanes).
+    // The matrix form takes heads of 32 .. 128 that start on 16 bytes and have one scale each.  Its time hardly
+    // depends on how many heads share a row (256 queries x 1,000 x 4 heads of 64: 60 us for 2 .. 8; by lanes 81, 96,
+    // 112 and 206).  Short lists of many queries are bound by what comes before and after the entries, which the
+    // lanes do for several units at once (2,048 queries x 64 entries, shared by 2, 3, 4, 8: 43 us against 34, 46, 54
+    // and 99); a head of its own gains nothing.
     auto one_scale = [&](const RowsView& c) { return c.affine || c.n_groups == 1 || c.group % a->head == 0; };
     auto on_16 = [](const RowsView& c) { return aligned16(c.codes) && c.stride % 16 == 0; };
-    const bool matrix = forward && a->shared >= 2 && a->head % 32 == 0 && a->head <= 128 && one_scale(k) && one_scale(v) &&
+    const bool pays = a->shared >= 4 || a->found >= 128 || a->queries * (a->heads / a->shared) < 148 * 8;
+    const bool matrix = forward && a->shared >= 2 && pays && a->head % 32 == 0 && a->head <= 128 && one_scale(k) && one_scale(v) &&
                         on_16(k) && on_16(v);
     p.form = matrix ? kFormMma : rows_on_8(k) && rows_on_8(v) ? kFormLanes : kFormBytes;
     const size_t size = dtype_size(a->dtype);
