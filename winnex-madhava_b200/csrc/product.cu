@@ -451,17 +451,26 @@ __global__ void __launch_bounds__(256) k_product_join(const __grid_constant__ Pr
     }
 }
 
-// Rows of 16-bit elements -> rows of `pitch` elements (what follows the row is not read).
-__global__ void __launch_bounds__(256) k_pack_rows(const uint16_t* __restrict__ src, int64_t stride, int64_t rows,
-                                                   int64_t width, uint16_t* __restrict__ dst, int64_t pitch) {
-    const int64_t pieces = pitch / 8, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// Rows of 16-bit elements -> rows of `pitch` elements (what follows the row is
+// not read); one operand for each blockIdx.y.
+struct PackJob {
+    const uint16_t* src;
+    uint16_t* dst;
+    int64_t stride, rows, width, pitch;
+};
+struct PackJobs {
+    PackJob job[2];
+};
+__global__ void __launch_bounds__(256) k_pack_rows(const __grid_constant__ PackJobs jobs) {
+    const PackJob& p = jobs.job[blockIdx.y];
+    const int64_t pieces = p.pitch / 8, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t r = at / pieces;
-    if (r >= rows) return;
+    if (r >= p.rows) return;
     const int64_t c = (at - r * pieces) * 8;
     uint16_t e[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) e[j] = c + j < width ? src[r * stride + c + j] : (uint16_t)0;
-    *reinterpret_cast<uint4*>(dst + r * pitch + c) = *reinterpret_cast<const uint4*>(e);
+    for (int j = 0; j < 8; j++) e[j] = c + j < p.width ? p.src[r * p.stride + c + j] : (uint16_t)0;
+    *reinterpret_cast<uint4*>(p.dst + r * p.pitch + c) = *reinterpret_cast<const uint4*>(e);
 }
 
 // ------------------------------------------------------------ host
@@ -492,11 +501,15 @@ Plan plan_product(int64_t m, int64_t n, int64_t nkb) {
     for (int bn : {256, 128, 64}) {
         const double block = bn == 256 ? 1.0 : bn == 128 ? 0.55 : 0.35;
         const int64_t tiles = ceil_div(m, BM) * ceil_div(n, bn);
-        for (int s = 1; s <= 64 && s <= nkb; s++) {
+        // Unsplit, or the fewest parts that bring a part down to what 1, 2 or 3 rounds of the SMs allow.
+        for (int rounds = 0; rounds <= 3; rounds++) {
+            int64_t s = rounds ? std::min<int64_t>({64, nkb, 148 * rounds / tiles}) : 1;
+            if (rounds && s < 2) continue;
+            s = ceil_div(nkb, ceil_div(nkb, s));
             const double waves = (double)ceil_div(tiles * s, 148);
             double cost = waves * ((double)ceil_div(nkb, s) * block + 3.0);
             if (s > 1) cost += 10.0 + (double)(s + 1) * m * n * 4 / 3.0e6;
-            if (cost < best_cost) best_cost = cost, best = {bn, s};
+            if (cost < best_cost) best_cost = cost, best = {bn, (int)s};
         }
     }
     return best;
@@ -516,14 +529,20 @@ int64_t packed_bytes(const ProductOperand& o, int64_t rows, int64_t k) {
     return readable(o) ? 0 : lines(o, rows, k) * round_up(line(o, rows, k), 8) * 2;
 }
 
-ProductOperand pack(const ProductOperand& o, int64_t rows, int64_t k, void* to, cudaStream_t st) {
+// The operand itself, or where its packed copy will be and the job that makes it.
+ProductOperand packed(const ProductOperand& o, int64_t rows, int64_t k, void* to, PackJobs& jobs, int& n) {
     if (readable(o)) return o;
-    const int64_t n = lines(o, rows, k), width = line(o, rows, k), pitch = round_up(width, 8);
-    const int64_t blocks = ceil_div(n * (pitch / 8), 256);
-    MDH_REQUIRE(blocks <= INT32_MAX, MDH_ERR_UNSUPPORTED, "linear: operand too large");
-    k_pack_rows<<<(unsigned)blocks, 256, 0, st>>>((const uint16_t*)o.p, o.stride, n, width, (uint16_t*)to, pitch);
-    check_launch();
+    const int64_t width = line(o, rows, k), pitch = round_up(width, 8);
+    jobs.job[n++] = {(const uint16_t*)o.p, (uint16_t*)to, o.stride, lines(o, rows, k), width, pitch};
     return {to, pitch, o.k_major};
+}
+void pack(const PackJobs& jobs, int n, cudaStream_t st) {
+    if (n == 0) return;
+    int64_t blocks = 0;
+    for (int i = 0; i < n; i++) blocks = std::max(blocks, ceil_div(jobs.job[i].rows * (jobs.job[i].pitch / 8), 256));
+    MDH_REQUIRE(blocks <= INT32_MAX, MDH_ERR_UNSUPPORTED, "linear: operand too large");
+    k_pack_rows<<<dim3((unsigned)blocks, (unsigned)n), 256, 0, st>>>(jobs);
+    check_launch();
 }
 
 void tensor_map(CUtensorMap* map, const ProductOperand& o, int64_t rows, int64_t k, int tile_rows) {
@@ -562,10 +581,13 @@ void product(const ProductOperand& a0, const ProductOperand& b0, int64_t m, int6
              const ProductEpilogue& ep, void* ws, cudaStream_t st) {
     const int sms = device_sm_count(current_device());
     char* at = static_cast<char*>(ws);
-    const ProductOperand a = pack(a0, m, k, at, st);
+    PackJobs jobs{};
+    int n_jobs = 0;
+    const ProductOperand a = packed(a0, m, k, at, jobs, n_jobs);
     at += round_up(packed_bytes(a0, m, k), 128);
-    const ProductOperand b = pack(b0, n, k, at, st);
+    const ProductOperand b = packed(b0, n, k, at, jobs, n_jobs);
     at += round_up(packed_bytes(b0, n, k), 128);
+    pack(jobs, n_jobs, st);
     const Plan plan = plan_product(m, n, ceil_div(k, KB));
     ProductParams p{};
     p.m = (int)m;

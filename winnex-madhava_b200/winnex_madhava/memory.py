@@ -99,8 +99,13 @@ def _call(index, fn, *args):
             fn(*args, _stream_of(index))
 
 
-def _workspace(size, device):
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+def _like(t):
+    """A contiguous tensor of t's shape, type and device, not initialised."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(tuple(t.shape))
+
+
+def _workspace(size, t):
+    return t.new_empty((size,), dtype=torch.uint8) if size else None
 
 
 # ------------------------------------------------------------------ layer norm
@@ -126,10 +131,11 @@ def _norm_forward(x, weight, bias, eps, keep):
     if width < 1:
         raise ValueError("x must have a last dimension of at least 1")
     kind = _norm_weights(index, width, x.dtype, weight, bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _like(x)
     mean = rstd = None
     if keep:
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        mean = x.new_empty((rows,), dtype=torch.float32)
+        rstd = torch.empty_like(mean)
     _call(index, _native._layer_norm_forward, x2.data_ptr(), stride, code, _ptr(weight), _ptr(bias), _DTYPES[kind],
           rows, width, eps, y.data_ptr(), width, _ptr(mean), _ptr(rstd))
     return y, mean, rstd
@@ -164,10 +170,11 @@ def layer_norm_backward(dy, x, weight, mean, rstd, *, weight_dtype=None):
         _require(t.dtype == torch.float32, f"{name} must be float32")
         _on(index, t, name)
     _on(index, dy, "dy")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw, db = torch.empty((2, width), dtype=kind, device=x.device)
+    dx = _like(x)
+    dw = x.new_empty((width,), dtype=kind)
+    db = torch.empty_like(dw)
     size = _native._layer_norm_backward_workspace(rows, width)
-    ws = _workspace(size, x.device)
+    ws = _workspace(size, x)
     _call(index, _native._layer_norm_backward, dy2.data_ptr(), dy_stride, x2.data_ptr(), stride, code, _ptr(weight),
           _DTYPES[kind], mean.data_ptr(), rstd.data_ptr(), rows, width, dx.data_ptr(), width, dw.data_ptr(),
           db.data_ptr(), _ptr(ws), size)
@@ -254,11 +261,11 @@ def linear_forward(x, weight, bias=None, *, activation=None, residual=None, keep
         _on(index, residual, "residual")
         _, _, res_stride, r2 = _rows(residual, "residual")
         res = r2.data_ptr()
-    y = torch.empty(shape, dtype=kind, device=x.device)
-    z = torch.empty(shape, dtype=kind, device=x.device) if keep_preactivation and act else None
+    y = x.new_empty(tuple(shape))
+    z = torch.empty_like(y) if keep_preactivation and act else None
     xp, wp = x2.data_ptr(), w2.data_ptr()
     size = _native._linear_forward_workspace(xp, xs, wp, ws, rows, inner, outer)
-    space = _workspace(size, x.device)
+    space = _workspace(size, x)
     _call(index, _native._linear_forward, xp, xs, wp, ws, _ptr(bias), res, res_stride, _DTYPES[kind], act, rows, inner,
           outer, y.data_ptr(), outer, _ptr(z), _ptr(space), size)
     return y, z
@@ -281,12 +288,12 @@ def linear_backward(dy, x, weight, z=None, *, activation=None, need=(True, True,
         if z is None or z.shape != shape or z.dtype != kind or not z.is_contiguous():
             raise ValueError("z must be what linear_forward kept: y's shape, x's type, contiguous")
         _on(index, z, "z")
-    dx = torch.empty(x.shape, dtype=kind, device=x.device) if need[0] else None
-    dw = torch.empty((outer, inner), dtype=kind, device=x.device) if need[1] else None
-    db = torch.empty(outer, dtype=kind, device=x.device) if need[2] else None
+    dx = _like(x) if need[0] else None
+    dw = _like(weight) if need[1] else None
+    db = x.new_empty((outer,)) if need[2] else None
     xp, wp, dp = x2.data_ptr(), w2.data_ptr(), dy2.data_ptr()
     size = _native._linear_backward_workspace(dp, dys, xp, xs, wp, ws, act, rows, inner, outer)
-    space = _workspace(size, x.device)
+    space = _workspace(size, x)
     _call(index, _native._linear_backward, dp, dys, xp, xs, wp, ws, _ptr(z if act else None), _DTYPES[kind], act, rows,
           inner, outer, _ptr(dx), _ptr(dw), _ptr(db), _ptr(space), size)
     return dx, dw, db
@@ -395,7 +402,7 @@ class RowCache:
         code = _DTYPES.get(dtype)
         if code is None:
             raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
-        out = torch.empty(ids.shape + (self.width,), dtype=dtype, device=self.codes.device)
+        out = self.codes.new_empty((*ids.shape, self.width), dtype=dtype)
         _call(self.index, _native._rows_read, self._native, ids.data_ptr(), bits, ids.numel(), out.data_ptr(),
               self.width, code)
         return out
@@ -453,10 +460,10 @@ def _attend_args(q, ids, keys, values, scale, cap, bias, query_docs, row_docs):
 
 def _attend(q, ids, keys, values, scale, cap, bias, query_docs, row_docs):
     index, args = _attend_args(q, ids, keys, values, scale, cap, bias, query_docs, row_docs)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    out = _like(q)
+    lse = q.new_empty((q.shape[0], q.shape[1]), dtype=torch.float32)
     size = _native._attend_workspace(args)
-    ws = _workspace(size, q.device)
+    ws = _workspace(size, q)
     _call(index, _native._attend, args, keys._native, values._native, out.data_ptr(), lse.data_ptr(), _ptr(ws), size)
     return out, lse
 
@@ -473,10 +480,10 @@ def attend_backward(dout, q, ids, keys, values, lse, *, scale=None, cap=0.0, bia
         raise ValueError("lse must be what attend returned")
     _on(index, dout, "dout")
     _on(index, lse, "lse")
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dbias = None if bias is None else torch.empty(ids.shape, dtype=torch.float32, device=q.device)
+    dq = _like(q)
+    dbias = None if bias is None else q.new_empty(tuple(ids.shape), dtype=torch.float32)
     size = _native._attend_backward_workspace(args, dbias is not None)
-    ws = _workspace(size, q.device)
+    ws = _workspace(size, q)
     _call(index, _native._attend_backward, args, keys._native, values._native, dout.data_ptr(), lse.data_ptr(),
           dq.data_ptr(), _ptr(dbias), _ptr(ws), size)
     return dq, dbias
