@@ -114,11 +114,44 @@ __device__ __forceinline__ float half_at(const void* p, int64_t i, bool f16) {
 // Offset of 16-byte piece `piece` of row `row` in a warp's staging chunk.
 __device__ __forceinline__ uint32_t staged(int row, int piece) { return row * 64 + ((piece ^ (row >> 1)) & 3) * 16; }
 
+// The forms of the two below for rows that start on fewer than 8 bytes.
+__device__ __forceinline__ void chunk_out_any(const uint8_t* stage, uint16_t* out, int64_t stride, int width, int row0,
+                                           int col0, int m, int n, int lane) {
+    // Rows that start anywhere: lanes side by side, a row (or two, by words) at a time.
+    const int per = width == 4 ? 2 : 1, sub = width == 4 ? lane >> 4 : 0, e = width == 4 ? (lane & 15) * 2 : lane;
+    const int col = col0 + e;
+#pragma unroll 8
+    for (int r = sub; r < 32; r += per) {
+        if (row0 + r >= m || col >= n) continue;
+        const uint8_t* src = stage + staged(r, e >> 3) + (e & 7) * 2;
+        uint16_t* dst = out + (int64_t)(row0 + r) * stride + col;
+        if (width == 4 && col + 1 < n) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+        else *dst = *reinterpret_cast<const uint16_t*>(src);
+    }
+}
+__device__ __forceinline__ void chunk_in_any(uint8_t* stage, const uint16_t* in, int64_t stride, int row0, int col0, int m,
+                                          int n, int lane) {
+    // Lanes side by side; eight rows are in flight before the first is stored (more would cost the other forms
+    // registers).
+    const int col = col0 + lane;
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += 8) {
+        uint16_t v[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++)
+            v[r] = row0 + r0 + r < m && col < n ? __ldg(in + (int64_t)(row0 + r0 + r) * stride + col) : (uint16_t)0;
+#pragma unroll
+        for (int r = 0; r < 8; r++)
+            *reinterpret_cast<uint16_t*>(stage + staged(r0 + r, lane >> 3) + (lane & 7) * 2) = v[r];
+    }
+}
+
 // Staging chunk -> 32 rows x 32 columns of p at (row0, col0), clipped to m x
 // n; rows start on `width` bytes (16, 8, 4 or 2).
 __device__ __forceinline__ void chunk_out(const uint8_t* stage, void* p, int64_t stride, int width, int row0, int col0,
                                           int m, int n, int lane) {
     uint16_t* out = static_cast<uint16_t*>(p);
+    if (width < 8) return chunk_out_any(stage, out, stride, width, row0, col0, m, n, lane);
 #pragma unroll
     for (int it = 0; it < 4; it++) {
         const int r = it * 8 + (lane >> 2), piece = lane & 3, col = col0 + piece * 8;
@@ -130,10 +163,6 @@ __device__ __forceinline__ void chunk_out(const uint8_t* stage, void* p, int64_t
         } else if (width == 8 && col + 8 <= n) {
             reinterpret_cast<uint2*>(dst)[0] = make_uint2(v.x, v.y);
             reinterpret_cast<uint2*>(dst)[1] = make_uint2(v.z, v.w);
-        } else if (width >= 4 && col + 8 <= n) {
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) reinterpret_cast<uint32_t*>(dst)[j] = w[j];
         } else {
             const uint16_t* e = reinterpret_cast<const uint16_t*>(&v);
 #pragma unroll
@@ -146,6 +175,7 @@ __device__ __forceinline__ void chunk_out(const uint8_t* stage, void* p, int64_t
 __device__ __forceinline__ void chunk_in(uint8_t* stage, const void* p, int64_t stride, int width, int row0, int col0,
                                          int m, int n, int lane) {
     const uint16_t* in = static_cast<const uint16_t*>(p);
+    if (width < 8) return chunk_in_any(stage, in, stride, row0, col0, m, n, lane);
 #pragma unroll
     for (int it = 0; it < 4; it++) {
         const int r = it * 8 + (lane >> 2), piece = lane & 3, col = col0 + piece * 8;
