@@ -1,0 +1,79 @@
+"""Edges of the operators around the search on the GPU: strides that only the C ABI takes, values at the ends of a type's
+range, gradients through every output, and what a failed call leaves behind."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import memory_plain as plain
+from helpers import capi
+from memory_plain import assert_close, d64
+
+pytestmark = pytest.mark.gpu
+
+memory = pytest.importorskip("winnex_madhava.memory")
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+P, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+
+
+def rand(seed, *shape, kind=F32, scale=1.0, shift=0.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale + shift).to(kind).cuda()
+
+
+def address(t):
+    return P(0 if t is None else t.data_ptr())
+
+
+# ------------------------------------------------------------------ layer norm at strides of the caller's choice
+def with_gap(rows, width, gap, kind, seed=None):
+    """[rows][width + gap] whose gap, and whole where there is no seed, holds 7."""
+    t = torch.full((rows, width + gap), 7.0, dtype=kind, device="cuda")
+    if seed is not None:
+        t[:, :width] = rand(seed, rows, width, kind=kind, scale=1.5, shift=0.3)
+    return t
+
+
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("rows,width", [(5, 256), (3001, 256), (5, 512), (700, 768), (9, 1024), (7, 1536), (6, 2048),
+                                        (3, 8192), (3, 16384), (5, 767), (5, 2047)])
+def test_layer_norm_every_stride_odd(kind, rows, width):
+    """16-bit rows, inputs and outputs all an odd number of elements apart: every element is read, summed and written,
+    the gaps between rows stay as they are."""
+    L = capi()
+    L.mdh_layer_norm_forward.argtypes = [P, i64, i32, P, P, i32, i64, i32, ctypes.c_float, P, i64, P, P, P]
+    L.mdh_layer_norm_backward_workspace.argtypes, L.mdh_layer_norm_backward_workspace.restype = [i64, i32], i64
+    L.mdh_layer_norm_backward.argtypes = [P, i64, P, i64, i32, P, i32, P, P, i64, i32, P, i64, P, P, P, i64, P]
+    code, gap, eps = 1 if kind == BF16 else 2, 1 + width % 2, 1e-5
+    x, dy = with_gap(rows, width, gap, kind, 1), with_gap(rows, width, gap + 2, kind, 2)
+    x[:, width:], dy[:, width:] = math.nan, math.nan          # what lies between rows takes no part
+    w, b = rand(3, width, scale=0.2, shift=1.0), rand(4, width)
+    y, dx = with_gap(rows, width, gap + 4, kind), with_gap(rows, width, gap, kind)
+    mean, rstd = torch.full((rows,), math.nan, device="cuda"), torch.full((rows,), math.nan, device="cuda")
+    stream = P(torch.cuda.current_stream().cuda_stream)
+    assert L.mdh_layer_norm_forward(address(x), x.stride(0), code, address(w), address(b), 0, rows, width, eps, address(y),
+                                    y.stride(0), address(mean), address(rstd), stream) == 0, L.mdh_last_error()
+    x64, w64, dy64 = d64(x[:, :width]), d64(w), d64(dy[:, :width])
+    want, off, m, r, _, _ = plain.norm(x64, w64, d64(b), eps)
+    assert_close(y[:, :width], want, off, "y")
+    n = (width + 8) * plain.U32
+    assert_close(mean, m[:, 0], n * x64.abs().mean(1), "mean")
+    assert_close(rstd, r[:, 0], r[:, 0] * (n + n * x64.abs().mean(1) * r[:, 0]), "rstd")
+    assert (y[:, width:] == 7).all()
+
+    size = L.mdh_layer_norm_backward_workspace(rows, width)
+    grads = plain.norm_grads(dy64, x64, w64, eps)
+    for out in (dx, None):                                    # with the rows' gradient, and the weights' alone
+        ws = torch.full((size // 4,), math.nan, device="cuda")
+        dw, db = torch.full((width,), math.nan, device="cuda"), torch.full((width,), math.nan, device="cuda")
+        assert L.mdh_layer_norm_backward(address(dy), dy.stride(0), address(x), x.stride(0), code, address(w), 0,
+                                         address(mean), address(rstd), rows, width, address(out), dx.stride(0),
+                                         address(dw), address(db), address(ws), size, stream) == 0, L.mdh_last_error()
+        assert_close(dw, *grads[1], "dw")
+        assert_close(db, *grads[2], "db")
+    assert_close(dx[:, :width], *grads[0], "dx")
+    assert (dx[:, width:] == 7).all()
+
+

@@ -58,7 +58,8 @@ __device__ __forceinline__ float weight_at(const void* w, bool w_f32, int c) {
 }
 
 // A thread's places for its shares of the next rows: elements (i * nt + t) * V
-// - shift + 0 .. V - 1 of a row.  Those outside the row are 0.
+// - shift + 0 .. V - 1 of a row.  Those outside the row are 0.  A shifted row
+// takes one place more than it has elements (vector_of sees to it).
 // A ring has four stages, fewer where a block's rows are too large for them:
 // three small blocks share an SM, larger ones have it for themselves.
 constexpr int stages_of(int threads, int bytes) {
@@ -382,8 +383,14 @@ void allow_shared() {
     set.fetch_or(bit, std::memory_order_relaxed);
 }
 
+// Elements of a row that its threads have places for: 8, 16, 24 or 32 a lane
+// of a warp, kBlockElems a thread of a group of whole warps beyond.
+int places_of(int width) { return (int)round_up(width, width <= 1024 ? 256 : 32 * kBlockElems); }
+
 // Elements of a vector: 16 bytes of them, 2 of 16 bits, or 1.  A null
-// array does not count.
+// array does not count.  Rows an odd stride apart begin in the middle of a
+// word every other time, so pairs need a place beside the row's; a row that
+// fills its places goes by single elements (768 of stride 769, 1,024 of 1,025).
 template <class T>
 int vector_of(int width, std::initializer_list<std::pair<const void*, int64_t>> arrays, bool weights_aligned) {
     constexpr int V = 16 / sizeof(T);
@@ -396,6 +403,7 @@ int vector_of(int width, std::initializer_list<std::pair<const void*, int64_t>> 
         words = words && reinterpret_cast<uintptr_t>(p) % 4 == 0 && (parity < 0 || parity == (stride & 1));
         parity = stride & 1;
     }
+    words = words && (parity != 1 || width < places_of(width));
     return whole ? V : words ? 2 : 1;
 }
 template <class T, class F>
