@@ -77,3 +77,21 @@ def test_layer_norm_every_stride_odd(kind, rows, width):
     assert (dx[:, width:] == 7).all()
 
 
+# ------------------------------------------------------------------ linear at the ends of its range
+@pytest.mark.parametrize("name", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_linear_gradients_where_z_leaves_float16(name, rows):
+    """z of -90,000 and 90,000 are infinite in float16; the slopes there are 0 and 1."""
+    x = torch.full((rows, 1), 300.0, dtype=F16, device="cuda")
+    w = torch.tensor([[-300.0], [300.0], [0.25]], dtype=F16, device="cuda")
+    y, z = memory.linear_forward(x, w, activation=name, keep_preactivation=True)
+    assert torch.isneginf(z[:, 0]).all() and torch.isposinf(z[:, 1]).all()
+    assert not y[:, 0].any() and torch.isposinf(y[:, 1]).all()
+    dy = torch.tensor([[0.5, 0.25, 1.0]], dtype=F16, device="cuda").expand(rows, 3).contiguous()
+    dx, dw, db = memory.linear_backward(dy, x, w, z, activation=name)
+    dz = torch.tensor([0.0, 0.25, 1.0], device="cuda")        # 75 is past where either slope differs from 1
+    assert torch.equal(dx.float(), torch.full((rows, 1), 0.25 * 300 + 0.25, device="cuda"))
+    assert torch.equal(dw.float()[:, 0], 300.0 * rows * dz)
+    assert torch.equal(db.float(), rows * dz)
+
+

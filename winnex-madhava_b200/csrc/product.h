@@ -84,7 +84,20 @@ __device__ __forceinline__ f32x2 activate(f32x2 z, int act) {
     }
     return z;
 }
+// Infinities become numbers so large that every slope has its limit there (0
+// times infinity would be NaN); NaN stays.
+__device__ __forceinline__ float bounded(float z) {
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(z), "f"(1e30f));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(z), "f"(-1e30f));
+    return z;
+}
+// act'(z).  z comes as it was kept, in 16 bits: a float16 z is infinite past
+// 65,504, where the value that the forward pass went on with was finite.
 __device__ __forceinline__ f32x2 activation_slope(f32x2 z, int act) {
+    if (act == MDH_ACT_GELU || act == MDH_ACT_SILU) {
+        const float2 f = unpair(z);
+        z = pair(bounded(f.x), bounded(f.y));
+    }
     if (act == MDH_ACT_RELU) {
         const float2 f = unpair(z);
         return pair(f.x > 0.0f ? 1.0f : 0.0f, f.y > 0.0f ? 1.0f : 0.0f);
