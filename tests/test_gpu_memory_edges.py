@@ -95,3 +95,35 @@ def test_linear_gradients_where_z_leaves_float16(name, rows):
     assert torch.equal(db.float(), rows * dz)
 
 
+def gelu_tail(kind, n):
+    """n values of z in [-12, -1], and there in 64 bits: z, z Phi(z), Phi(z) + z phi(z) and the relative error that
+    float32 arithmetic may add to a term.  e^(-z^2 / 2) has that of its argument, a few roundings of z^2 / 2; the rest is
+    held to 2^-18."""
+    z = torch.linspace(-12, -1, n, dtype=torch.float64).to(kind)
+    z64 = z.double()
+    cdf = torch.special.erfc(-z64 / math.sqrt(2)) / 2
+    density = torch.exp(-z64 * z64 / 2) / math.sqrt(2 * math.pi)
+    rel = 2.0 ** -18 + 3 * z64 * z64 * plain.U32
+    return z.cuda(), (z64 * cdf, rel * (z64 * cdf).abs()), (cdf + z64 * density, rel * (cdf + (z64 * density).abs()))
+
+
+@pytest.mark.parametrize("kind", [BF16, F16])
+def test_gelu_tail_by_relative_error(kind):
+    n = 4096
+    z, (want, off), (slope, slope_off) = gelu_tail(kind, n)
+    one = torch.ones(1, 1, dtype=kind, device="cuda")
+    # The tiles, and the gradient: dx is dz, rounded once to the type (the product's one term is exact).
+    y, kept = memory.linear_forward(z[:, None], one, activation="gelu", keep_preactivation=True)
+    assert torch.equal(kept[:, 0], z)
+    assert_close(y[:, 0], want, off, "y")
+    dx, dw, db = memory.linear_backward(torch.ones_like(y), z[:, None], one, kept, activation="gelu")
+    assert_close(dx[:, 0], slope, slope_off, "dx")
+    # A few rows, and a k that is split over blocks.
+    y = memory.linear(one, z[:, None], activation="gelu")
+    assert_close(y[0], want, off, "y of one row")
+    x, w = (torch.zeros(rows, 4096, dtype=kind, device="cuda") for rows in (16, 256))
+    x[:, 70], w[:, 70] = 1, z[::16]
+    y = memory.linear(x, w, activation="gelu")
+    assert_close(y, want[::16].expand(16, 256), off[::16].expand(16, 256), "y of split k")
+
+
