@@ -388,6 +388,19 @@ mdh_status mdh_linear_backward(const void* dy, int64_t dy_stride, const void* x,
                                int32_t inner, int32_t outer, void* dx, void* dw, void* db, void* ws, int64_t ws_bytes,
                                void* stream);
 
+/* The products' waits on the device are bounded.  One that expires voids the
+ * results of its call and is recorded for its device; the next call there that
+ * runs a product (the forward pass of more than 8 rows, the backward pass)
+ * returns MDH_ERR_TIMEOUT once and enqueues nothing.  mdh_linear_status asks
+ * without a call, for the current device: MDH_ERR_TIMEOUT once if a wait
+ * expired since the last report, else MDH_OK.  It does not wait; after the
+ * stream has been waited for it covers the last call and the replays of a
+ * captured graph, which no later call would report.
+ * mdh_linear_set_expired records on the current device what an expired wait
+ * does, for tests. */
+mdh_status mdh_linear_status(void);
+mdh_status mdh_linear_set_expired(void);
+
 /* A cache of 8-bit rows in the caller's memory: codes [slots][width], one
  * byte each, `stride` bytes from row to row.
  *   code 0, int8: `group` (a positive multiple of 16, or 0 for the whole row)

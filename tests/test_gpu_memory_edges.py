@@ -127,3 +127,21 @@ def test_gelu_tail_by_relative_error(kind):
     assert_close(y, want[::16].expand(16, 256), off[::16].expand(16, 256), "y of split k")
 
 
+def test_linear_expired_wait_is_reported_once():
+    """A wait of an earlier product that gave up (its word set from the host) fails the next product, or the call that
+    asks, once; forms without waits go on."""
+    L = capi()
+    x, w = rand(1, 40, 64, kind=BF16), rand(2, 24, 64, kind=BF16)
+    want = memory.linear(x, w)
+    memory.linear_status()
+    for call in (lambda: memory.linear(x, w), lambda: memory.linear_backward(want, x, w), memory.linear_status,
+                 lambda: memory.linear_status("cuda:0")):
+        assert L.mdh_linear_set_expired() == 0, L.mdh_last_error()
+        row = memory.linear(x[:1], w)                          # reads nothing that a wait guards
+        with pytest.raises(RuntimeError, match="expired"):
+            call()
+        memory.linear_status()
+        assert torch.equal(memory.linear(x, w), want) and row.shape == (1, 24)
+    assert L.mdh_linear_status() == 0
+
+

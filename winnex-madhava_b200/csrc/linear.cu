@@ -229,8 +229,7 @@ mdh_status mdh_linear_forward(const void* x, int64_t x_stride, const void* w, in
         current_device();
         if (rows == 0) return;
         MDH_REQUIRE(y, MDH_ERR_INVALID_ARG, "linear: null output");
-        check_product_status();
-        if (rows <= kFewRows) {
+        if (rows <= kFewRows) {  // no waits
             by_half(dtype, [&](auto zero) {
                 using T = decltype(zero);
                 auto run = [&](auto group) {
@@ -248,6 +247,7 @@ mdh_status mdh_linear_forward(const void* x, int64_t x_stride, const void* w, in
         }
         MDH_REQUIRE(enough(ws, ws_bytes, mdh_linear_forward_workspace(x, x_stride, w, w_stride, rows, inner, outer)),
                     MDH_ERR_INVALID_ARG, "linear: workspace too small or not 16-byte aligned");
+        check_product_status();
         ProductEpilogue ep;
         ep.bias = bias;
         ep.residual = residual;
@@ -258,6 +258,14 @@ mdh_status mdh_linear_forward(const void* x, int64_t x_stride, const void* w, in
         ep.z = z_out;
         product({x, x_stride, true}, {w, w_stride, true}, rows, outer, inner, dtype, ep, ws, (cudaStream_t)stream);
     });
+}
+
+mdh_status mdh_linear_status(void) {
+    return guarded([&] { check_product_status(); });
+}
+
+mdh_status mdh_linear_set_expired(void) {
+    return guarded([&] { set_product_expired(); });
 }
 
 int64_t mdh_linear_backward_workspace(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
@@ -283,10 +291,10 @@ mdh_status mdh_linear_backward(const void* dy, int64_t dy_stride, const void* x,
             if (db) MDH_CUDA(cudaMemsetAsync(db, 0, (size_t)outer * 2, st));
             return;
         }
-        check_product_status();
         const BackwardLayout lay = backward_layout(dy, dy_stride, x, x_stride, w, w_stride, activation, rows, inner, outer);
         MDH_REQUIRE(enough(ws, ws_bytes, lay.bytes), MDH_ERR_INVALID_ARG,
                     "linear: workspace too small or not 16-byte aligned");
+        check_product_status();
         char* base = static_cast<char*>(ws);
         by_half(dtype, [&](auto zero) {
             using T = decltype(zero);

@@ -11,7 +11,8 @@
 // two accumulators let an epilogue overlap the next tile's products.  A
 // product with few tiles and a long k is split over k: the parts are written
 // in float32 and joined in order by a second kernel.  Every mbarrier wait is
-// bounded; one that gives up is reported by the next call.  16,384 x 768 x
+// bounded; one that gives up is reported once, by the device's next product or
+// by mdh_linear_status.  16,384 x 768 x
 // 2,048 bf16 on B200: 46-49 us for a gradient's product (1.05-1.1 PFLOP/s; its
 // 384 tiles fill 148 SMs to 86%, and 48 KB of operands a block of k come from
 // L2), 63 us for the forward one with GELU, z and y in its epilogue.
@@ -504,17 +505,19 @@ __global__ void __launch_bounds__(256) k_pack_rows(const __grid_constant__ PackJ
 }
 
 // ------------------------------------------------------------ host
-// The word that a product which gave up a wait writes: pinned host memory.
-int32_t* status_word() {
+// The words that products which gave up a wait write, one a device: pinned
+// host memory.
+constexpr int kDevices = 64;
+int32_t* status_word(int dev) {
     static std::once_flag once;
-    static int32_t* word = nullptr;
+    static int32_t* words = nullptr;
     std::call_once(once, [] {
         int32_t* w = nullptr;
-        MDH_CUDA(cudaHostAlloc((void**)&w, sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped));
-        *w = 0;
-        word = w;
+        MDH_CUDA(cudaHostAlloc((void**)&w, kDevices * sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped));
+        std::fill_n(w, kDevices, 0);
+        words = w;
     });
-    return word;
+    return words + dev % kDevices;
 }
 
 struct Plan {
@@ -609,7 +612,7 @@ int64_t product_workspace(const ProductOperand& a, const ProductOperand& b, int6
 
 void product(const ProductOperand& a0, const ProductOperand& b0, int64_t m, int64_t n, int64_t k, int32_t dtype,
              const ProductEpilogue& ep, void* ws, cudaStream_t st) {
-    const int sms = device_sm_count(current_device());
+    const int dev = current_device(), sms = device_sm_count(dev);
     char* at = static_cast<char*>(ws);
     PackJobs jobs{};
     int n_jobs = 0;
@@ -646,7 +649,7 @@ void product(const ProductOperand& a0, const ProductOperand& b0, int64_t m, int6
     p.b_vec = aligned16(ep.bias);
     p.pitch = round_up(n, 4);
     p.part = p.splits > 1 ? reinterpret_cast<float*>(at) : nullptr;
-    p.status = status_word();
+    p.status = status_word(dev);
     CUtensorMap ta, tb;
     tensor_map(&ta, a, m, k, BM);
     tensor_map(&tb, b, n, k, plan.bn);
@@ -668,9 +671,12 @@ void product(const ProductOperand& a0, const ProductOperand& b0, int64_t m, int6
 }
 
 void check_product_status() {
-    const int32_t s = *reinterpret_cast<volatile int32_t*>(status_word());
-    MDH_REQUIRE(s == 0, MDH_ERR_TIMEOUT, "linear: a device-side wait of an earlier call expired; its results are void");
+    const int32_t s = __atomic_exchange_n(status_word(current_device()), 0, __ATOMIC_ACQ_REL);
+    MDH_REQUIRE(s == 0, MDH_ERR_TIMEOUT,
+                "linear: a device-side wait of an earlier call expired; the results since the last check are void");
 }
+
+void set_product_expired() { __atomic_store_n(status_word(current_device()), (int32_t)kDevTimeout, __ATOMIC_RELEASE); }
 
 }  // namespace op
 }  // namespace mdh

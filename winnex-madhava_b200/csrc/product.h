@@ -32,8 +32,11 @@ int64_t product_workspace(const ProductOperand& a, const ProductOperand& b, int6
 void product(const ProductOperand& a, const ProductOperand& b, int64_t m, int64_t n, int64_t k, int32_t dtype,
              const ProductEpilogue& ep, void* ws, cudaStream_t st);
 
-// Throws MDH_ERR_TIMEOUT when an earlier product gave up one of its waits.
+// Throws MDH_ERR_TIMEOUT when a product on the current device gave up one of its
+// waits since the last call of this.
 void check_product_status();
+// Records what such a product does.
+void set_product_expired();
 
 // 2^x and 1 / x by the hardware (relative errors about 2^-22 and 2^-23).
 __device__ __forceinline__ float fast_exp2(float x) {

@@ -916,6 +916,7 @@ PYBIND11_MODULE(_winnex_madhava, m) {
               check(mdh_linear_backward((void*)dy, dys, (void*)x, xs, (void*)w, wst, (void*)z, dtype, act, rows, inner,
                                         outer, (void*)dx, (void*)dw, (void*)db, (void*)ws, ws_bytes, (void*)stream));
           });
+    m.def("_linear_status", [] { check(mdh_linear_status()); });
     m.def("_rows_write", [](const mdh_rows& c, uintptr_t ids, int32_t bits, uintptr_t rows, int64_t stride,
                             int32_t dtype, int64_t n, uintptr_t stream) {
         check(mdh_rows_write(&c, (void*)ids, bits, (void*)rows, stride, dtype, n, (void*)stream));

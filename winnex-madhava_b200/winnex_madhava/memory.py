@@ -23,7 +23,7 @@ import torch
 from . import _native
 
 __all__ = ["layer_norm", "layer_norm_forward", "layer_norm_backward", "linear", "linear_forward", "linear_backward",
-           "RowCache", "attend", "attend_backward"]
+           "linear_status", "RowCache", "attend", "attend_backward"]
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
@@ -325,6 +325,16 @@ def linear(x, weight, bias=None, *, activation=None, residual=None):
     if _wants_grad(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, activation)
     return linear_forward(x, weight, bias, activation=activation, residual=residual)[0]
+
+
+def linear_status(device=None):
+    """Raises ``RuntimeError``, once, if a device-side wait of an earlier
+    :func:`linear` call on the device (default: the current one) expired: what
+    was computed since the last report is void.  The next call that runs a
+    product says the same; this one covers the last call and the replays of a
+    graph.  It does not wait: synchronise first."""
+    with torch.cuda.device(device):
+        _native._linear_status()
 
 
 # ------------------------------------------------------------------ rows in 8 bits
