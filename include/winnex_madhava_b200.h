@@ -369,7 +369,7 @@ mdh_status mdh_layer_norm_backward(const void* dy, int64_t dy_stride, const void
  * w [outer][inner], bias [outer] (NULL: 0), residual and y [rows][outer], all
  * of type `dtype` (bfloat16 or float16; float32 accumulators).  z_out (NULL
  * allowed, [rows][outer] contiguous) receives z rounded to `dtype`, which the
- * backward pass takes.  GELU is z Phi(z). */
+ * backward pass takes.  GELU is z Phi(z).  rows, inner and outer <= 2^30. */
 int64_t mdh_linear_forward_workspace(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t rows,
                                      int32_t inner, int32_t outer);
 mdh_status mdh_linear_forward(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
@@ -379,7 +379,8 @@ mdh_status mdh_linear_forward(const void* x, int64_t x_stride, const void* w, in
 /* Gradients from dy [rows][outer]: dz = dy act'(z) rounded to `dtype` (the
  * products' operand type), dx = dz w, dw = dz^T x, db = the column sums of dz
  * in float32.  dx, dw and db may be NULL (not formed) and are contiguous;
- * z may be NULL for MDH_ACT_NONE.  The residual's gradient is dy itself. */
+ * z may be NULL for MDH_ACT_NONE.  The residual's gradient is dy itself.
+ * outer <= 65,535 x 256. */
 int64_t mdh_linear_backward_workspace(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
                                       const void* w, int64_t w_stride, int32_t activation, int64_t rows, int32_t inner,
                                       int32_t outer);
@@ -446,7 +447,7 @@ mdh_status mdh_rows_read(const mdh_rows* cache, const void* ids, int32_t id_bits
  * of 8 up to 256; key and value caches have the same slots and width (and
  * may differ in code).  A list stride of 0 gives every query the same list.
  * out and dq are contiguous and 16-byte aligned; the caches' row stride is
- * below 2^31. */
+ * below 2^31, found at most 2^31 - 1025. */
 typedef struct {
     const void* q;          /* [queries][heads][head], strides below, `head` contiguous */
     const int32_t* ids;     /* [queries][found], ids_stride */

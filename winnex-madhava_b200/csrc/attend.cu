@@ -1236,6 +1236,8 @@ AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const 
     const RowsView k = rows_view(keys), v = rows_view(values);
     MDH_REQUIRE(dtype_ok(a->dtype), MDH_ERR_INVALID_ARG, "attend: dtype must be float32, bfloat16 or float16");
     MDH_REQUIRE(a->queries >= 0 && a->found >= 0, MDH_ERR_INVALID_ARG, "attend: queries and found must be >= 0");
+    // Places in a list are 32 bits and run past its end by what a block looks at.
+    MDH_REQUIRE(a->found <= INT32_MAX - kMaxWarps * kRound, MDH_ERR_UNSUPPORTED, "attend: found is limited to 2^31 - 1025");
     MDH_REQUIRE(a->heads >= 1 && a->shared >= 1 && a->heads % a->shared == 0, MDH_ERR_INVALID_ARG,
                 "attend: heads must be a positive multiple of shared");
     MDH_REQUIRE(a->head >= 8 && a->head % 8 == 0 && a->head <= kMaxHead, MDH_ERR_UNSUPPORTED,

@@ -170,7 +170,10 @@ void check_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stri
     MDH_REQUIRE(act >= MDH_ACT_NONE && act <= MDH_ACT_SILU, MDH_ERR_INVALID_ARG, "linear: unknown activation");
     MDH_REQUIRE(rows >= 0 && inner >= 1 && outer >= 1, MDH_ERR_INVALID_ARG,
                 "linear: rows must be >= 0, inner and outer >= 1");
-    MDH_REQUIRE(rows <= INT32_MAX / 2, MDH_ERR_UNSUPPORTED, "linear: rows are limited to 2^30");
+    // Row, column and k indices are 32 bits and run past the size by a tile.
+    constexpr int32_t kMost = 1 << 30;
+    MDH_REQUIRE(rows <= kMost && inner <= kMost && outer <= kMost, MDH_ERR_UNSUPPORTED,
+                "linear: rows, inner and outer are limited to 2^30");
     MDH_REQUIRE(w && (rows == 0 || x), MDH_ERR_INVALID_ARG, "linear: null x or w");
     MDH_REQUIRE((rows <= 1 || x_stride >= inner) && (outer == 1 || w_stride >= inner), MDH_ERR_INVALID_ARG,
                 "linear: row stride below the inner size");
@@ -281,6 +284,8 @@ mdh_status mdh_linear_backward(const void* dy, int64_t dy_stride, const void* x,
                                void* stream) {
     return guarded([&] {
         check_linear(x, x_stride, w, w_stride, dtype, activation, rows, inner, outer);
+        MDH_REQUIRE(ceil_div(outer, 32 * kChunk) <= 65535, MDH_ERR_UNSUPPORTED,
+                    "linear: gradients are limited to an outer size of 65,535 x 256");
         MDH_REQUIRE(rows <= 1 || dy_stride >= outer, MDH_ERR_INVALID_ARG, "linear: row stride below the outer size");
         MDH_REQUIRE(rows == 0 || (dy && (activation == MDH_ACT_NONE || z)), MDH_ERR_INVALID_ARG,
                     "linear: null dy, or no z for the activation's slope");
