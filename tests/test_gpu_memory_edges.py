@@ -145,3 +145,37 @@ def test_linear_expired_wait_is_reported_once():
     assert L.mdh_linear_status() == 0
 
 
+# ------------------------------------------------------------------ attention
+def filled(slots, width, group, code, seed):
+    cache = memory.RowCache.empty(slots, width, code=code, group=group, lo=-2.0, step=4 / 255)
+    cache.write(torch.arange(slots, device="cuda"), rand(seed, slots, width))
+    return cache
+
+
+def held(cache, head):
+    """What the codes stand for in 64 bits (the stored scale is a float32 value)."""
+    c = cache.codes.cpu().double()
+    if cache.scales is None:
+        v = float(torch.tensor(cache.lo)) + float(torch.tensor(cache.step)) * c
+    else:
+        v = c * cache.scales.cpu().double().repeat_interleave(cache.group or cache.width, 1)[:, :cache.width]
+    return v.view(cache.slots, -1, head)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("shared,head", [(1, 64), (4, 32), (8, 64), (2, 96), (4, 128)])
+def test_attend_query_elements_of_any_size(kind, shared, head):
+    """An element of a query counts by its own size, however large another one is: the keys are 0 where the large one is."""
+    slots, found, nq = 60, 200, 3
+    keys, values = filled(slots, 2 * head, 0, "int8", 1), filled(slots, 2 * head, 0, "int8", 2)
+    keys.codes[:, [5, head + 5]] = 0
+    q, dout = rand(3, nq, 2 * shared, head, kind=kind), rand(4, nq, 2 * shared, head, kind=kind)
+    q[..., 5] = 30000.0 if kind == F16 else 2.0 ** 60
+    q[0, ..., 6] = 2.0 ** -20                                  # and small ones stay
+    ids = torch.randint(0, slots, (nq, found), generator=torch.Generator().manual_seed(5), dtype=torch.int32).cuda()
+    out, lse = memory.attend(q, ids, keys, values)
+    want = plain.attend(d64(q), ids.cpu(), held(keys, head), held(values, head), head ** -0.5, 0.0)
+    assert_close(out, *want["out"], "out")
+    assert_close(lse, *want["lse"], "lse")
+
+

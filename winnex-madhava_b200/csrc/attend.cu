@@ -37,6 +37,7 @@
 // the query's elements, or of the weights.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "op_rows.cuh"
 
@@ -653,14 +654,16 @@ __global__ void __launch_bounds__(32 * kMaxWarps, RB == 1 ? 3 : 2) k_attend(cons
 // products (mma.sync m16n8k16, float32 sums): a warp holds one unit, up to 8
 // heads, and 16 entries at a time.
 //
-// Scores: A rows 0-7 are the heads' queries rounded to float16 (scaled by a
-// power of two to use its range), rows 8-15 what the rounding left, so their
-// sum carries 22 bits; B are the key codes, exact in float16, as bytes of
-// 1024 + (c + 128) less 1152.  Values: A are the value codes with dimensions
-// as rows, exact in bfloat16 (a byte's low 7 bits over 128 less 128 or 256,
-// its top bit), B the weights p times the row's scale as three bfloat16 parts:
-// 24 bits at any size, since a weight may count where the larger ones' values
-// are 0.  A lane finds its codes as 32-bit words: which
+// Scores: A rows 0-7 are the heads' queries and B the key codes, exact in
+// float16 (bytes of 1024 + (c + 128) less 1152) and in bfloat16 (a byte's low 7
+// bits over 128 less 128 or 256, its top bit).  16-bit queries are taken in
+// their own type, float32 ones as three bfloat16 parts (rows 8-15 hold the
+// second and, in a product of their own, the third): all their bits at any
+// size, since an element may count where larger ones meet keys of 0.  Values: A
+// are the value codes with dimensions as rows, in bfloat16, B the weights p
+// times the row's scale as three bfloat16 parts: 24 bits at any size, since a
+// weight may count where the larger ones' values are 0.  A lane finds its codes
+// as 32-bit words: which
 // dimension a word's bytes stand for is the same on both sides of a product,
 // so no byte moves between lanes.  Each entry's head lies in shared memory
 // 16 bytes past a multiple of the bank width, so those words hit all banks.
@@ -712,21 +715,53 @@ __device__ __forceinline__ uint32_t half_codes(uint32_t w, bool high) {
     const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&x), off);
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Two floats as float16 and what is left of them.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-}
-// The power of two at x > 0 or just below; 1 where x is 0 or not finite.
-__device__ __forceinline__ float power_of_two(float x) {
-    const uint32_t e = __float_as_uint(x) & 0x7f800000u;
-    return e == 0 || e == 0x7f800000u ? 1.0f : __uint_as_float(e);
-}
+// Four elements of a query as A's registers: of its own 16-bit type two, of
+// float32 three bfloat16 parts of two each, cut off rather than rounded (no part
+// leaves the float range).  An infinity is its first part.
+template <class Q>
+struct Query {
+    static constexpr int REGS = sizeof(Q) == 2 ? 2 : 6;
+    static constexpr bool BF16_CODES = !std::is_same<Q, f16>::value;
+    static __device__ __forceinline__ void set(const float (&x)[4], uint32_t (&r)[REGS]) {
+        if constexpr (std::is_same<Q, f16>::value) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+                r[j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        } else {
+            float v[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+            for (int k = 0; k < REGS / 2; k++) {
+                uint32_t top[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    top[j] = __float_as_uint(v[j]);
+                    if (REGS > 2) v[j] = fabsf(v[j]) == INFINITY ? 0.0f : v[j] - __uint_as_float(top[j] & 0xffff0000u);
+                }
+                r[2 * k] = __byte_perm(top[0], top[1], 0x7632);
+                r[2 * k + 1] = __byte_perm(top[2], top[3], 0x7632);
+            }
+        }
+    }
+    // d += 16 dimensions' products with the codes of `word` (bytes c + 128, or c for bfloat16).
+    static __device__ __forceinline__ void dot(float (&d)[4], const uint32_t (&r)[REGS], uint32_t word) {
+        if constexpr (std::is_same<Q, f16>::value) {
+            mma16816(d, {r[0], 0u, r[1], 0u}, half_codes(word, false), half_codes(word, true));
+        } else {
+            const uint32_t low = word & 0x7f7f7f7fu, top = word & 0x80808080u;
+            const uint32_t b0 = bf16_codes(low, top, false), b1 = bf16_codes(low, top, true);
+            if constexpr (REGS == 2) {
+                mma16816_bf16(d, {r[0], 0u, r[1], 0u}, b0, b1);
+            } else {
+                mma16816_bf16(d, {0u, r[4], 0u, r[5]}, b0, b1);
+                mma16816_bf16(d, {r[0], r[2], r[1], r[3]}, b0, b1);
+            }
+        }
+    }
+};
 
-template <int NS>
+template <int NS, class Q>
 __global__ void __launch_bounds__(32 * kMaxWarps, NS > 4 ? 1 : 2) k_attend_mma(const __grid_constant__ AttendParams a) {
     using M = Mma<NS>;
     extern __shared__ uint8_t sm[];  // the warps' rings, later the vectors to join; then the entries
@@ -740,34 +775,19 @@ __global__ void __launch_bounds__(32 * kMaxWarps, NS > 4 ? 1 : 2) k_attend_mma(c
     const bool mine = g < w.nr;  // this lane's score rows are a head
 
     // Queries: head g, dimensions 16 s + 4 c + 0 .. 3.
-    uint32_t q[NS][4];
-    float unscale, kb;
-    {
-        float x[NS][4], top = 0.0f, sum = 0.0f;
+    uint32_t q[NS][Query<Q>::REGS];
+    float kb = 0.0f;
 #pragma unroll
-        for (int s = 0; s < NS; s++) {
-            if (mine) load4(a.q, w.i * a.q_stride + (w.h0 + g) * a.q_head_stride + 16 * s + 4 * c, a.dtype, a.q_vec, x[s]);
-            else x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.0f;
+    for (int s = 0; s < NS; s++) {
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (mine) load4(a.q, w.i * a.q_stride + (w.h0 + g) * a.q_head_stride + 16 * s + 4 * c, a.dtype, a.q_vec, x);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                top = fmaxf(top, fabsf(x[s][j]));
-                sum += x[s][j];
-            }
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        }
-        const float unit = power_of_two(fmaxf(top, 0x1p-100f)), up = 1024.0f / unit;  // the largest lies in [1024, 2048)
-#pragma unroll
-        for (int s = 0; s < NS; s++) {
-            split2(x[s][0] * up, x[s][1] * up, q[s][0], q[s][1]);
-            split2(x[s][2] * up, x[s][3] * up, q[s][2], q[s][3]);
-        }
-        unscale = a.scale * unit * (1.0f / 1024.0f);
-        kb = a.scale * a.k.base * sum;
+        for (int j = 0; j < 4; j++) kb += x[j];
+        Query<Q>::set(x, q[s]);
     }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) kb += __shfl_xor_sync(0xffffffffu, kb, o);
+    kb *= a.scale * a.k.base;
     float acc[NS][4];  // dimensions x heads 2 c, 2 c + 1
 #pragma unroll
     for (int t = 0; t < NS; t++)
@@ -797,7 +817,8 @@ __global__ void __launch_bounds__(32 * kMaxWarps, NS > 4 ? 1 : 2) k_attend_mma(c
         copy_commit();
     };
 
-    const uint32_t v_flip = a.v.flip ^ 0x80808080u;  // bytes c here, c + 128 with the keys
+    // Bytes c for bfloat16, c + 128 for float16.
+    const uint32_t k_flip = Query<Q>::BF16_CODES ? a.k.flip ^ 0x80808080u : a.k.flip, v_flip = a.v.flip ^ 0x80808080u;
     const int32_t doc = a.query_docs ? a.query_docs[w.i] : 0;
     const int j0 = (int)min((int64_t)blockIdx.y * a.split_len, (int64_t)a.found);
     const int j1 = (int)min((int64_t)j0 + a.split_len, (int64_t)a.found);
@@ -824,17 +845,14 @@ __global__ void __launch_bounds__(32 * kMaxWarps, NS > 4 ? 1 : 2) k_attend_mma(c
                 float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 const uint32_t* row = reinterpret_cast<const uint32_t*>(at + (8 * n + g) * M::ROW);
 #pragma unroll
-                for (int s = 0; s < NS; s++) {
-                    const uint32_t word = row[4 * s + c] ^ a.k.flip;
-                    mma16816(d, q[s], half_codes(word, false), half_codes(word, true));
-                }
+                for (int s = 0; s < NS; s++) Query<Q>::dot(d, q[s], row[4 * s + c] ^ k_flip);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     const int e = 8 * n + 2 * c + j;
-                    const float ks = ksp ? scales[e] : a.k.scale;
+                    const float ks = ksp ? scales[e] : a.k.scale, dot = Query<Q>::REGS > 2 ? d[j] + d[2 + j] : d[j];
                     float th;
-                    p[2 * n + j] = t + e < hi ? score_of(a, fmaf((d[j] + d[2 + j]) * unscale, ks, kb), list.bias[t + e], th)
-                                              : -INFINITY;
+                    p[2 * n + j] =
+                        t + e < hi ? score_of(a, fmaf(dot * a.scale, ks, kb), list.bias[t + e], th) : -INFINITY;
                 }
             }
             float top = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
@@ -1361,12 +1379,15 @@ void launch_lanes(const AttendParams& p, cudaStream_t st) {
     else launch_warps<k_attend<LANES, RB, ALIGNED>, kWarpBytes, kMaxWarps>(p, st);
 }
 void launch_mma(const AttendParams& p, cudaStream_t st) {
-    switch (p.head) {
-        case 32: launch_warps<k_attend_mma<2>, Mma<2>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
-        case 64: launch_warps<k_attend_mma<4>, Mma<4>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
-        case 96: launch_warps<k_attend_mma<6>, Mma<6>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
-        default: launch_warps<k_attend_mma<8>, Mma<8>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
-    }
+    by_dtype(p.dtype, [&](auto zero) {
+        using Q = decltype(zero);
+        switch (p.head) {
+            case 32: launch_warps<k_attend_mma<2, Q>, Mma<2>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
+            case 64: launch_warps<k_attend_mma<4, Q>, Mma<4>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
+            case 96: launch_warps<k_attend_mma<6, Q>, Mma<6>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
+            default: launch_warps<k_attend_mma<8, Q>, Mma<8>::RING + kEntriesBytes, kMaxWarps>(p, st); break;
+        }
+    });
 }
 
 }  // namespace
