@@ -470,6 +470,13 @@ int64_t mdh_attend_backward_workspace(const mdh_attend_args* a, int32_t want_dbi
 mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values,
                                const void* dout, const float* lse, void* dq, float* dbias, void* ws, int64_t ws_bytes,
                                void* stream);
+/* The same where lse takes part in what is differentiated, as it does where
+ * this attention was joined with another's: dlse (float32 [queries][heads],
+ * NULL: zeros) is its gradient.  lse is always the forward call's own, never
+ * the joined one.  A query without an entry has no gradient whatever its dlse. */
+mdh_status mdh_attend_backward_lse(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values,
+                                   const void* dout, const float* lse, const float* dlse, void* dq, float* dbias,
+                                   void* ws, int64_t ws_bytes, void* stream);
 
 /* Options (process-wide): force the scan path for testing and measurement.
  * path: 0 = automatic, 1 = CUDA-core scan only, 2 = tensor-core scan on

@@ -179,3 +179,81 @@ def test_attend_query_elements_of_any_size(kind, shared, head):
     assert_close(lse, *want["lse"], "lse")
 
 
+def slopes64(q, ids, keys, values, bias, cap, dout, dlse):
+    """dq and dbias in 64 bits by differentiation of the 64-bit form."""
+    head = q.shape[2]
+    q64, b64 = d64(q).requires_grad_(), d64(bias).requires_grad_()
+    r = plain.attend(q64, ids.cpu(), held(keys, head), held(values, head), head ** -0.5, cap, b64)
+    loss = (r["lse"][0] * d64(dlse)).sum()
+    if dout is not None:
+        loss = loss + (r["out"][0] * d64(dout)).sum()
+    return torch.autograd.grad(loss, (q64, b64))
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("nq,found,groups,shared,head", [(3, 20, 2, 3, 64), (2, 1500, 2, 4, 32), (40, 64, 3, 1, 40)])
+@pytest.mark.parametrize("through_out", [True, False])
+def test_attend_gradient_through_lse(kind, nq, found, groups, shared, head, through_out):
+    """A loss of out and lse, and of lse alone."""
+    slots, cap = 300, 3.0
+    keys, values = (filled(slots, groups * head, 0, "int8", s) for s in (1, 2))
+    q, bias = rand(3, nq, groups * shared, head, kind=kind), -torch.rand(nq, found, generator=torch.Generator().manual_seed(4)).cuda()
+    ids = torch.randint(-3, slots, (nq, found), generator=torch.Generator().manual_seed(5), dtype=torch.int32).cuda()
+    dlse = rand(6, nq, groups * shared)
+    dout = rand(7, nq, groups * shared, head, kind=kind) if through_out else None
+    q.requires_grad_(), bias.requires_grad_()
+    out, lse = memory.attend(q, ids, keys, values, cap=cap, bias=bias)
+    loss = (lse * dlse).sum() + (0 if dout is None else (out.float() * dout.float()).sum())
+    loss.backward()
+    dq, dbias = slopes64(q, ids, keys, values, bias, cap, dout, dlse)
+    # The bounds for dout alone, and dlse as what it is beside dP: a number of its own size for each entry.
+    dp = dlse[..., None].expand(nq, groups * shared, head) / head
+    room = plain.attend(d64(q), ids.cpu(), held(keys, head), held(values, head).abs() + 1, head ** -0.5, cap, d64(bias),
+                        dout=(0 if dout is None else d64(dout).abs()) + d64(dp).abs())
+    assert_close(q.grad, dq, 4 * room["dq"][1], "dq")
+    assert_close(bias.grad, dbias, 4 * room["dbias"][1], "dbias")
+
+
+def test_attend_joined_by_lse_trains_as_one():
+    """Two parts of a list joined by their lse inside autograd give the gradients of the whole list, empty parts included."""
+    head, slots, nq = 64, 80, 6
+    keys, values = filled(slots, 2 * head, 64, "int8", 1), filled(slots, 2 * head, 64, "int8", 2)
+    ids = torch.randint(0, slots, (nq, 24), generator=torch.Generator().manual_seed(5), dtype=torch.int32).cuda()
+    ids[1, :9] = -1
+    ids[2, 9:] = -1
+    dout = rand(4, nq, 2, head)
+    grads = []
+    for parts in ([ids], [ids[:, :9], ids[:, 9:]]):
+        q = rand(3, nq, 2, head).requires_grad_()
+        done = [memory.attend(q, part, keys, values) for part in parts]
+        weight = torch.softmax(torch.stack([lse for _, lse in done]), 0)
+        sum(w[..., None] * o for w, (o, _) in zip(weight, done)).backward(dout)
+        grads.append(d64(q.grad))
+    want = plain.attend(d64(rand(3, nq, 2, head)), ids.cpu(), held(keys, head), held(values, head), head ** -0.5, 0.0,
+                        dout=d64(dout))["dq"]
+    for g in grads:
+        assert ((g - want[0]).abs() <= 8 * want[1] + plain.U32 * want[0].abs()).all()
+
+
+def test_attend_lse_gradient_of_empty_lists():
+    """No entry, no gradient, whatever comes back for an lse of -infinity."""
+    keys, values = filled(10, 64, 64, "int8", 1), filled(10, 64, 64, "int8", 2)
+    q, dout = rand(1, 3, 2, 32), rand(2, 3, 2, 32)
+    ids = torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+    ids[2] = 5
+    bias = torch.zeros(3, 4, device="cuda")
+    _, lse = memory.attend(q, ids, keys, values, bias=bias)
+    dlse = torch.tensor([[math.nan, math.inf], [-math.inf, 3.0], [0.5, 0.5]], device="cuda")
+    dq, dbias = memory.attend_backward(dout, q, ids, keys, values, lse, bias=bias, dlse=dlse)
+    assert not dq[:2].any() and not dbias[:2].any() and torch.isfinite(dq).all() and dq[2].any()
+
+
+def test_attend_refuses_another_shape_of_dlse():
+    keys = filled(10, 64, 64, "int8", 1)
+    q, ids = rand(1, 3, 2, 32), torch.zeros(3, 4, dtype=torch.int32, device="cuda")
+    _, lse = memory.attend(q, ids, keys, keys)
+    for bad in (lse[:2], lse.double(), lse.t().contiguous().t(), lse.cpu()):
+        with pytest.raises(ValueError, match="dlse"):
+            memory.attend_backward(q, q, ids, keys, keys, lse, dlse=bad)
+
+

@@ -8,7 +8,8 @@
 //   dbias_j = sum over heads of p_j (dP_j - D)
 //   dq = scale sum_j p_j (dP_j - D) (1 - t_j^2) k_j = scale (A - D B),
 //   A = sum_j p_j dP_j (1 - t_j^2) k_j,  B = sum_j p_j (1 - t_j^2) k_j:
-// one pass over the rows as well, since p_j follows from lse.
+// one pass over the rows as well, since p_j follows from lse.  A gradient of
+// lse itself adds p_j dlse to each score's: D - dlse stands for D.
 //
 // A unit is a head of the rows and up to kMaxShared query heads that share it.
 // LANES lanes hold a row's head, 8 elements each (an 8-byte load of codes); the
@@ -92,8 +93,9 @@ struct AttendParams {
     // backward
     const void* dout;
     const float* lse_in;
+    const float* dlse;     // or null
     float2* pd;            // [queries][heads][found] p dP and p, or null
-    float2* sum_d;         // [queries][heads] D / P and 1 / P, or null
+    float2* sum_d;         // [queries][heads] D / P - dlse and 1 / P, or null
 };
 
 using u64 = f32x2;
@@ -446,6 +448,7 @@ __device__ __forceinline__ void finish_backward(const AttendParams& a, int64_t a
                                                 const float (&y)[8], float sum_d, float sum_p) {
     const float inv = sum_p != 0.0f ? 1.0f / sum_p : 0.0f, f = a.scale * inv;
     sum_d *= inv;
+    if (a.dlse && sum_p != 0.0f) sum_d -= __ldg(a.dlse + at);  // a list without entries has no gradient
 #pragma unroll
     for (int j = 0; j < 8; j++) x[j] = f * (x[j] - sum_d * y[j]);
     store_elements(a.out, at * a.head + d, a.dtype, x);
@@ -1182,7 +1185,7 @@ __global__ void __launch_bounds__(128) k_attend_backward_join(const __grid_const
     if (d0 < a.head) finish_backward(a, at, d0, x, y, d, p);
 }
 
-// dbias[i][j] = sum over heads of (p dP - p D / P) / P, in head order; 0 at hidden entries.
+// dbias[i][j] = sum over heads of (p dP - p (D / P - dlse)) / P, in head order; 0 at hidden entries.
 __global__ void __launch_bounds__(256) k_attend_dbias(const __grid_constant__ AttendParams a, float* __restrict__ dbias) {
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (at >= a.queries * a.found) return;
@@ -1437,6 +1440,12 @@ int64_t mdh_attend_backward_workspace(const mdh_attend_args* a, int32_t want_dbi
 mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values,
                                const void* dout, const float* lse, void* dq, float* dbias, void* ws, int64_t ws_bytes,
                                void* stream) {
+    return mdh_attend_backward_lse(a, keys, values, dout, lse, nullptr, dq, dbias, ws, ws_bytes, stream);
+}
+
+mdh_status mdh_attend_backward_lse(const mdh_attend_args* a, const mdh_rows* keys, const mdh_rows* values,
+                                   const void* dout, const float* lse, const float* dlse, void* dq, float* dbias,
+                                   void* ws, int64_t ws_bytes, void* stream) {
     return guarded([&] {
         AttendParams p = check_attend(a, keys, values, false);
         current_device();
@@ -1460,6 +1469,7 @@ mdh_status mdh_attend_backward(const mdh_attend_args* a, const mdh_rows* keys, c
         p.dout = dout;
         p.dout_vec = aligned16(dout) && a->head * dtype_size(a->dtype) % 16 == 0;
         p.lse_in = lse;
+        p.dlse = dlse;
         by_shape(p, [&](auto lanes, auto rb, auto aligned) {
             launch_lanes<lanes, rb, aligned, true>(p, st);
         });

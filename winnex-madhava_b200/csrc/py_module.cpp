@@ -945,8 +945,8 @@ PYBIND11_MODULE(_winnex_madhava, m) {
           [](const mdh_attend_args& a, bool want) { return mdh_attend_backward_workspace(&a, want ? 1 : 0); });
     m.def("_attend_backward",
           [](const mdh_attend_args& a, const mdh_rows& keys, const mdh_rows& values, uintptr_t dout, uintptr_t lse,
-             uintptr_t dq, uintptr_t dbias, uintptr_t ws, int64_t ws_bytes, uintptr_t stream) {
-              check(mdh_attend_backward(&a, &keys, &values, (void*)dout, (float*)lse, (void*)dq, (float*)dbias,
-                                        (void*)ws, ws_bytes, (void*)stream));
+             uintptr_t dlse, uintptr_t dq, uintptr_t dbias, uintptr_t ws, int64_t ws_bytes, uintptr_t stream) {
+              check(mdh_attend_backward_lse(&a, &keys, &values, (void*)dout, (float*)lse, (float*)dlse, (void*)dq,
+                                            (float*)dbias, (void*)ws, ws_bytes, (void*)stream));
           });
 }

@@ -479,10 +479,11 @@ def _attend(q, ids, keys, values, scale, cap, bias, query_docs, row_docs):
 
 
 def attend_backward(dout, q, ids, keys, values, lse, *, scale=None, cap=0.0, bias=None, query_docs=None,
-                    row_docs=None):
+                    row_docs=None, dlse=None):
     """``(dq, dbias)`` of :func:`attend` from the gradient of its output and
-    its lse; dbias (float32, summed over the heads) is None without a bias.
-    The caches are constants."""
+    its own lse (never one joined with another attention's); dlse is the
+    gradient of lse where that took part too.  dbias (float32, summed over the
+    heads) is None without a bias.  The caches are constants."""
     index, args = _attend_args(q, ids, keys, values, scale, cap, bias, query_docs, row_docs)
     if dout.shape != q.shape or dout.dtype != q.dtype or not dout.is_contiguous():
         raise ValueError("dout must be contiguous, of q's shape and type")
@@ -490,12 +491,16 @@ def attend_backward(dout, q, ids, keys, values, lse, *, scale=None, cap=0.0, bia
         raise ValueError("lse must be what attend returned")
     _on(index, dout, "dout")
     _on(index, lse, "lse")
+    if dlse is not None:
+        if dlse.shape != lse.shape or dlse.dtype != torch.float32 or not dlse.is_contiguous():
+            raise ValueError("dlse must be contiguous float32 of lse's shape")
+        _on(index, dlse, "dlse")
     dq = _like(q)
     dbias = None if bias is None else q.new_empty(tuple(ids.shape), dtype=torch.float32)
     size = _native._attend_backward_workspace(args, dbias is not None)
     ws = _workspace(size, q)
     _call(index, _native._attend_backward, args, keys._native, values._native, dout.data_ptr(), lse.data_ptr(),
-          dq.data_ptr(), _ptr(dbias), _ptr(ws), size)
+          _ptr(dlse), dq.data_ptr(), _ptr(dbias), _ptr(ws), size)
     return dq, dbias
 
 
@@ -505,16 +510,18 @@ class _Attend(torch.autograd.Function):
         out, lse = _attend(q, ids, keys, values, scale, cap, bias, query_docs, row_docs)
         ctx.save_for_backward(q, bias, ids, lse, query_docs, row_docs)
         ctx.rest = (keys, values, scale, cap)
-        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)  # a loss mostly leaves lse out
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, _):
+    def backward(ctx, dout, dlse):
         q, bias, ids, lse, query_docs, row_docs = ctx.saved_tensors
         keys, values, scale, cap = ctx.rest
-        dq, dbias = attend_backward(dout.contiguous(), q, ids, keys, values, lse, scale=scale, cap=cap, bias=bias,
-                                    query_docs=query_docs, row_docs=row_docs)
+        dout = q.new_zeros(tuple(q.shape)) if dout is None else dout.contiguous()
+        dlse = None if dlse is None else dlse.contiguous()
+        dq, dbias = attend_backward(dout, q, ids, keys, values, lse, scale=scale, cap=cap, bias=bias,
+                                    query_docs=query_docs, row_docs=row_docs, dlse=dlse)
         return (dq, dbias) + (None,) * 7
 
 
@@ -529,9 +536,9 @@ def attend(q, ids, keys, values, *, scale=None, cap=0.0, bias=None, query_docs=N
     hidden where its id is outside the cache, its bias is -infinity, or
     ``row_docs[id] != query_docs[query]``.  A query whose entries are all
     hidden gives zeros and an lse of -infinity.  lse [queries, heads] joins
-    this attention with another over other rows.  ``out`` is differentiable
-    in q and bias; lse and the caches are constants, and rows that a query
-    read must not be rewritten before its backward pass."""
+    this attention with another over other rows.  Both are differentiable in q
+    and bias; the caches are constants, and rows that a query read must not be
+    rewritten before its backward pass."""
     if _wants_grad(q, bias):
         return _Attend.apply(q, bias, ids, keys, values, scale, cap, query_docs, row_docs)
     return _attend(q, ids, keys, values, scale, cap, bias, query_docs, row_docs)
