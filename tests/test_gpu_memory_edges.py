@@ -257,3 +257,29 @@ def test_attend_refuses_another_shape_of_dlse():
             memory.attend_backward(q, q, ids, keys, keys, lse, dlse=bad)
 
 
+# ------------------------------------------------------------------ gradients that nobody asked for
+def spied(monkeypatch, name):
+    """Records the arguments of a native call."""
+    calls, real = [], getattr(memory._native, name)
+    monkeypatch.setattr(memory._native, name, lambda *a: (calls.append(a), real(*a))[1])
+    return calls
+
+
+def test_layer_norm_forms_what_is_needed(monkeypatch):
+    x, w, b = rand(1, 50, 96, kind=BF16), rand(2, 96), rand(3, 96)
+    dy = rand(4, 50, 96, kind=BF16)
+    y, mean, rstd = memory.layer_norm_forward(x, w, b)
+    full = memory.layer_norm_backward(dy, x, w, mean, rstd)
+    calls = spied(monkeypatch, "_layer_norm_backward")
+    for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True), (True, True, True)):
+        some = memory.layer_norm_backward(dy, x, w, mean, rstd, need=need)
+        leaves = [t.clone().requires_grad_(n) for t, n in zip((x, w, b), need)]
+        memory.layer_norm(*leaves).backward(dy)
+        for n, s, f, leaf in zip(need, some, full, leaves):
+            assert torch.equal(s, f) and torch.equal(leaf.grad, f) if n else s is None and leaf.grad is None
+        for args in calls:
+            assert [args[k] != 0 for k in (11, 13, 14)] == list(need)
+            assert (args[15] != 0) == (need[1] or need[2])     # scratch only where sums are formed
+        calls.clear()
+
+

@@ -147,11 +147,12 @@ def layer_norm_forward(x, weight=None, bias=None, *, eps=1e-5):
     return _norm_forward(x, weight, bias, eps, True)
 
 
-def layer_norm_backward(dy, x, weight, mean, rstd, *, weight_dtype=None):
+def layer_norm_backward(dy, x, weight, mean, rstd, *, weight_dtype=None, need=(True, True, True)):
     """``(dx, dweight, dbias)`` of :func:`layer_norm` from the gradient of y.
 
     dweight and dbias have the weight's type (``weight_dtype`` where there is
-    no weight; default x's type)."""
+    no weight; default x's type).  ``need`` says which of the three to form;
+    the others are None."""
     index = _device(x, "x")
     code = _dtype(x, "x")
     if dy.shape != x.shape or dy.dtype != x.dtype:
@@ -170,14 +171,14 @@ def layer_norm_backward(dy, x, weight, mean, rstd, *, weight_dtype=None):
         _require(t.dtype == torch.float32, f"{name} must be float32")
         _on(index, t, name)
     _on(index, dy, "dy")
-    dx = _like(x)
-    dw = x.new_empty((width,), dtype=kind)
-    db = torch.empty_like(dw)
-    size = _native._layer_norm_backward_workspace(rows, width)
+    dx = _like(x) if need[0] else None
+    dw = x.new_empty((width,), dtype=kind) if need[1] else None
+    db = x.new_empty((width,), dtype=kind) if need[2] else None
+    size = _native._layer_norm_backward_workspace(rows, width) if need[1] or need[2] else 0
     ws = _workspace(size, x)
     _call(index, _native._layer_norm_backward, dy2.data_ptr(), dy_stride, x2.data_ptr(), stride, code, _ptr(weight),
-          _DTYPES[kind], mean.data_ptr(), rstd.data_ptr(), rows, width, dx.data_ptr(), width, dw.data_ptr(),
-          db.data_ptr(), _ptr(ws), size)
+          _DTYPES[kind], mean.data_ptr(), rstd.data_ptr(), rows, width, _ptr(dx), width, _ptr(dw),
+          _ptr(db), _ptr(ws), size)
     return dx, dw, db
 
 
@@ -193,9 +194,8 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
-        dx, dw, db = layer_norm_backward(dy.contiguous(), x, weight, mean, rstd, weight_dtype=ctx.kind)
-        need = ctx.needs_input_grad
-        return dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None
+        return (*layer_norm_backward(dy.contiguous(), x, weight, mean, rstd, weight_dtype=ctx.kind,
+                                     need=ctx.needs_input_grad[:3]), None)
 
 
 def _wants_grad(*tensors):
