@@ -283,3 +283,20 @@ def test_layer_norm_forms_what_is_needed(monkeypatch):
         calls.clear()
 
 
+def test_attend_forms_the_bias_gradient_where_it_is_needed(monkeypatch):
+    keys, values = filled(50, 64, 64, "int8", 1), filled(50, 64, 64, "int8", 2)
+    q, ids = rand(3, 4, 2, 32), torch.randint(0, 50, (4, 9), generator=torch.Generator().manual_seed(5), dtype=torch.int32).cuda()
+    bias, dout = rand(4, 4, 9), rand(6, 4, 2, 32)
+    out, lse = memory.attend(q, ids, keys, values, bias=bias)
+    dq, dbias = memory.attend_backward(dout, q, ids, keys, values, lse, bias=bias)
+    calls = spied(monkeypatch, "_attend_backward")
+    alone, none = memory.attend_backward(dout, q, ids, keys, values, lse, bias=bias, need=(True, False))
+    assert torch.equal(alone, dq) and none is None
+    none, alone = memory.attend_backward(dout, q, ids, keys, values, lse, bias=bias, need=(False, True))
+    assert none is None and torch.equal(alone, dbias)
+    q2 = q.clone().requires_grad_()
+    memory.attend(q2, ids, keys, values, bias=bias)[0].backward(dout)
+    assert torch.equal(q2.grad, dq)
+    assert [[a[k] != 0 for k in (6, 7)] for a in calls] == [[True, False], [True, True], [True, False]]
+
+

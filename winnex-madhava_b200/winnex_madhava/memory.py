@@ -479,11 +479,13 @@ def _attend(q, ids, keys, values, scale, cap, bias, query_docs, row_docs):
 
 
 def attend_backward(dout, q, ids, keys, values, lse, *, scale=None, cap=0.0, bias=None, query_docs=None,
-                    row_docs=None, dlse=None):
+                    row_docs=None, dlse=None, need=(True, True)):
     """``(dq, dbias)`` of :func:`attend` from the gradient of its output and
     its own lse (never one joined with another attention's); dlse is the
     gradient of lse where that took part too.  dbias (float32, summed over the
-    heads) is None without a bias.  The caches are constants."""
+    heads) is None without a bias.  The caches are constants.  ``need`` says
+    which of the two to give; the other is None.  dbias takes 8 bytes of scratch
+    for each query, head and entry (4 GB for 8,192 x 16 x 4,096)."""
     index, args = _attend_args(q, ids, keys, values, scale, cap, bias, query_docs, row_docs)
     if dout.shape != q.shape or dout.dtype != q.dtype or not dout.is_contiguous():
         raise ValueError("dout must be contiguous, of q's shape and type")
@@ -496,12 +498,12 @@ def attend_backward(dout, q, ids, keys, values, lse, *, scale=None, cap=0.0, bia
             raise ValueError("dlse must be contiguous float32 of lse's shape")
         _on(index, dlse, "dlse")
     dq = _like(q)
-    dbias = None if bias is None else q.new_empty(tuple(ids.shape), dtype=torch.float32)
+    dbias = q.new_empty(tuple(ids.shape), dtype=torch.float32) if bias is not None and need[1] else None
     size = _native._attend_backward_workspace(args, dbias is not None)
     ws = _workspace(size, q)
     _call(index, _native._attend_backward, args, keys._native, values._native, dout.data_ptr(), lse.data_ptr(),
           _ptr(dlse), dq.data_ptr(), _ptr(dbias), _ptr(ws), size)
-    return dq, dbias
+    return dq if need[0] else None, dbias
 
 
 class _Attend(torch.autograd.Function):
@@ -521,7 +523,7 @@ class _Attend(torch.autograd.Function):
         dout = q.new_zeros(tuple(q.shape)) if dout is None else dout.contiguous()
         dlse = None if dlse is None else dlse.contiguous()
         dq, dbias = attend_backward(dout, q, ids, keys, values, lse, scale=scale, cap=cap, bias=bias,
-                                    query_docs=query_docs, row_docs=row_docs, dlse=dlse)
+                                    query_docs=query_docs, row_docs=row_docs, dlse=dlse, need=ctx.needs_input_grad[:2])
         return (dq, dbias) + (None,) * 7
 
 
