@@ -408,12 +408,15 @@ mdh_status mdh_linear_set_expired(void);
  *   elements share one float32 scale, scales [slots][ceil(width / group)];
  *   an element reads back as code * scale.  Writing takes the group's
  *   largest magnitude a: scale = a * (1 / 127), code = round(x * (127 * (1 /
- *   a))), each operation rounded to float32, halves to even.  a < 2^-100 stores zeros; a group
- *   with an infinity or NaN reads back as NaN throughout.
+ *   a))), each operation rounded to float32, halves to even.  a < 2^-100
+ *   stores zeros; a group with an infinity or NaN reads back as NaN throughout.
  *   code 1, uint8: one affine map for the cache: code = round((x - lo) *
  *   (1 / step)) limited to [0, 255] (NaN to 0), read back as lo + step *
- *   code; lo, step, 1 / step and each result are rounded to float32.  These codes are a corpus of the exact u8 search: its distances
- *   times step^2 are the distances of the rows as read back.
+ *   code; lo, step, 1 / step and each result are rounded to float32.  These
+ *   codes are a corpus of the exact u8 search, whose distances times step^2 are
+ *   the distances of the rows as read back.  mdh_index_create_u8_device takes
+ *   rows that lie side by side: codes with stride > width are copied to such
+ *   rows first.
  * width <= 65536, slots < 2^31. */
 typedef struct {
     void* codes;

@@ -300,3 +300,30 @@ def test_attend_forms_the_bias_gradient_where_it_is_needed(monkeypatch):
     assert [[a[k] != 0 for k in (6, 7)] for a in calls] == [[True, False], [True, True], [True, False]]
 
 
+# ------------------------------------------------------------------ a cache as a corpus
+@pytest.mark.parametrize("width", [100, 128])
+def test_codes_side_by_side_are_a_corpus(width):
+    """The codes of a cache as the corpus of a device index, copied to rows side by side where the cache pads them; the
+    ids found are those of the codes."""
+    L = capi()
+    n, asked, k = 5000, 40, 8
+    cache = memory.RowCache.empty(n, width, code="uint8", lo=-3.0, step=6 / 255)
+    cache.write(torch.arange(n, device="cuda"), rand(1, n, width))
+    assert cache.codes.is_contiguous() == (width % 16 == 0)
+    corpus = cache.codes.contiguous()
+    queries = corpus[::n // asked][:asked].contiguous()
+    torch.cuda.synchronize()
+    index = P()
+    assert L.mdh_index_create_u8_device(address(corpus), n, width, 1, 0, ctypes.byref(index)) == 0, L.mdh_last_error()
+    ids, dist = (torch.full((asked, k), -1, dtype=torch.int32, device="cuda") for _ in range(2))
+    assert L.mdh_search_u8_device(index, address(queries), asked, k, address(ids), address(dist), None, None) == 0, L.mdh_last_error()
+    assert L.mdh_index_destroy(index) == 0
+    far = (queries.double()[:, None] - corpus.double()[None]).square().sum(2)
+    want, at = torch.sort(far, dim=1, stable=True)             # ties go to the lowest id
+    assert torch.equal(ids.long(), at[:, :k]) and torch.equal(dist.double(), want[:, :k])
+    # By distance, the rows found are those that the cache reads back nearest.
+    back = cache.read(ids)
+    asked_back = cache.read(ids[:, :1].contiguous())
+    assert (((back - asked_back).double().square().sum(2) - want[:, :k] * cache.step ** 2).abs() < 1e-3).all()
+
+

@@ -345,7 +345,9 @@ class RowCache:
     elements (a multiple of 16, or 0 for the whole row) share a scale, a
     element stands for code * scale.  codes uint8: one affine map, an element
     stands for lo + step * code; these codes are a corpus of the exact u8
-    search.  :meth:`empty` allocates with the row stride that reads fastest.
+    search.  :meth:`empty` allocates with the row stride that reads fastest, a
+    multiple of 16 bytes; what takes a device pointer and no stride (the C ABI's
+    index over device memory) wants ``codes.contiguous()``.
     """
 
     def __init__(self, codes, scales=None, *, group=0, lo=0.0, step=1.0):
