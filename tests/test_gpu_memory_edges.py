@@ -327,3 +327,17 @@ def test_codes_side_by_side_are_a_corpus(width):
     assert (((back - asked_back).double().square().sum(2) - want[:, :k] * cache.step ** 2).abs() < 1e-3).all()
 
 
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+def test_codes_are_those_that_torch_makes_on_the_gpu(kind):
+    """The definition's products (scale a (1 / 127), inverse 127 (1 / a)) are what torch's quotients compute on a GPU, so
+    a program that quantises its rows itself gets the same codes and scales, bit for bit."""
+    n, width, group = 20_000, 256, 64
+    x = rand(1, n, width, kind=kind, scale=1.7)
+    cache = memory.RowCache.empty(n, width, group=group)
+    cache.write(torch.arange(n, device="cuda"), x)
+    parts = x.float().view(n, -1, group)
+    top = parts.abs().amax(2, keepdim=True)
+    assert torch.equal(cache.scales, (top / 127)[..., 0])
+    assert torch.equal(cache.codes, (parts * (127 / top)).round().to(torch.int8).view(n, width))
+
+

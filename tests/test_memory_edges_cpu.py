@@ -1,9 +1,14 @@
-"""Edges of the operators around the search that need no GPU: sizes at the ends of a call's index arithmetic."""
+"""Edges of the operators around the search that need no GPU: sizes at the ends of a call's index arithmetic, and the
+definitions of the row cache's codes beside one another."""
 import ctypes
+import importlib.util
+import os
 
 import pytest
+import torch
 
-from helpers import capi
+import memory_plain as plain
+from helpers import ROOT, capi
 
 P, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
 SOME = P(4096)  # an address that is checked and never read
@@ -50,3 +55,28 @@ def test_attend_lists_past_the_index_arithmetic():
         at = ctypes.byref(a), ctypes.byref(cache), ctypes.byref(cache)
         assert L.mdh_attend(*at, SOME, SOME, SOME, 2 ** 62, None) == UNSUPPORTED and b"found" in L.mdh_last_error()
         assert L.mdh_attend_backward(*at, SOME, SOME, SOME, None, SOME, 2 ** 62, None) == UNSUPPORTED
+
+
+# ------------------------------------------------------------------ one definition of the codes
+def test_codes_beside_the_plain_and_exact_forms_of_the_cases():
+    """A row's codes and values by the definition (inverse 127 (1 / a) and scale a (1 / 127)) beside the forms that the
+    measured cases carry, which divide: the same codes but where a value lies on a step's edge, scales within one unit."""
+    spec = importlib.util.spec_from_file_location("operators", os.path.join(ROOT, "perf", "operators.py"))
+    operators = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(operators)
+    n, width, group = 400, 96, 32
+    x = torch.randn((n, width), generator=torch.Generator().manual_seed(3)) * 1.7
+    codes, scales = plain.quantise(x, group)
+    want = plain.stands_for(codes, scales, group, 0.0, 1.0).double()
+    ids = torch.arange(n, dtype=torch.int32)
+
+    def case():
+        return dict(slots=n, width=width, write=n, read=n, group=group, code="int8", type="f32", back="f32", rows=x, slot=ids,
+                    ids=ids, codes=torch.zeros((n, width), dtype=torch.int8), scales=torch.zeros((n, 3)), lo=0.0, step=1.0)
+
+    step = scales.double().repeat_interleave(group, 1)
+    for form in (operators._rows_plain, operators._exact_rows):
+        off = (form(case())["back"].double() - want).abs()
+        moved = off > 0.5 * step
+        assert moved.sum() <= 2                                 # about one code in a million
+        assert (off[~moved] <= 2.0 ** -22 * want[~moved].abs()).all()   # a unit of the scale, a rounding of the value

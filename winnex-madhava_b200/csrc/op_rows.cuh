@@ -32,7 +32,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // Scale and inverse of a group with largest magnitude a.  Below 2^-100 the
 // inverse would leave the float range: such groups are stored as zeros.  An
 // infinity or NaN becomes the scale itself with all codes 0, so the group
-// reads back as NaN.
+// reads back as NaN.  Products by an inverse, each rounded, and not quotients
+// rounded once: they are what torch's a / 127 and 127 / a compute on a GPU, so a
+// program that quantises rows there gets the same codes bit for bit.  Against
+// the quotients 4% of the scales move by their last bit (largest relative error
+// 1.06 instead of 0.99 times 2^-24) and 0.8 codes in a million by one.
 __device__ __forceinline__ void group_scale(float a, float& scale, float& inv) {
     const bool finite = a < INFINITY, some = a >= 0x1p-100f;
     scale = !finite ? a : some ? __fmul_rn(a, 1.0f / 127.0f) : 0.0f;
