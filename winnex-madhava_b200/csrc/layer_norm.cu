@@ -35,15 +35,16 @@ constexpr int kWarpsPerBlock = 8;     // rows at a time of a block, warp form
 constexpr int kBlockElems = 16;       // elements of a thread, block form
 constexpr int kMaxWidth = 16384;
 
-// Sums over the `warps` warps of a row that share barrier `id` and red[warps].
-__device__ __forceinline__ float2 row_sums(float2 v, float2* red, int warp, int warps, int id) {
+// Sums over the warps of a row: one warp, or all `warps` of the block, which
+// share red[warps].
+__device__ __forceinline__ float2 row_sums(float2 v, float2* red, int warp, int warps) {
     v.x = warp_sum(v.x);
     v.y = warp_sum(v.y);
     if (warps > 1) {
         const int lane = threadIdx.x & 31;
-        asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(32 * warps) : "memory");  // the previous sums have been read
+        __syncthreads();  // the previous sums have been read
         if (lane == 0) red[warp] = v;
-        asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(32 * warps) : "memory");
+        __syncthreads();
         v = lane < warps ? red[lane] : make_float2(0.0f, 0.0f);
         v.x = warp_sum(v.x);
         v.y = warp_sum(v.y);
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
         for (int p = 0; p < PAIRS; p++) sum = add2(sum, v[p]);
         const float2 s = unpair(sum);
         const float mean =
-            row_sums(make_float2(s.x + s.y, 0.0f), red, threadIdx.x >> 5, WIDE ? nt >> 5 : 1, 0).x / (float)width;
+            row_sums(make_float2(s.x + s.y, 0.0f), red, threadIdx.x >> 5, WIDE ? nt >> 5 : 1).x / (float)width;
         const f32x2 away = pair(-mean, -mean);
         f32x2 sq = 0;
 #pragma unroll
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
         }
         const float2 q = unpair(sq);
         const float var =
-            row_sums(make_float2(q.x + q.y, 0.0f), red, threadIdx.x >> 5, WIDE ? nt >> 5 : 1, 0).x / (float)width;
+            row_sums(make_float2(q.x + q.y, 0.0f), red, threadIdx.x >> 5, WIDE ? nt >> 5 : 1).x / (float)width;
         const float rstd = 1.0f / sqrtf(var + eps);
         if (t == 0) {
             if (mean_out) mean_out[row] = mean;
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 3 : 1)
         copy_commit();
         if (dx) {
             const float2 a = unpair(sg), b = unpair(sgx);
-            const float2 s = row_sums(make_float2(a.x + a.y, b.x + b.y), red + g * warps, t >> 5, warps, 1 + g);
+            const float2 s = row_sums(make_float2(a.x + a.y, b.x + b.y), red, t >> 5, warps);
             const float mg = s.x / (float)width, mgx = s.y / (float)width;
             const f32x2 mg2 = pair(-mg, -mg), mgx2 = pair(-mgx, -mgx);
 #pragma unroll
@@ -353,8 +354,8 @@ __global__ void __launch_bounds__(1024) k_norm_join(const float* __restrict__ pa
     }
 }
 
-// Backward: threads that hold a row, such groups in a block (named barriers 1
-// .. 4 serve those of several warps), and blocks that stay.
+// Backward: threads that hold a row, such groups in a block (of one warp each,
+// or one group of several warps), and blocks that stay.
 int backward_group(int width) { return width <= 1024 ? 32 : (int)round_up(ceil_div(width, kBlockElems), 32); }
 int backward_groups(int width) { return std::max(1, 128 / backward_group(width)); }
 int backward_blocks(int64_t rows, int width) {

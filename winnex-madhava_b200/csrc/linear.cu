@@ -3,6 +3,13 @@
 //
 //   z = x w^T + b,  y = act(z) + residual
 //   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  db = sum_rows dz
+//
+// Two roundings to 16 bits stand between the passes.  dz is an operand of the
+// tensor cores, which take no other type: with it a gradient's relative error
+// is 2.35e-3 in bfloat16 and 2.9e-4 in float16, where rounding the result alone
+// gives 1.65e-3 and 2.1e-4.  z is kept between the passes in the operands' type,
+// as its layer's activations are: 2.41e-3 and 3.0e-4 with both, for half of the
+// memory and of the passes over it (67 MB each at 16,384 x 2,048).
 #include <algorithm>
 
 #include "product.h"

@@ -6,16 +6,16 @@
 // k-major (k contiguous: rows of 128 bytes in shared memory) or row-major in
 // its other index (64 x 64 boxes whose 128-byte rows run along m or n), so
 // the layer's product and both of its gradients read x, w and dy as they lie
-// in memory.  Warps 0-7 are the epilogue (tensor-memory lane quarter w % 4,
-// half of the columns each), warp 8 issues the TMA loads, warp 9 the MMAs;
-// two accumulators let an epilogue overlap the next tile's products.  A
-// product with few tiles and a long k is split over k: the parts are written
-// in float32 and joined in order by a second kernel.  Every mbarrier wait is
-// bounded; one that gives up is reported once, by the device's next product or
-// by mdh_linear_status.  16,384 x 768 x
-// 2,048 bf16 on B200: 46-49 us for a gradient's product (1.05-1.1 PFLOP/s; its
-// 384 tiles fill 148 SMs to 86%, and 48 KB of operands a block of k come from
-// L2), 63 us for the forward one with GELU, z and y in its epilogue.
+// in memory.  Warps 0-15 are the epilogue (tensor-memory lane quarter w % 4,
+// columns by w / 4), warp 16 issues the TMA loads, warp 17 the MMAs; two
+// accumulators let an epilogue overlap the next tile's products.  A product
+// with few tiles and a long k is split over k: the parts are written in float32
+// and joined in order by a second kernel.  Every mbarrier wait is bounded; one
+// that gives up is reported once, by the device's next product or by
+// mdh_linear_status.  16,384 x 768 x 2,048 bf16 on B200: 46-49 us for a
+// gradient's product (1.05-1.1 PFLOP/s; its 384 tiles fill 148 SMs to 86%, and
+// 48 KB of operands a block of k come from L2), 63 us for the forward one with
+// GELU, z and y in its epilogue.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
