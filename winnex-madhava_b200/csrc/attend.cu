@@ -28,7 +28,7 @@
 // joined in the block, ranges of other blocks by a second kernel, in a fixed
 // order.  On B200: 4,096 queries x 100 entries (a quarter visible) x 12 heads
 // of 64 in 82 us, bound by instructions; 2,048 queries x 64 entries x 12 heads
-// on 4 in 47 us forward, 66 + 9 us backward; 8 queries x 4,096 entries x 16
+// on 4 in 49 us forward, 67 + 9 us backward; 8 queries x 4,096 entries x 16
 // heads of 128 on 2 in 19 + 4 us by the matrix form (36 + 5 us by lanes).
 //
 // Codes become floats without a conversion instruction: the byte c + 128 in
@@ -1279,8 +1279,8 @@ AttendParams check_attend(const mdh_attend_args* a, const mdh_rows* keys, const 
     p.k = code_view(k);
     p.v = code_view(v);
     // The matrix form takes heads of 32 .. 128 that start on 16 bytes and have one scale each.  Its time hardly
-    // depends on how many heads share a row (256 queries x 1,000 x 4 heads of 64: 60 us for 2 .. 8; by lanes 81, 96,
-    // 112 and 206).  Short lists of many queries are bound by what comes before and after the entries, which the
+    // depends on how many heads share a row (256 queries x 1,000 x 4 heads of 64, shared by 2, 3, 4, 8: 58 us in
+    // float16, 62 in bfloat16, 66 in float32; by lanes 81, 96, 112 and 206).  Short lists of many queries are bound by what comes before and after the entries, which the
     // lanes do for several units at once (2,048 queries x 64 entries, shared by 2, 3, 4, 8: 43 us against 34, 46, 54
     // and 99); a head of its own gains nothing.
     auto one_scale = [&](const RowsView& c) { return c.affine || c.n_groups == 1 || c.group % a->head == 0; };

@@ -17,8 +17,10 @@
 // A row belongs to one warp up to 1024 elements (its sums are shuffles), to a
 // group of warps beyond, 16 elements a thread; weights, and backward the
 // running sums of a thread's columns, stay in registers.  65,536 x 768 bf16 on
-// B200: forward 35 us (5.7 TB/s), backward 60 + 4 us (5.0 TB/s of dy, x and
-// dx); without the ring 55 and 178 us.
+// B200: forward 35.6 us (5.7 TB/s), backward 60.5 + 3.7 us (5.0 TB/s of dy, x
+// and dx); without the ring 55 and 178 us.  x 1,024: 47 us (5.7 TB/s) and 116 +
+// 4 us (3.5 TB/s; 32 elements a lane of x, dy and their sums do not fit its
+// registers).
 #include <algorithm>
 #include <atomic>
 #include <initializer_list>

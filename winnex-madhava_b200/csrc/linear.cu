@@ -23,7 +23,7 @@ using namespace op;
 // column sums of a block's rows.  A lane holds 8 columns, a warp every eighth
 // of the block's rows; the next three are on their way into the thread's own
 // shared memory.  Bound by memory, three passes over [rows][n]: 16,384 x 2,048
-// with GELU 36 us on B200 (5.6 TB/s; 61 us without the copies ahead).
+// with GELU 38 us on B200 (5.3 TB/s; 61 us without the copies ahead).
 constexpr int kSlopeRows = 64, kSlopeStages = 4;
 // 8 16-bit elements as they lie in memory, zeros past `left`.
 template <class T>

@@ -12,10 +12,10 @@
 // with few tiles and a long k is split over k: the parts are written in float32
 // and joined in order by a second kernel.  Every mbarrier wait is bounded; one
 // that gives up is reported once, by the device's next product or by
-// mdh_linear_status.  16,384 x 768 x 2,048 bf16 on B200: 46-49 us for a
-// gradient's product (1.05-1.1 PFLOP/s; its 384 tiles fill 148 SMs to 86%, and
-// 48 KB of operands a block of k come from L2), 63 us for the forward one with
-// GELU, z and y in its epilogue.
+// mdh_linear_status.  16,384 x 768 x 2,048 bf16 on B200: 48 and 50 us
+// for the gradients' products (1.04-1.07 PFLOP/s; their 384 tiles fill 148 SMs
+// to 86%, and 48 KB of operands a block of k come from L2), 65 us for the
+// forward one with GELU, z and y in its epilogue.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
